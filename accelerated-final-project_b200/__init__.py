@@ -6,6 +6,7 @@ loading fails when the shared library has not been built.
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # B200ATTN_LIB names another build of the same library (a profiling build, an older build to compare with)
@@ -37,6 +38,55 @@ class Args(C.Structure):
 
 
 _ARGS_SIZE = C.sizeof(Args)
+
+
+def _with_views(*fields):
+    """Field list of a b200attn_*_args: a bare name is a b200attn_view (pointer and strides of sequence, head and row)."""
+    out = [("struct_size", C.c_size_t)]
+    for f in fields:
+        out += [(f, C.c_void_p), (f + "_b", C.c_longlong), (f + "_h", C.c_longlong), (f + "_l", C.c_longlong)] if isinstance(f, str) else [f]
+    return out
+
+
+class AttendArgs(C.Structure):
+    _fields_ = _with_views("Q", "K", "V", "Kd", "Vd", "out", ("lse", C.c_void_p), ("length", C.c_void_p), ("mask", C.c_void_p),
+                           ("mask_stride_b", C.c_longlong), ("batch_sz", C.c_int), ("num_heads", C.c_int), ("num_kv_heads", C.c_int),
+                           ("len_new", C.c_int), ("capacity", C.c_int), ("head_d", C.c_int), ("dtype", C.c_int), ("scale", C.c_float),
+                           ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p), ("flags", C.c_uint))
+
+
+class CommitArgs(C.Structure):
+    _fields_ = _with_views("K", "V", "Kd", "Vd", ("length", C.c_void_p), ("length_out", C.c_void_p), ("accepted", C.c_void_p),
+                           ("max_accepted", C.c_int), ("weights", C.c_void_p), ("pos", C.c_void_p), ("next_pos", C.c_void_p),
+                           ("batch_sz", C.c_int), ("num_kv_heads", C.c_int), ("len_new", C.c_int), ("capacity", C.c_int), ("head_d", C.c_int),
+                           ("dtype", C.c_int), ("stream", C.c_void_p), ("flags", C.c_uint))
+
+
+class WeightsArgs(C.Structure):
+    _fields_ = _with_views("Q", "K", ("length", C.c_void_p), ("lse", C.c_void_p), ("accepted", C.c_void_p), ("max_accepted", C.c_int),
+                           ("weights", C.c_void_p), ("batch_sz", C.c_int), ("num_heads", C.c_int), ("num_kv_heads", C.c_int),
+                           ("len_new", C.c_int), ("capacity", C.c_int), ("head_d", C.c_int), ("dtype", C.c_int), ("scale", C.c_float),
+                           ("stream", C.c_void_p), ("flags", C.c_uint))
+
+
+class EvictArgs(C.Structure):
+    _fields_ = _with_views("K", "V", ("weights", C.c_void_p), ("pos", C.c_void_p), ("length", C.c_void_p), ("next_pos", C.c_void_p),
+                           ("length_out", C.c_void_p), ("kept", C.c_void_p), ("keep", C.c_int), ("sink", C.c_int), ("recent", C.c_int),
+                           "K_out", "V_out", ("weights_out", C.c_void_p), ("pos_out", C.c_void_p), ("capacity_out", C.c_int),
+                           ("batch_sz", C.c_int), ("num_kv_heads", C.c_int), ("capacity", C.c_int), ("head_d", C.c_int), ("dtype", C.c_int),
+                           ("stream", C.c_void_p), ("flags", C.c_uint))
+
+
+def _packer(cls):
+    """Fills a `cls` from values in the order of its fields, as bytes (a tenth of the time that ctypes takes to fill the structure)."""
+    code = {C.c_size_t: "N", C.c_void_p: "P", C.c_longlong: "q", C.c_int: "i", C.c_float: "f", C.c_uint: "I"}
+    packed = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    size = C.sizeof(cls)
+    tail = bytes(size - packed.size)   # the structure's own alignment
+    return lambda *values: packed.pack(size, *values) + tail
+
+
+_pack_attend, _pack_commit, _pack_weights, _pack_evict = (_packer(c) for c in (AttendArgs, CommitArgs, WeightsArgs, EvictArgs))
 
 
 class B200AttnError(RuntimeError):
@@ -89,6 +139,11 @@ def lib():
         L.b200attn_synth_fill.restype = C.c_int
         L.b200attn_rope_k.argtypes = [C.c_void_p, C.c_void_p] + [C.c_int] * 7 + [C.c_float, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
         L.b200attn_rope_k.restype = C.c_int
+        for name in ("attend", "commit", "weights", "evict"):
+            getattr(L, "b200attn_cache_" + name).argtypes = [C.c_char_p]   # a filled structure's bytes
+            getattr(L, "b200attn_cache_" + name).restype = C.c_int
+        L.b200attn_cache_attend_workspace.argtypes = [C.c_char_p]
+        L.b200attn_cache_attend_workspace.restype = C.c_size_t
         L.b200attn_set_option.argtypes = [C.c_int, C.c_longlong]
         L.b200attn_set_option.restype = C.c_int
         L.b200attn_debug_kernel_times.argtypes = [C.c_int, C.POINTER(C.c_double)]
@@ -210,6 +265,197 @@ def rope_k(X, out=None, pairing=PE_ROPE_INTERLEAVED, rotary_dim=0, rope_base=0.0
                                     rope_base, pos0, cos_cache.data_ptr() if cos_cache is not None else None,
                                     sin_cache.data_ptr() if sin_cache is not None else None, stream))
     return out
+
+
+# ---- a key/value cache ----------------------------------------------------------------------------------------------
+
+_INVALID_ARG = 1
+
+
+def _refuse(message):
+    raise B200AttnError(_INVALID_ARG, message)
+
+
+def _view(t, name, shape, dtype, dev):
+    """(address, strides of sequence, head and row) of a [B, heads, rows, D] tensor, after its checks."""
+    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 4:
+        _refuse(f"{name} must be a 4-dimensional {dtype} tensor on device {dev}")
+    if t.shape != shape:
+        _refuse(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    sb, sh, sl, sd = t.stride()
+    if sd != 1 and shape[3] != 1:
+        _refuse(f"the last dimension of {name} must be contiguous")
+    return t.data_ptr(), sb, sh, sl
+
+
+def _dense(t, name, shape, dtype, dev):
+    """Address of a dense tensor (0 for None), after its checks."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on device {dev}")
+    return t.data_ptr()
+
+
+def _cache_shape(K):
+    torch = _torch or _with_torch()
+    if not K.is_cuda or K.dim() != 4 or K.dtype not in _DTYPES:
+        _refuse("the cache must be a 4-dimensional float32, bfloat16 or float16 CUDA tensor [B, heads, rows, D]")
+    return torch, K.get_device(), K.shape
+
+
+def _call_on(dev, fn, packed):
+    torch = _torch
+    if dev == torch.cuda.current_device():
+        status = fn(packed)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(packed)
+    if status != OK:
+        check(status)
+
+
+def _elsewhere(stream, dev):
+    """The stream to allocate on and to enter where `stream` is given and is not the current one, else None: memory that torch hands out belongs to
+    the stream that was current then, and may be handed out again as soon as that stream is done with it."""
+    torch = _torch
+    if stream is None or stream == torch._C._cuda_getCurrentRawStream(dev):
+        return None
+    return torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+
+
+_attend_ws = {}   # bytes of workspace by the sizes they depend on
+
+
+def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=None, lse=None, stream=None, flags=0):
+    """Attention of T new tokens, Q [B, Hq, T, D], over the first length[b] rows of a cache K, V [B, Hkv, S, D] and over the new tokens' own Kd, Vd
+    [B, Hkv, T, D] where mask [B or 1, T, T] (uint8 or bool) is not 0; without a mask token t sees the tokens u <= t; without Kd and Vd the cache alone
+    (an encoder's states).  Tensors may be views whose last dimension is contiguous.  Returns (out [B, Hq, T, D], lse [B, Hq, T] float32)
+    (b200attn_cache_attend).  The workspace comes from torch's allocator: calls on different streams do not share it."""
+    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
+    at = _elsewhere(stream, dev)
+    if at is not None:
+        with torch.cuda.stream(at):
+            return cache_attend(Q, K, V, length, Kd, Vd, mask, scale, out, lse, None, flags)
+    if Q.dim() != 4 or not Q.is_cuda:
+        _refuse("Q must be a 4-dimensional CUDA tensor [B, heads, new tokens, D]")
+    Hq, T = Q.shape[1], Q.shape[2]
+    dtype, q_shape = K.dtype, (B, Hq, T, D)
+    if out is None:
+        out = torch.empty_like(Q)
+    if lse is None:
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=Q.device)
+    if (Kd is None) != (Vd is None):
+        _refuse("Kd and Vd must be given together")
+    none = (0, 0, 0, 0)
+    mask_at = mask_b = 0
+    if mask is not None:
+        if mask.dtype not in (torch.uint8, torch.bool) or mask.get_device() != dev or not mask.is_contiguous() or \
+                tuple(mask.shape) not in ((B, T, T), (1, T, T), (T, T)):
+            _refuse(f"mask must be a contiguous uint8 or bool tensor of shape {(B, T, T)}, {(1, T, T)} or {(T, T)} on device {dev}")
+        mask_at, mask_b = mask.data_ptr(), T * T if mask.dim() == 3 and mask.shape[0] == B else 0
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    L = _lib or lib()
+    head = _view(Q, "Q", q_shape, dtype, dev) + _view(K, "K", K.shape, dtype, dev) + _view(V, "V", K.shape, dtype, dev) + \
+        (none + none if Kd is None else _view(Kd, "Kd", (B, Hkv, T, D), dtype, dev) + _view(Vd, "Vd", (B, Hkv, T, D), dtype, dev)) + \
+        _view(out, "out", q_shape, dtype, dev) + (_dense(lse, "lse", (B, Hq, T), torch.float32, dev),
+                                                  _dense(length, "length", (B,), torch.int32, dev), mask_at, mask_b,
+                                                  B, Hq, Hkv, T, S, D, _DTYPES[dtype], scale)
+    # the size goes by shapes, alignment and the device: kept per combination of them, it costs no second call
+    key = (dev, dtype, B, Hq, Hkv, T, S, D, Kd is None, mask is None, flags)
+    need = _attend_ws.get(key)
+    if need is None:
+        with torch.cuda.device(dev):
+            need = L.b200attn_cache_attend_workspace(_pack_attend(*head, 0, 0, 0, flags))
+        if need == 0:
+            _refuse(L.b200attn_last_error().decode())
+        if len(_attend_ws) >= 4096:
+            _attend_ws.clear()
+        _attend_ws[key] = need
+    ws = torch.empty(need, dtype=torch.uint8, device=Q.device)
+    _call_on(dev, L.b200attn_cache_attend, _pack_attend(*head, ws.data_ptr(), need, stream, flags))
+    return out, lse
+
+
+def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, next_pos=None, stream=None, flags=0):
+    """The accepted ones of T new tokens (accepted [B, A] int32, padded with -1; None: all) become rows of the cache from row length[b] on:
+    K, V [B, Hkv, S, D] are written from Kd, Vd [B, Hkv, T, D], weights [B, Hkv, S] with 0, pos [B, Hkv, S] with next_pos[b] + i.  Returns the new
+    lengths [B] (int32); `length` stays (b200attn_cache_commit)."""
+    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
+    at = _elsewhere(stream, dev)
+    if at is not None:
+        with torch.cuda.stream(at):
+            return cache_commit(K, V, length, Kd, Vd, accepted, weights, pos, next_pos, None, flags)
+    if Kd.dim() != 4 or (accepted is not None and accepted.dim() != 2):
+        _refuse("Kd must be [B, heads, new tokens, D] and accepted [B, most accepted tokens]")
+    T, dtype, i32 = Kd.shape[2], K.dtype, torch.int32
+    A = 0 if accepted is None else accepted.shape[1]
+    out = torch.empty((B,), dtype=i32, device=K.device)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    d_shape = (B, Hkv, T, D)
+    packed = _pack_commit(*_view(K, "K", K.shape, dtype, dev), *_view(V, "V", K.shape, dtype, dev), *_view(Kd, "Kd", d_shape, dtype, dev),
+                          *_view(Vd, "Vd", d_shape, dtype, dev), _dense(length, "length", (B,), i32, dev), out.data_ptr(),
+                          _dense(accepted, "accepted", (B, A), i32, dev), A, _dense(weights, "weights", (B, Hkv, S), torch.float32, dev),
+                          _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev), B, Hkv, T, S, D, _DTYPES[dtype],
+                          stream, flags)
+    _call_on(dev, (_lib or lib()).b200attn_cache_commit, packed)
+    return out
+
+
+def cache_weights(Q, K, length, lse, weights, accepted=None, scale=0.0, stream=None, flags=0):
+    """Adds to weights [B, Hkv, S] the attention weight that each cached row had from the accepted tokens, which are the cache's last rows by now:
+    Q [B, Hq, T, D] and lse [B, Hq, T] are those of the cache_attend call, `length` and `accepted` those after and of cache_commit.  Returns
+    `weights` (b200attn_cache_weights)."""
+    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
+    at = _elsewhere(stream, dev)
+    if at is not None:
+        with torch.cuda.stream(at):
+            return cache_weights(Q, K, length, lse, weights, accepted, scale, None, flags)
+    if Q.dim() != 4 or (accepted is not None and accepted.dim() != 2):
+        _refuse("Q must be [B, heads, new tokens, D] and accepted [B, most accepted tokens]")
+    Hq, T, dtype = Q.shape[1], Q.shape[2], K.dtype
+    A = 0 if accepted is None else accepted.shape[1]
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if length is None or lse is None or weights is None:
+        _refuse("length, lse and weights must be given")
+    packed = _pack_weights(*_view(Q, "Q", (B, Hq, T, D), dtype, dev), *_view(K, "K", K.shape, dtype, dev), _dense(length, "length", (B,), torch.int32, dev),
+                           _dense(lse, "lse", (B, Hq, T), torch.float32, dev), _dense(accepted, "accepted", (B, A), torch.int32, dev), A,
+                           _dense(weights, "weights", (B, Hkv, S), torch.float32, dev), B, Hq, Hkv, T, S, D, _DTYPES[dtype], scale, stream, flags)
+    _call_on(dev, (_lib or lib()).b200attn_cache_weights, packed)
+    return weights
+
+
+def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_pos=None, into=None, kept=None, stream=None, flags=0):
+    """Leaves at most `keep` rows in each head of the cache: the tokens of the first `sink` and the last `recent` positions, then the rows of largest
+    weight.  In place, or into another cache (K, V, weights, pos; pos None where `pos` is None).  Returns (kept [B, Hkv, keep] int32: the former index
+    of each row or -1, the new lengths [B]); `length` stays (b200attn_cache_evict)."""
+    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
+    at = _elsewhere(stream, dev)
+    if at is not None:
+        with torch.cuda.stream(at):
+            return cache_evict(K, V, length, weights, keep, sink, recent, pos, next_pos, into, kept, None, flags)
+    dtype, i32, f32 = K.dtype, torch.int32, torch.float32
+    if kept is None:
+        kept = torch.empty((B, Hkv, max(keep, 0)), dtype=i32, device=K.device)
+    out = torch.empty((B,), dtype=i32, device=K.device)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if length is None or weights is None:
+        _refuse("length and weights must be given")
+    target, So = (0,) * 10, 0
+    if into is not None:
+        Ko, Vo, Wo, Po = into
+        if Ko.dim() != 4 or Wo is None or (Po is None) != (pos is None):
+            _refuse("`into` must be (K, V, weights, pos), with pos where this cache has one")
+        So = Ko.shape[2]
+        o_shape = (B, Hkv, So, D)
+        target = _view(Ko, "K of `into`", o_shape, dtype, dev) + _view(Vo, "V of `into`", o_shape, dtype, dev) + (
+            _dense(Wo, "weights of `into`", (B, Hkv, So), f32, dev), _dense(Po, "pos of `into`", (B, Hkv, So), i32, dev))
+    packed = _pack_evict(*_view(K, "K", K.shape, dtype, dev), *_view(V, "V", K.shape, dtype, dev), _dense(weights, "weights", (B, Hkv, S), f32, dev),
+                         _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(length, "length", (B,), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev),
+                         out.data_ptr(), _dense(kept, "kept", (B, Hkv, max(keep, 0)), i32, dev), keep, sink, recent, *target, So, B, Hkv, S, D,
+                         _DTYPES[dtype], stream, flags)
+    _call_on(dev, (_lib or lib()).b200attn_cache_evict, packed)
+    return kept, out
 
 
 def set_option(option, value):

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/b200attn.h"
+#include "host.h"
 #include "splitd.cuh"
 #include "splitd_tc.cuh"
 #include "splitd_stream.cuh"
@@ -33,7 +34,7 @@ static thread_local std::string t_last_error;
 static thread_local const char *t_last_path = "";
 static std::atomic<unsigned long long> g_launches{0};
 
-static int fail(int status, const char *fmt, ...) {
+int fail(int status, const char *fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -131,6 +132,8 @@ struct DeviceCtx {
     TcTables tc_tables;            // positional-encoding tables of the tensor-core path
     TcwScratch tcw;                // scratch of the wide-head tensor-core path
     F32Scratch f32;                // scratch of the fp32 path for longer sequences
+    void *ws = nullptr;            // workspace of b200attn_cache_attend calls that bring none
+    size_t ws_bytes = 0;
 };
 static DeviceCtx g_ctx[kMaxDevices];
 
@@ -672,6 +675,22 @@ static int check_kernel_errors(DeviceCtx &c, cudaStream_t st, bool sync) {
     return report_kernel_errors(c, "kernel");
 }
 
+// The call is made to wait, on the device, for everything enqueued so far on the stream of the device's previous call.
+static int order_after_last(DeviceCtx &c, cudaStream_t st) {
+    if (c.have_last_stream && c.last_stream != st) {
+        if (!c.last_event) CU_TRY(cudaEventCreateWithFlags(&c.last_event, cudaEventDisableTiming));
+        cudaError_t e = cudaEventRecord(c.last_event, c.last_stream);
+        if (e == cudaSuccess) e = cudaStreamWaitEvent(st, c.last_event, 0);
+        if (e != cudaSuccess) {   // the earlier stream is gone or unusable: order by waiting for the device
+            (void)cudaGetLastError();
+            CU_TRY(cudaDeviceSynchronize());
+        }
+    }
+    c.last_stream = st;
+    c.have_last_stream = true;
+    return B200ATTN_OK;
+}
+
 // `n` > 1: the entries a[0 .. n) are independent problems that one launch may take (batch_group); -1 when it does not.
 static int forward_device(const b200attn_args *a, bool independent_of_prev = false, bool batched = false, int n = 1) {
     int rd; float base;
@@ -687,17 +706,7 @@ static int forward_device(const b200attn_args *a, bool independent_of_prev = fal
         cudaDeviceSynchronize();   // let the failed work drain before the scratch is cleaned
         return report_kernel_errors(*c, "an earlier asynchronous call");
     }
-    if (c->have_last_stream && c->last_stream != st) {
-        if (!c->last_event) CU_TRY(cudaEventCreateWithFlags(&c->last_event, cudaEventDisableTiming));
-        cudaError_t e = cudaEventRecord(c->last_event, c->last_stream);
-        if (e == cudaSuccess) e = cudaStreamWaitEvent(st, c->last_event, 0);
-        if (e != cudaSuccess) {   // the earlier stream is gone or unusable: order by waiting for the device
-            (void)cudaGetLastError();
-            CU_TRY(cudaDeviceSynchronize());
-        }
-    }
-    c->last_stream = st;
-    c->have_last_stream = true;
+    if ((rc = order_after_last(*c, st))) return rc;
     if (n > 1) {
         c->prev_sdtc = false;
         return run_sw(*c, a, n, rd, base, st);
@@ -855,6 +864,50 @@ static int batch_group(const b200attn_args *a, int n, int *run) {
                 return m;
     }
     return g;
+}
+
+void count_launches(unsigned long long n) { g_launches.fetch_add(n); }
+void set_last_path(const char *name) { t_last_path = name; }
+
+int host_begin(HostCall *h) {
+    DeviceCtx *c;
+    int rc = get_ctx(&c, &h->dev);
+    if (rc) return rc;
+    h->sm_count = c->sm_count;
+    h->max_smem = c->max_smem_optin;
+    h->err_dev = c->err_dev; h->err_sys = c->err_host_dev;
+    h->spin_limit = current_spin_limit();
+    if (*reinterpret_cast<volatile unsigned *>(c->err_host) != 0) {
+        std::lock_guard<std::mutex> lk(c->mu);
+        cudaDeviceSynchronize();
+        return report_kernel_errors(*c, "an earlier asynchronous call");
+    }
+    return B200ATTN_OK;
+}
+
+int host_workspace(HostCall *h, size_t bytes, cudaStream_t st, void **ws) {
+    DeviceCtx &c = g_ctx[h->dev];
+    h->lock = std::unique_lock<std::mutex>(c.mu);
+    int rc = order_after_last(c, st);
+    if (rc) return rc;
+    c.prev_sdtc = false;
+    if (bytes > c.ws_bytes) {
+        if (c.ws) CU_TRY(cudaFree(c.ws));
+        c.ws = nullptr; c.ws_bytes = 0;
+        CU_TRY(cudaMalloc(&c.ws, bytes));
+        c.ws_bytes = bytes;
+    }
+    *ws = c.ws;
+    return B200ATTN_OK;
+}
+
+int host_end(HostCall *h, cudaStream_t st, bool async) {
+    if (h->lock.owns_lock()) h->lock.unlock();
+    if (async) return B200ATTN_OK;
+    CU_TRY(cudaStreamSynchronize(st));
+    DeviceCtx &c = g_ctx[h->dev];
+    std::lock_guard<std::mutex> lk(c.mu);
+    return report_kernel_errors(c, "kernel");
 }
 
 static int ensure_stage(DeviceCtx &c, int i, size_t bytes) {
@@ -1238,6 +1291,8 @@ void b200attn_release_workspace(void) {
         if (c.sw_S) cudaFree(c.sw_S);
         if (c.sw_cnt) cudaFree(c.sw_cnt);
         c.sw_S = nullptr; c.sw_cnt = nullptr;
+        if (c.ws) cudaFree(c.ws);
+        c.ws = nullptr; c.ws_bytes = 0;
         c.prev_sdtc = false;
     }
     cudaSetDevice(prev);

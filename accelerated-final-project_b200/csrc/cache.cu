@@ -1,0 +1,331 @@
+// Entry points of the key/value cache (include/b200attn.h, "A key/value cache"): checks of the arguments, choice of the kernel, launches.
+#include <cmath>
+#include <cstring>
+
+#include "host.h"
+#include "cache.cuh"
+
+namespace b200attn {
+namespace {
+
+#define CU_TRY(expr)                                                                                  \
+    do {                                                                                              \
+        cudaError_t e_ = (expr);                                                                      \
+        if (e_ != cudaSuccess)                                                                        \
+            return fail(B200ATTN_ERR_CUDA, "CUDA error %d (%s) at %s:%d: %s", (int)e_,                \
+                        cudaGetErrorString(e_), __FILE__, __LINE__, #expr);                           \
+    } while (0)
+
+size_t esize(int dtype) { return dtype == B200ATTN_F32 ? 4 : 2; }
+
+int check_dtype(int dtype) {
+    if (dtype != B200ATTN_F32 && dtype != B200ATTN_BF16 && dtype != B200ATTN_F16) return fail(B200ATTN_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+    return B200ATTN_OK;
+}
+
+int check_view(const char *name, const b200attn_view &v, int dtype) {
+    if (v.ptr == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be non-NULL", name);
+    if ((uintptr_t)v.ptr & (esize(dtype) - 1)) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be aligned to the element size", name);
+    if (v.stride_b < 0 || v.stride_h < 0 || v.stride_l < 0) return fail(B200ATTN_ERR_INVALID_ARG, "strides of %s must not be negative", name);
+    return B200ATTN_OK;
+}
+
+// The bytes from a view's first element to behind its last.
+size_t extent(const b200attn_view &v, long long B, long long H, long long L, long long D, int dtype) {
+    return (size_t)((B - 1) * v.stride_b + (H - 1) * v.stride_h + (L - 1) * v.stride_l + D) * esize(dtype);
+}
+bool meet(const void *a, size_t na, const void *b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
+
+// What is written: rows of a view must not share elements (the dimensions, sorted by stride, each have to clear what is inside them).
+int check_written(const char *name, const b200attn_view &v, long long B, long long H, long long L, long long D) {
+    long long n[3] = {B, H, L}, s[3] = {v.stride_b, v.stride_h, v.stride_l}, inside = D;
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (s[j] < s[i]) { long long t = s[i]; s[i] = s[j]; s[j] = t; t = n[i]; n[i] = n[j]; n[j] = t; }
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        if (s[i] < inside) return fail(B200ATTN_ERR_INVALID_ARG, "rows of %s, which is written, overlap each other", name);
+        inside = s[i] * (n[i] - 1) + inside;
+    }
+    return B200ATTN_OK;
+}
+
+CaView strides(const b200attn_view &v, long long unit = 1) { return CaView{v.stride_b * unit, v.stride_h * unit, v.stride_l * unit}; }
+bool aligned16(const b200attn_view &v, int dtype) {
+    const long long e = (long long)esize(dtype);
+    return (((uintptr_t)v.ptr | (uintptr_t)(v.stride_b * e) | (uintptr_t)(v.stride_h * e) | (uintptr_t)(v.stride_l * e)) & 15) == 0;
+}
+
+int raise_smem(const void *kern, size_t bytes) {
+    if (bytes > 48 * 1024) CU_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return B200ATTN_OK;
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------
+int validate(const b200attn_attend_args *a, bool pointers) {
+    if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
+    if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
+    if (a->batch_sz <= 0 || a->num_heads <= 0 || a->num_kv_heads <= 0 || a->len_new <= 0 || a->capacity <= 0 || a->head_d <= 0)
+        return fail(B200ATTN_ERR_INVALID_ARG, "batch_sz, num_heads, num_kv_heads, len_new, capacity, head_d must be positive (got %d,%d,%d,%d,%d,%d)", a->batch_sz,
+                    a->num_heads, a->num_kv_heads, a->len_new, a->capacity, a->head_d);
+    int rc = check_dtype(a->dtype);
+    if (rc) return rc;
+    if (a->num_heads % a->num_kv_heads) return fail(B200ATTN_ERR_INVALID_ARG, "num_heads (%d) must be a multiple of num_kv_heads (%d)", a->num_heads, a->num_kv_heads);
+    if (a->head_d > CA_MAX_D) return fail(B200ATTN_ERR_INVALID_ARG, "head_d must be at most %d (got %d)", CA_MAX_D, a->head_d);
+    if ((long long)a->len_new * (a->num_heads / a->num_kv_heads) > (1ll << 30))
+        return fail(B200ATTN_ERR_TOO_LARGE, "len_new times the query heads of a key head is %lld, at most 2^30 are taken", (long long)a->len_new * (a->num_heads / a->num_kv_heads));
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");
+    if ((a->Kd.ptr == nullptr) != (a->Vd.ptr == nullptr)) return fail(B200ATTN_ERR_INVALID_ARG, "Kd and Vd must be given together");
+    if (a->mask && a->Kd.ptr == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "a mask needs Kd and Vd");
+    if (a->mask && a->mask_stride_b != 0 && a->mask_stride_b != (long long)a->len_new * a->len_new)
+        return fail(B200ATTN_ERR_INVALID_ARG, "mask_stride_b must be 0 or len_new * len_new");
+    if (!pointers) return B200ATTN_OK;
+    if ((rc = check_view("Q", a->Q, a->dtype)) || (rc = check_view("K", a->K, a->dtype)) || (rc = check_view("V", a->V, a->dtype)) || (rc = check_view("out", a->out, a->dtype)))
+        return rc;
+    if (a->Kd.ptr && ((rc = check_view("Kd", a->Kd, a->dtype)) || (rc = check_view("Vd", a->Vd, a->dtype)))) return rc;
+    const long long B = a->batch_sz, Hq = a->num_heads, Hkv = a->num_kv_heads, T = a->len_new, S = a->capacity, D = a->head_d;
+    if ((rc = check_written("out", a->out, B, Hq, T, D))) return rc;
+    if (!a->length) return fail(B200ATTN_ERR_INVALID_ARG, "length must be non-NULL");
+    if (((uintptr_t)a->length | (uintptr_t)a->lse) & 3) return fail(B200ATTN_ERR_INVALID_ARG, "length and lse must be aligned to 4 bytes");
+    const size_t no = extent(a->out, B, Hq, T, D, a->dtype);
+    if (meet(a->out.ptr, no, a->Q.ptr, extent(a->Q, B, Hq, T, D, a->dtype)) || meet(a->out.ptr, no, a->K.ptr, extent(a->K, B, Hkv, S, D, a->dtype)) ||
+        meet(a->out.ptr, no, a->V.ptr, extent(a->V, B, Hkv, S, D, a->dtype)) ||
+        (a->Kd.ptr && (meet(a->out.ptr, no, a->Kd.ptr, extent(a->Kd, B, Hkv, T, D, a->dtype)) || meet(a->out.ptr, no, a->Vd.ptr, extent(a->Vd, B, Hkv, T, D, a->dtype)))))
+        return fail(B200ATTN_ERR_INVALID_ARG, "out must not overlap an input");
+    return B200ATTN_OK;
+}
+
+// Workspace: the slots of cut units, then the entries.
+size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + (size_t)p.grid * 8 * sizeof(int); }
+
+void share_out(CaParams &p, int RT, int TK, int grid) {
+    p.RT = RT; p.TK = TK; p.grid = grid;
+    p.nrt = (p.R + RT - 1) / RT;
+    p.DT = 0;
+    if (p.drafts)
+        for (int rt = 0; rt < p.nrt; ++rt) p.DT += ca_draft_tiles(rt, p.R, RT, p.G, p.T, TK, p.mask == nullptr);
+}
+
+void fill(CaParams &p, const b200attn_attend_args &a) {
+    p.Q = a.Q.ptr; p.K = a.K.ptr; p.V = a.V.ptr; p.Kd = a.Kd.ptr; p.Vd = a.Vd.ptr; p.O = a.out.ptr;
+    p.q = strides(a.Q); p.k = strides(a.K); p.v = strides(a.V); p.kd = strides(a.Kd); p.vd = strides(a.Vd); p.o = strides(a.out);
+    p.lse = a.lse; p.len = a.length; p.mask = a.mask; p.mask_b = a.mask_stride_b;
+    p.B = a.batch_sz; p.Hq = a.num_heads; p.Hkv = a.num_kv_heads; p.G = a.num_heads / a.num_kv_heads;
+    p.T = a.len_new; p.S = a.capacity; p.D = a.head_d;
+    p.R = p.T * p.G;
+    p.drafts = a.Kd.ptr != nullptr;
+    p.scale_log2 = (a.scale == 0.0f ? 1.0f / sqrtf((float)a.head_d) : a.scale) * 1.4426950408889634f;
+}
+
+template <typename T, int DB>
+int launch_generic(const CaParams &p, cudaStream_t st) {
+    const size_t smem = cg_smem_bytes(p.D);
+    int rc = raise_smem((const void *)ca_generic_kernel<T, DB>, smem);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_generic_kernel<T, DB>, dim3((unsigned)p.grid), CG_THREADS, smem, 1, st, p));
+    return B200ATTN_OK;
+}
+template <typename T>
+int launch_attend(const CaParams &p, cudaStream_t st) {
+    int rc = p.D <= 64 ? launch_generic<T, 64>(p, st) : p.D <= 128 ? launch_generic<T, 128>(p, st) : launch_generic<T, 256>(p, st);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    count_launches(2);
+    return B200ATTN_OK;
+}
+
+int attend(const b200attn_attend_args *a, size_t *need) {
+    int rc = validate(a, need == nullptr);
+    if (rc) return rc;
+    HostCall c;
+    if ((rc = host_begin(&c))) return rc;
+    cudaStream_t st = (cudaStream_t)a->stream;
+    CaParams p{};
+    fill(p, *a);
+    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    share_out(p, CG_ROWS, CG_KEYS, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
+    const size_t bytes = attend_bytes(p);
+    if (need) { *need = bytes; return B200ATTN_OK; }
+    void *ws = a->workspace;
+    if (ws) {
+        if (a->workspace_bytes < bytes) return fail(B200ATTN_ERR_INVALID_ARG, "workspace_bytes is %zu, this call needs %zu", a->workspace_bytes, bytes);
+        if ((uintptr_t)ws & 15) return fail(B200ATTN_ERR_INVALID_ARG, "workspace must be aligned to 16 bytes");
+    } else if ((rc = host_workspace(&c, bytes, st, &ws))) {
+        return rc;
+    }
+    p.part = (float *)ws;
+    p.entries = (int *)((char *)ws + bytes - (size_t)p.grid * 8 * sizeof(int));
+    rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, st) : launch_attend<__nv_bfloat16>(p, st);
+    if (rc) return rc;
+    set_last_path("cache_generic");
+    return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
+}
+
+// ---- lists of accepted tokens ------------------------------------------------------------------------------------------
+int check_accepted(const int *accepted, int max_accepted) {
+    if (accepted && max_accepted <= 0) return fail(B200ATTN_ERR_INVALID_ARG, "max_accepted must be positive (got %d)", max_accepted);
+    if ((uintptr_t)accepted & 3) return fail(B200ATTN_ERR_INVALID_ARG, "accepted must be aligned to 4 bytes");
+    return B200ATTN_OK;
+}
+int check_grid(int B, int Hkv) {
+    if (B > 65535 || Hkv > 65535) return fail(B200ATTN_ERR_TOO_LARGE, "batch_sz and num_kv_heads must be at most 65535 (got %d, %d)", B, Hkv);
+    return B200ATTN_OK;
+}
+
+int commit(const b200attn_commit_args *a) {
+    if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
+    if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
+    if (a->batch_sz <= 0 || a->num_kv_heads <= 0 || a->len_new <= 0 || a->capacity <= 0 || a->head_d <= 0)
+        return fail(B200ATTN_ERR_INVALID_ARG, "batch_sz, num_kv_heads, len_new, capacity, head_d must be positive (got %d,%d,%d,%d,%d)", a->batch_sz, a->num_kv_heads,
+                    a->len_new, a->capacity, a->head_d);
+    int rc = check_dtype(a->dtype);
+    if (rc || (rc = check_grid(a->batch_sz, a->num_kv_heads))) return rc;
+    if (a->head_d > (1 << 20)) return fail(B200ATTN_ERR_TOO_LARGE, "head_d must be at most 2^20 (got %d)", a->head_d);
+    const long long B = a->batch_sz, H = a->num_kv_heads, T = a->len_new, S = a->capacity, D = a->head_d;
+    if ((rc = check_view("K", a->K, a->dtype)) || (rc = check_view("V", a->V, a->dtype)) || (rc = check_view("Kd", a->Kd, a->dtype)) || (rc = check_view("Vd", a->Vd, a->dtype)) ||
+        (rc = check_written("K", a->K, B, H, S, D)) || (rc = check_written("V", a->V, B, H, S, D)) || (rc = check_accepted(a->accepted, a->max_accepted)))
+        return rc;
+    if (!a->length) return fail(B200ATTN_ERR_INVALID_ARG, "length must be non-NULL");
+    if (((uintptr_t)a->length | (uintptr_t)a->length_out | (uintptr_t)a->weights | (uintptr_t)a->pos | (uintptr_t)a->next_pos) & 3)
+        return fail(B200ATTN_ERR_INVALID_ARG, "length, length_out, weights, pos and next_pos must be aligned to 4 bytes");
+    if (a->length_out && (meet(a->length_out, 4 * B, a->length, 4 * B) || (a->next_pos && meet(a->length_out, 4 * B, a->next_pos, 4 * B))))
+        return fail(B200ATTN_ERR_INVALID_ARG, "length_out must not overlap length or next_pos");
+    const size_t nk = extent(a->K, B, H, S, D, a->dtype), nv = extent(a->V, B, H, S, D, a->dtype), nkd = extent(a->Kd, B, H, T, D, a->dtype), nvd = extent(a->Vd, B, H, T, D, a->dtype);
+    if (meet(a->K.ptr, nk, a->Kd.ptr, nkd) || meet(a->K.ptr, nk, a->Vd.ptr, nvd) || meet(a->V.ptr, nv, a->Kd.ptr, nkd) || meet(a->V.ptr, nv, a->Vd.ptr, nvd))
+        return fail(B200ATTN_ERR_INVALID_ARG, "Kd and Vd must not overlap the cache");
+    HostCall c;
+    if ((rc = host_begin(&c))) return rc;
+    cudaStream_t st = (cudaStream_t)a->stream;
+    const long long e = (long long)esize(a->dtype);
+    CcParams p{};
+    p.K = a->K.ptr; p.V = a->V.ptr; p.Kd = a->Kd.ptr; p.Vd = a->Vd.ptr;
+    p.k = strides(a->K, e); p.v = strides(a->V, e); p.kd = strides(a->Kd, e); p.vd = strides(a->Vd, e);
+    p.len = a->length; p.accepted = a->accepted; p.next_pos = a->next_pos; p.len_out = a->length_out; p.pos = a->pos; p.weights = a->weights;
+    p.A = a->accepted ? a->max_accepted : a->len_new;
+    p.B = a->batch_sz; p.Hkv = a->num_kv_heads; p.T = a->len_new; p.S = a->capacity; p.row_bytes = (int)(D * e);
+    const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && aligned16(a->Kd, a->dtype) && aligned16(a->Vd, a->dtype) && p.row_bytes % 16 == 0;
+    const long long blocks = ((long long)p.A * p.Hkv + CC_THREADS / 32 - 1) / (CC_THREADS / 32);
+    if (blocks > 0x7fffffffll) return fail(B200ATTN_ERR_TOO_LARGE, "%lld rows to commit in a sequence are too many", (long long)p.A * p.Hkv);
+    const dim3 grid((unsigned)blocks, (unsigned)p.B);
+    CU_TRY(wide ? launch_dependent(cc_commit_kernel<uint4>, grid, CC_THREADS, 0, 1, st, p)
+                : e == 4 ? launch_dependent(cc_commit_kernel<uint32_t>, grid, CC_THREADS, 0, 1, st, p) : launch_dependent(cc_commit_kernel<uint16_t>, grid, CC_THREADS, 0, 1, st, p));
+    count_launches(1);
+    return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
+}
+
+template <typename T>
+int launch_weights(const CwParams &p, cudaStream_t st) {
+    const size_t smem = cg_smem_bytes(p.D);
+    int rc = raise_smem((const void *)cw_generic_kernel<T>, smem);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(cw_generic_kernel<T>, dim3((unsigned)((p.S + CG_KEYS - 1) / CG_KEYS), (unsigned)p.Hkv, (unsigned)p.B), CG_THREADS, smem, 1, st, p));
+    count_launches(1);
+    return B200ATTN_OK;
+}
+
+int weights(const b200attn_weights_args *a) {
+    if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
+    if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
+    if (a->batch_sz <= 0 || a->num_heads <= 0 || a->num_kv_heads <= 0 || a->len_new <= 0 || a->capacity <= 0 || a->head_d <= 0)
+        return fail(B200ATTN_ERR_INVALID_ARG, "batch_sz, num_heads, num_kv_heads, len_new, capacity, head_d must be positive (got %d,%d,%d,%d,%d,%d)", a->batch_sz,
+                    a->num_heads, a->num_kv_heads, a->len_new, a->capacity, a->head_d);
+    int rc = check_dtype(a->dtype);
+    if (rc || (rc = check_grid(a->batch_sz, a->num_kv_heads))) return rc;
+    if (a->num_heads % a->num_kv_heads) return fail(B200ATTN_ERR_INVALID_ARG, "num_heads (%d) must be a multiple of num_kv_heads (%d)", a->num_heads, a->num_kv_heads);
+    if (a->head_d > CA_MAX_D) return fail(B200ATTN_ERR_INVALID_ARG, "head_d must be at most %d (got %d)", CA_MAX_D, a->head_d);
+    const int A = a->accepted ? a->max_accepted : a->len_new, G = a->num_heads / a->num_kv_heads;
+    if ((long long)A * G > (1ll << 30)) return fail(B200ATTN_ERR_TOO_LARGE, "accepted tokens times the query heads of a key head are %lld, at most 2^30 are taken", (long long)A * G);
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");
+    if ((rc = check_view("Q", a->Q, a->dtype)) || (rc = check_view("K", a->K, a->dtype)) || (rc = check_accepted(a->accepted, a->max_accepted))) return rc;
+    if (!a->length || !a->lse || !a->weights) return fail(B200ATTN_ERR_INVALID_ARG, "length, lse and weights must be non-NULL");
+    if (((uintptr_t)a->length | (uintptr_t)a->lse | (uintptr_t)a->weights) & 3) return fail(B200ATTN_ERR_INVALID_ARG, "length, lse and weights must be aligned to 4 bytes");
+    HostCall c;
+    if ((rc = host_begin(&c))) return rc;
+    cudaStream_t st = (cudaStream_t)a->stream;
+    CwParams p{};
+    p.Q = a->Q.ptr; p.K = a->K.ptr; p.q = strides(a->Q); p.k = strides(a->K);
+    p.len = a->length; p.accepted = a->accepted; p.lse = a->lse; p.weights = a->weights;
+    p.A = A; p.B = a->batch_sz; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.G = G; p.T = a->len_new; p.S = a->capacity; p.D = a->head_d;
+    p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_d) : a->scale) * 1.4426950408889634f;
+    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    rc = a->dtype == B200ATTN_F32 ? launch_weights<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_weights<__half>(p, st) : launch_weights<__nv_bfloat16>(p, st);
+    if (rc) return rc;
+    set_last_path("cache_generic");
+    return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
+}
+
+int evict(const b200attn_evict_args *a) {
+    if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
+    if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
+    if (a->batch_sz <= 0 || a->num_kv_heads <= 0 || a->capacity <= 0 || a->head_d <= 0)
+        return fail(B200ATTN_ERR_INVALID_ARG, "batch_sz, num_kv_heads, capacity, head_d must be positive (got %d,%d,%d,%d)", a->batch_sz, a->num_kv_heads, a->capacity, a->head_d);
+    int rc = check_dtype(a->dtype);
+    if (rc || (rc = check_grid(a->batch_sz, a->num_kv_heads))) return rc;
+    if (a->head_d > (1 << 20)) return fail(B200ATTN_ERR_TOO_LARGE, "head_d must be at most 2^20 (got %d)", a->head_d);
+    if (a->capacity > B200ATTN_EVICT_MAX_ROWS) return fail(B200ATTN_ERR_TOO_LARGE, "capacity must be at most %d rows (got %d)", B200ATTN_EVICT_MAX_ROWS, a->capacity);
+    if (a->keep < 1 || a->sink < 0 || a->recent < 0 || (long long)a->sink + a->recent > a->keep)
+        return fail(B200ATTN_ERR_INVALID_ARG, "keep must be at least 1 and at least sink + recent, both not negative (got %d, %d, %d)", a->keep, a->sink, a->recent);
+    const bool into = a->K_out.ptr != nullptr;
+    if (into != (a->V_out.ptr != nullptr) || into != (a->weights_out != nullptr) || (a->pos_out != nullptr) != (into && a->pos != nullptr))
+        return fail(B200ATTN_ERR_INVALID_ARG, "K_out, V_out, weights_out and, with pos, pos_out must be given together");
+    if (into && a->capacity_out < (a->keep < a->capacity ? a->keep : a->capacity)) return fail(B200ATTN_ERR_INVALID_ARG, "capacity_out (%d) must be at least keep (%d)", a->capacity_out, a->keep);
+    const long long B = a->batch_sz, H = a->num_kv_heads, S = a->capacity, D = a->head_d, So = a->capacity_out;
+    if ((rc = check_view("K", a->K, a->dtype)) || (rc = check_view("V", a->V, a->dtype)) || (rc = check_written("K", a->K, B, H, S, D)) || (rc = check_written("V", a->V, B, H, S, D)))
+        return rc;
+    if (into && ((rc = check_view("K_out", a->K_out, a->dtype)) || (rc = check_view("V_out", a->V_out, a->dtype)) || (rc = check_written("K_out", a->K_out, B, H, So, D)) ||
+                 (rc = check_written("V_out", a->V_out, B, H, So, D))))
+        return rc;
+    if (!a->length || !a->weights || !a->kept) return fail(B200ATTN_ERR_INVALID_ARG, "length, weights and kept must be non-NULL");
+    if (((uintptr_t)a->length | (uintptr_t)a->length_out | (uintptr_t)a->weights | (uintptr_t)a->pos | (uintptr_t)a->next_pos | (uintptr_t)a->kept | (uintptr_t)a->weights_out |
+         (uintptr_t)a->pos_out) & 3)
+        return fail(B200ATTN_ERR_INVALID_ARG, "length, length_out, weights, pos, next_pos, kept and their counterparts must be aligned to 4 bytes");
+    if (a->length_out && (meet(a->length_out, 4 * B, a->length, 4 * B) || (a->next_pos && meet(a->length_out, 4 * B, a->next_pos, 4 * B))))
+        return fail(B200ATTN_ERR_INVALID_ARG, "length_out must not overlap length or next_pos");
+    if (into) {
+        const size_t nk = extent(a->K, B, H, S, D, a->dtype), nv = extent(a->V, B, H, S, D, a->dtype), nko = extent(a->K_out, B, H, So, D, a->dtype), nvo = extent(a->V_out, B, H, So, D, a->dtype);
+        const size_t nw = (size_t)(4 * B * H * S), nwo = (size_t)(4 * B * H * So);
+        if (meet(a->K.ptr, nk, a->K_out.ptr, nko) || meet(a->K.ptr, nk, a->V_out.ptr, nvo) || meet(a->V.ptr, nv, a->K_out.ptr, nko) || meet(a->V.ptr, nv, a->V_out.ptr, nvo) ||
+            meet(a->weights, nw, a->weights_out, nwo) || (a->pos && meet(a->pos, nw, a->pos_out, nwo)))
+            return fail(B200ATTN_ERR_INVALID_ARG, "the cache that the kept rows go into must not overlap this one");
+    }
+    HostCall c;
+    if ((rc = host_begin(&c))) return rc;
+    cudaStream_t st = (cudaStream_t)a->stream;
+    const long long e = (long long)esize(a->dtype);
+    CeParams p{};
+    p.K = a->K.ptr; p.V = a->V.ptr; p.K_out = a->K_out.ptr; p.V_out = a->V_out.ptr;
+    p.k = strides(a->K, e); p.v = strides(a->V, e); p.ko = strides(a->K_out, e); p.vo = strides(a->V_out, e);
+    p.weights = a->weights; p.weights_out = a->weights_out; p.pos = a->pos; p.pos_out = a->pos_out;
+    p.len = a->length; p.next_pos = a->next_pos; p.len_out = a->length_out; p.kept = a->kept;
+    p.keep = a->keep; p.sink = a->sink; p.recent = a->recent;
+    p.B = a->batch_sz; p.Hkv = a->num_kv_heads; p.S = a->capacity; p.S_out = a->capacity_out; p.row_bytes = (int)(D * e);
+    const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && p.row_bytes % 16 == 0 &&
+                      (!into || (aligned16(a->K_out, a->dtype) && aligned16(a->V_out, a->dtype)));
+    const size_t smem = ce_smem_bytes(p.S);
+    if ((rc = raise_smem((const void *)ce_select_kernel, smem))) return rc;
+    CU_TRY(launch_dependent(ce_select_kernel, dim3((unsigned)p.Hkv, (unsigned)p.B), CE_THREADS, smem, 1, st, p));
+    const int rows = CC_THREADS;   // of `kept` per block
+    const dim3 grid((unsigned)((p.keep + (long long)rows - 1) / rows), (unsigned)p.Hkv, (unsigned)p.B);
+    CU_TRY(wide ? launch_dependent(ce_move_kernel<uint4>, grid, CC_THREADS, 0, 1, st, p)
+                : e == 4 ? launch_dependent(ce_move_kernel<uint32_t>, grid, CC_THREADS, 0, 1, st, p) : launch_dependent(ce_move_kernel<uint16_t>, grid, CC_THREADS, 0, 1, st, p));
+    count_launches(2);
+    return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
+}
+
+}  // namespace
+}  // namespace b200attn
+
+using namespace b200attn;
+
+extern "C" {
+
+int b200attn_cache_attend(const b200attn_attend_args *args) { return attend(args, nullptr); }
+size_t b200attn_cache_attend_workspace(const b200attn_attend_args *args) {
+    size_t need = 0;
+    return attend(args, &need) == B200ATTN_OK ? need : 0;
+}
+int b200attn_cache_commit(const b200attn_commit_args *args) { return commit(args); }
+int b200attn_cache_weights(const b200attn_weights_args *args) { return weights(args); }
+int b200attn_cache_evict(const b200attn_evict_args *args) { return evict(args); }
+
+}  // extern "C"

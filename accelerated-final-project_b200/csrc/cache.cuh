@@ -1,0 +1,712 @@
+// A key/value cache: attention of new tokens over it and its upkeep (include/b200attn.h, "A key/value cache").  This file has the
+// share-out of the attention's work, the kernels that join its parts, the CUDA-core kernels that take every shape, and commit and eviction.
+//
+// Attention, for the rows r = t G + g of a key head (G query heads share it), visible keys j:
+//     s_rj = scale q_r . k_j,   lse_r = log sum_j exp(s_rj),   out_r = sum_j exp(s_rj - lse_r) v_j.
+// One pass over the keys with a running maximum m and sum l: when m grows to m', l and the accumulator are multiplied by exp(m - m').
+// Parts over different keys join by the same rule.
+//
+// Sharing out: a unit is (sequence, key head, tile of RT rows); its items are the tiles of TK cached keys, then those of the new tokens' keys.
+// The lengths are in device memory and differ, so no split can be chosen on the host: the items of all units, one after the other, are cut
+// into equal contiguous ranges, one per CTA, by each CTA for itself (a scan over the lengths).  A unit inside one range is finished there; one
+// that is cut leaves (accumulator, m, l) per row in the CTA's two slots of the workspace - only the first and the last unit of a range can be
+// cut - and ca_combine_kernel joins the parts in the order of their CTAs: no atomics, the same result every time.
+#pragma once
+
+#include "tc_common.cuh"
+
+namespace b200attn {
+
+constexpr int CA_MAX_D = 256;
+
+struct CaView { long long b, h, l; };   // strides in elements
+
+struct CaParams {
+    const void *Q, *K, *V, *Kd, *Vd;
+    void *O;
+    CaView q, k, v, kd, vd, o;
+    float *lse;
+    const int *len;
+    const unsigned char *mask;
+    long long mask_b;
+    int B, Hq, Hkv, G, T, S, D;
+    int R;               // rows of a key head: T * G
+    int RT, nrt, TK;     // rows of a unit, units of a key head, keys of a tile
+    long long DT;        // items of new keys, summed over the units of a key head
+    int drafts;          // new keys are given
+    int grid;            // CTAs that share the items out
+    float scale_log2;    // scale * log2(e)
+    float *part;         // [grid][2] slots of [RT][D] accumulators and [RT][2] (m in log2 units, l)
+    int *entries;        // [grid][8]: the cut unit whose first cut lies in front of this CTA (ca_entry)
+    unsigned *err, *err_sys;
+    unsigned spin_limit;
+};
+
+__host__ __device__ inline size_t ca_slot_floats(int RT, int D) { return (size_t)RT * (D + 2); }
+
+// rows cached for a sequence
+__device__ __forceinline__ int ca_len(const int *len, int b, int S) { return min(max(__ldg(len + b), 0), S); }
+// items of cached keys (a call without new keys has one at least, so that every unit has an item)
+__device__ __forceinline__ int ca_tiles(const CaParams &p, int n) {
+    const int ct = (n + p.TK - 1) / p.TK;
+    return p.drafts ? ct : max(ct, 1);
+}
+// items of new keys of unit rt: the last row of a chain sees its own token last
+__host__ __device__ inline int ca_draft_tiles(int rt, int R, int RT, int G, int T, int TK, bool chain) {
+    const long long end = (long long)(rt + 1) * RT;
+    const int t = chain ? (int)(((end < R ? end : R) - 1) / G) + 1 : T;
+    return (t + TK - 1) / TK;
+}
+__device__ __forceinline__ int ca_draft_tiles(const CaParams &p, int rt) {
+    return p.drafts ? ca_draft_tiles(rt, p.R, p.RT, p.G, p.T, p.TK, p.mask == nullptr) : 0;
+}
+
+struct CaStart { long long total; int b; int grid; long long rem; };   // all items; where a CTA's range begins: sequence, item within it; CTAs with work
+
+__device__ __forceinline__ long long ca_range(long long total, int grid, int c) { return total * c / grid; }
+__device__ __forceinline__ int ca_cta_of(long long total, int grid, long long i) { return (int)(((i + 1) * grid - 1) / total); }
+
+// By one whole warp: where the range of CTA `c` begins.
+__device__ __forceinline__ CaStart ca_locate(const CaParams &p, int c) {
+    const int lane = threadIdx.x & 31;
+    long long total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * ca_tiles(p, ca_len(p.len, b0 + lane, p.S)) + p.DT) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        total += x;
+    }
+    CaStart s{total, 0, (int)min((long long)p.grid, total), 0};
+    if (c >= s.grid) return s;
+    const long long i0 = ca_range(total, s.grid, c);
+    long long before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * ca_tiles(p, ca_len(p.len, b0 + lane, p.S)) + p.DT) : 0;
+        long long incl = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + incl > i0);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            s.b = b0 + at;
+            s.rem = i0 - before - __shfl_sync(0xffffffffu, incl - x, at);
+            return s;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return s;   // (not reached: i0 < total)
+}
+
+// The units of a CTA's range, one after the other; each role of a CTA keeps a walk of its own.
+struct CaWalk {
+    long long left, u0;   // items left of the range; first item of the unit, counted over all
+    int b, h, rt, n;      // the unit; rows cached
+    int tile, ct, nt;     // first item of this CTA in the unit; items of cached keys; all items
+    __device__ __forceinline__ void unit(const CaParams &p) { nt = ct + ca_draft_tiles(p, rt); }
+    __device__ __forceinline__ void start(const CaParams &p, const CaStart &s, int c) {
+        const long long i0 = ca_range(s.total, s.grid, c);
+        left = c < s.grid ? ca_range(s.total, s.grid, c + 1) - i0 : 0;
+        if (left == 0) return;
+        b = s.b;
+        n = ca_len(p.len, b, p.S);
+        ct = ca_tiles(p, n);
+        const long long per = (long long)p.nrt * ct + p.DT;
+        h = (int)(s.rem / per);
+        long long rem = s.rem % per;
+        for (rt = 0;; ++rt) {
+            unit(p);
+            if (rem < nt) break;
+            rem -= nt;
+        }
+        tile = (int)rem;
+        u0 = i0 - rem;
+    }
+    __device__ __forceinline__ int end() const { return (int)min((long long)nt, tile + left); }
+    __device__ __forceinline__ bool whole() const { return tile == 0 && left >= nt; }
+    __device__ __forceinline__ void next(const CaParams &p) {
+        left -= end() - tile;
+        if (left == 0) return;
+        u0 += nt;
+        tile = 0;
+        if (++rt == p.nrt) {
+            rt = 0;
+            if (++h == p.Hkv) {
+                h = 0;
+                ++b;
+                n = ca_len(p.len, b, p.S);
+                ct = ca_tiles(p, n);
+            }
+        }
+        unit(p);
+    }
+};
+
+// By one thread, for the first unit of a CTA's range: where that unit was cut by this range's beginning, and by none before it, its parts are
+// listed for ca_combine_kernel: {first CTA or -1, its slot, last CTA, b, h, rt}.  Every other part is in slot 0 of its CTA.
+__device__ __forceinline__ void ca_entry(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
+    int *e = p.entries + (size_t)c * 8;
+    e[0] = -1;
+    if (w.left == 0 || w.tile == 0) return;
+    const int first = ca_cta_of(s.total, s.grid, w.u0);
+    if (ca_cta_of(s.total, s.grid, w.u0 + w.tile - 1) != first) return;
+    e[1] = ca_range(s.total, s.grid, first) == w.u0 ? 0 : 1;
+    e[2] = ca_cta_of(s.total, s.grid, w.u0 + w.nt - 1);
+    e[3] = w.b; e[4] = w.h; e[5] = w.rt;
+    e[0] = first;
+}
+
+template <typename T>
+__device__ __forceinline__ T *ca_row(void *base, const CaView &v, int b, int h, long long l) {
+    return reinterpret_cast<T *>(base) + b * v.b + h * v.h + l * v.l;
+}
+template <typename T>
+__device__ __forceinline__ const T *ca_row(const void *base, const CaView &v, int b, int h, long long l) {
+    return reinterpret_cast<const T *>(base) + b * v.b + h * v.h + l * v.l;
+}
+
+// ---- joining the parts of cut units ---------------------------------------------------------------------------------
+// Block (c, y): rows 8 y .. 8 y + 7 of the unit that entry c lists.  A row is taken by `per` warps that share its parts out, so that a row cut
+// over the whole chip (one sequence, one key head) does not wait for one part after the other.
+constexpr int CB_THREADS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(CB_THREADS)
+ca_combine_kernel(const CaParams p) {
+    __shared__ float s_acc[8][CA_MAX_D];
+    __shared__ float s_ml[8][2];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int *e = p.entries + (size_t)blockIdx.x * 8;
+    const int first = e[0];
+    if (first < 0) return;
+    const int slot0 = e[1], parts = e[2] - first + 1, b = e[3], h = e[4], rt = e[5];
+    const int rows = min(p.RT, p.R - rt * p.RT), row0 = blockIdx.y * 8;
+    if (row0 >= rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per = parts <= 12 ? 1 : parts <= 24 ? 2 : parts <= 48 ? 4 : 8;   // warps of a row
+    const size_t slot = ca_slot_floats(p.RT, p.D);
+    for (int r0 = 0; r0 < 8; r0 += 8 / per) {
+        const int row = row0 + r0 + warp / per;
+        float m = -INFINITY, l = 0.0f, acc[CA_MAX_D / 32];
+#pragma unroll
+        for (int i = 0; i < CA_MAX_D / 32; ++i) acc[i] = 0.0f;
+        if (row < rows) {
+            for (int c = warp % per; c < parts; c += per) {
+                const float *ps = p.part + ((size_t)(first + c) * 2 + (c == 0 ? slot0 : 0)) * slot;
+                const float pm = ps[(size_t)p.RT * p.D + 2 * row], pl = ps[(size_t)p.RT * p.D + 2 * row + 1];
+                const float mn = fmaxf(m, pm);
+                const float f = mn == -INFINITY ? 0.0f : exp2f(m - mn), pf = mn == -INFINITY ? 0.0f : exp2f(pm - mn);
+                l = l * f + pl * pf;
+                m = mn;
+#pragma unroll
+                for (int i = 0; i < CA_MAX_D / 32; ++i)
+                    if (lane + 32 * i < p.D) acc[i] = acc[i] * f + ps[(size_t)row * p.D + lane + 32 * i] * pf;
+            }
+        }
+        if (per > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < CA_MAX_D / 32; ++i)
+                if (lane + 32 * i < p.D) s_acc[warp][lane + 32 * i] = acc[i];
+            if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+            __syncthreads();
+            if (warp % per != 0) continue;
+            for (int w = warp + 1; w < warp + per; ++w) {
+                const float pm = s_ml[w][0], pl = s_ml[w][1], mn = fmaxf(m, pm);
+                const float f = mn == -INFINITY ? 0.0f : exp2f(m - mn), pf = mn == -INFINITY ? 0.0f : exp2f(pm - mn);
+                l = l * f + pl * pf;
+                m = mn;
+#pragma unroll
+                for (int i = 0; i < CA_MAX_D / 32; ++i)
+                    if (lane + 32 * i < p.D) acc[i] = acc[i] * f + s_acc[w][lane + 32 * i] * pf;
+            }
+        }
+        if (row >= rows) continue;
+        const int r = rt * p.RT + row, t = r / p.G, hq = h * p.G + r % p.G;
+        T *o = ca_row<T>(p.O, p.o, b, hq, t);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < CA_MAX_D / 32; ++i)
+            if (lane + 32 * i < p.D) o[lane + 32 * i] = OutCvt<T>::one(acc[i] * inv);
+        if (p.lse && lane == 0) p.lse[((long long)b * p.Hq + hq) * p.T + t] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    }
+}
+
+// ---- attention on the CUDA cores: every type, width and stride ---------------------------------------------------------
+// Units of 16 rows, tiles of 64 keys, 128 threads.  K and V pass through shared memory in fp32; a thread computes the scores of one key with
+// eight rows, then owns 16 outputs (8 rows of one column up to head_d 64, else 16 rows) per 128 columns.  Bound by FFMA and shared-memory reads.
+constexpr int CG_ROWS = 16, CG_KEYS = 64, CG_THREADS = 128;
+__host__ __device__ inline int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
+inline size_t cg_smem_bytes(int D) { return ((size_t)(CG_ROWS + 2 * CG_KEYS) * cg_pitch(D) + CG_KEYS * (CG_ROWS + 4)) * sizeof(float); }
+
+template <typename T, int DB>   // DB: columns rounded up to 64, 128 or 256
+__global__ void __launch_bounds__(CG_THREADS)
+ca_generic_kernel(const CaParams p) {
+    extern __shared__ __align__(16) float cg_smem[];
+    __shared__ CaStart s_start;
+    __shared__ float s_m[CG_ROWS], s_l[CG_ROWS], s_f[CG_ROWS];
+    const int pitch = cg_pitch(p.D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float *qs = cg_smem, *ks = qs + CG_ROWS * pitch, *vs = ks + CG_KEYS * pitch, *ps = vs + CG_KEYS * pitch;   // ps [64 keys][16 rows + 4]
+    constexpr int PP = CG_ROWS + 4;
+    constexpr int NC = DB <= 128 ? 1 : 2, NR = DB <= 64 ? 8 : 16;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (warp == 0) {
+        const CaStart s = ca_locate(p, blockIdx.x);
+        if (lane == 0) s_start = s;
+    }
+    __syncthreads();
+    CaWalk w;
+    w.start(p, s_start, blockIdx.x);
+    if (tid == 0) ca_entry(p, s_start, w, blockIdx.x);
+    const int col = DB <= 64 ? (tid & 63) : tid, rbase = DB <= 64 ? (tid >> 6) * 8 : 0;
+    for (bool first = true; w.left > 0; first = false) {
+        const int row0 = w.rt * p.RT, rows = min(p.RT, p.R - row0);
+        __syncthreads();
+        for (int i = tid; i < CG_ROWS * pitch; i += CG_THREADS) {
+            const int r = i / pitch, d = i % pitch;
+            float x = 0.0f;
+            if (r < rows && d < p.D) x = to_f32(ca_row<T>(p.Q, p.q, w.b, w.h * p.G + (row0 + r) % p.G, (row0 + r) / p.G)[d]);
+            qs[i] = x;
+        }
+        if (tid < CG_ROWS) { s_m[tid] = -INFINITY; s_l[tid] = 0.0f; }
+        float acc[NC][NR];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) acc[c][r] = 0.0f;
+        for (int tile = w.tile; tile < w.end(); ++tile) {
+            const bool draft = tile >= w.ct;
+            const int j0 = (draft ? tile - w.ct : tile) * CG_KEYS, nk = min(CG_KEYS, (draft ? p.T : w.n) - j0);   // keys of the tile (0: an empty cache)
+            __syncthreads();
+            for (int i = tid; i < CG_KEYS * pitch; i += CG_THREADS) {
+                const int j = i / pitch, d = i % pitch;
+                float x = 0.0f, y = 0.0f;
+                if (j < nk && d < p.D) {
+                    x = to_f32(draft ? ca_row<T>(p.Kd, p.kd, w.b, w.h, j0 + j)[d] : ca_row<T>(p.K, p.k, w.b, w.h, j0 + j)[d]);
+                    y = to_f32(draft ? ca_row<T>(p.Vd, p.vd, w.b, w.h, j0 + j)[d] : ca_row<T>(p.V, p.v, w.b, w.h, j0 + j)[d]);
+                }
+                ks[i] = x;
+                vs[i] = y;
+            }
+            __syncthreads();
+            {   // scores of key j with rows rb .. rb + 7, in log2 units; what a row does not see is -inf
+                const int j = tid & 63, rb = (tid >> 6) * 8;
+                float s[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) s[r] = 0.0f;
+                for (int d = 0; d < pitch - 3; d += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4 *>(ks + j * pitch + d);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const float4 q4 = *reinterpret_cast<const float4 *>(qs + (rb + r) * pitch + d);
+                        s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    bool see = j < nk && rb + r < rows;
+                    if (see && draft) {
+                        const int t = (row0 + rb + r) / p.G;
+                        see = p.mask ? p.mask[w.b * p.mask_b + (long long)t * p.T + j0 + j] != 0 : j0 + j <= t;
+                    }
+                    ps[j * PP + rb + r] = see ? s[r] * p.scale_log2 : -INFINITY;
+                }
+            }
+            __syncthreads();
+            for (int r = warp; r < CG_ROWS; r += CG_THREADS / 32) {
+                const float a = ps[lane * PP + r], b = ps[(lane + 32) * PP + r], mo = s_m[r];
+                const float mn = fmaxf(mo, warp_max(fmaxf(a, b)));
+                const float ea = a == -INFINITY ? 0.0f : exp2f(a - mn), eb = b == -INFINITY ? 0.0f : exp2f(b - mn);
+                const float sum = warp_sum(ea + eb);
+                ps[lane * PP + r] = ea;
+                ps[(lane + 32) * PP + r] = eb;
+                if (lane == 0) {
+                    const float f = mn == -INFINITY ? 0.0f : exp2f(mo - mn);
+                    s_f[r] = f;
+                    s_l[r] = s_l[r] * f + sum;
+                    s_m[r] = mn;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) acc[c][r] *= s_f[rbase + r];
+            for (int j = 0; j < nk; ++j) {
+                float v[NC];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) v[c] = col + 128 * c < pitch ? vs[j * pitch + col + 128 * c] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float e = ps[j * PP + rbase + r];
+                    // a key that the row does not see weighs exactly 0; its value may be NaN
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) acc[c][r] = draft && e == 0.0f ? acc[c][r] : fmaf(e, v[c], acc[c][r]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = w.whole();
+        float *part = p.part + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int rr = rbase + r;
+            if (rr >= rows) continue;
+            const float l = s_l[rr], inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T *o = whole ? ca_row<T>(p.O, p.o, w.b, w.h * p.G + (row0 + rr) % p.G, (row0 + rr) / p.G) : nullptr;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = col + 128 * c;
+                if (d >= p.D) continue;
+                if (whole) o[d] = OutCvt<T>::one(acc[c][r] * inv);
+                else part[(size_t)rr * p.D + d] = acc[c][r];
+            }
+        }
+        if (tid < rows) {
+            const float m = s_m[tid], l = s_l[tid];
+            if (!whole) {
+                part[(size_t)p.RT * p.D + 2 * tid] = m;
+                part[(size_t)p.RT * p.D + 2 * tid + 1] = l;
+            } else if (p.lse) {
+                const int r = row0 + tid;
+                p.lse[((long long)w.b * p.Hq + w.h * p.G + r % p.G) * p.T + r / p.G] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+            }
+        }
+        w.next(p);
+    }
+}
+
+// ---- lists of accepted tokens ------------------------------------------------------------------------------------------
+// By one whole warp: entries of the list in front of the first that names no token, `most` at the most.
+__device__ __forceinline__ int ca_count(const int *accepted, int b, int A, int T, int most) {
+    const int lane = threadIdx.x & 31;
+    if (accepted == nullptr) return min(T, most);
+    for (int i0 = 0; i0 < min(A, most); i0 += 32) {
+        const int i = i0 + lane;
+        const bool ends = i >= A || (unsigned)__ldg(accepted + (long long)b * A + i) >= (unsigned)T;
+        const unsigned any = __ballot_sync(0xffffffffu, ends);
+        if (any) return min(i0 + __ffs(any) - 1, most);
+    }
+    return min(A, most);
+}
+
+// ---- accumulated weights on the CUDA cores -------------------------------------------------------------------------------
+struct CwParams {
+    const void *Q, *K;
+    CaView q, k;
+    const int *len, *accepted;
+    const float *lse;
+    float *weights;
+    int A;               // entries of a list; T without lists
+    int B, Hq, Hkv, G, T, S, D;
+    float scale_log2;
+    unsigned *err, *err_sys;
+    unsigned spin_limit;
+};
+
+// Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows.
+template <typename T>
+__global__ void __launch_bounds__(CG_THREADS)
+cw_generic_kernel(const CwParams p) {
+    extern __shared__ __align__(16) float cg_smem[];
+    __shared__ float s_lse[CG_ROWS], s_half[CG_KEYS];
+    __shared__ int s_i[CG_ROWS];
+    const int pitch = cg_pitch(p.D), tid = threadIdx.x;
+    float *qs = cg_smem, *ks = qs + CG_ROWS * pitch;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int b = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * CG_KEYS;
+    const int n = ca_len(p.len, b, p.S);
+    if (j0 >= n) return;
+    const int count = ca_count(p.accepted, b, p.A, p.T, n);
+    if (count == 0) return;
+    for (int i = tid; i < CG_KEYS * pitch; i += CG_THREADS) {
+        const int j = i / pitch, d = i % pitch;
+        ks[i] = j0 + j < n && d < p.D ? to_f32(ca_row<T>(p.K, p.k, b, h, j0 + j)[d]) : 0.0f;
+    }
+    const int j = tid & 63, rb = (tid >> 6) * 8;
+    float sum = 0.0f;
+    for (int r0 = 0; r0 < count * p.G; r0 += CG_ROWS) {
+        __syncthreads();
+        if (tid < CG_ROWS) {
+            const int r = r0 + tid, i = r / p.G;
+            float x = -INFINITY;
+            if (i < count) x = p.lse[((long long)b * p.Hq + h * p.G + r % p.G) * p.T + (p.accepted ? p.accepted[(long long)b * p.A + i] : i)];
+            s_i[tid] = x == -INFINITY ? -1 : i;   // a token that saw nothing gave no weight
+            s_lse[tid] = x;
+        }
+        for (int i = tid; i < CG_ROWS * pitch; i += CG_THREADS) {
+            const int r = r0 + i / pitch, d = i % pitch, a = r / p.G;
+            float x = 0.0f;
+            if (a < count && d < p.D) x = to_f32(ca_row<T>(p.Q, p.q, b, h * p.G + r % p.G, p.accepted ? p.accepted[(long long)b * p.A + a] : a)[d]);
+            qs[i] = x;
+        }
+        __syncthreads();
+        float s[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] = 0.0f;
+        for (int d = 0; d < pitch - 3; d += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(ks + j * pitch + d);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float4 q4 = *reinterpret_cast<const float4 *>(qs + (rb + r) * pitch + d);
+                s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int i = s_i[rb + r];
+            if (i >= 0 && j0 + j <= n - count + i) sum += exp2f(fmaf(s[r], p.scale_log2, -1.4426950408889634f * s_lse[rb + r]));
+        }
+    }
+    if (tid >= 64) s_half[j] = sum;
+    __syncthreads();
+    if (tid < 64 && j0 + j < n) p.weights[((long long)b * p.Hkv + h) * p.S + j0 + j] += sum + s_half[j];
+}
+
+// ---- rows from one place to another ------------------------------------------------------------------------------------
+// A warp copies a row of `bytes` bytes in pieces of type P (16 bytes, or an element where rows are not that aligned).
+template <typename P>
+__device__ __forceinline__ void ca_copy_row(void *dst, const void *src, int bytes, int lane) {
+    const int n = bytes / (int)sizeof(P);
+    for (int i = lane; i < n; i += 32) reinterpret_cast<P *>(dst)[i] = reinterpret_cast<const P *>(src)[i];
+}
+
+struct CcParams {
+    void *K, *V;
+    const void *Kd, *Vd;
+    CaView k, v, kd, vd;   // strides in bytes
+    const int *len, *accepted, *next_pos;
+    int *len_out, *pos;
+    float *weights;
+    int A, B, Hkv, T, S, row_bytes;
+};
+constexpr int CC_THREADS = 256;
+
+// A warp per (head, accepted token), sequences along y: bound by memory where a prompt enters, else by the launch.
+template <typename P>
+__global__ void __launch_bounds__(CC_THREADS)
+cc_commit_kernel(const CcParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, b = blockIdx.y;
+    const int n = ca_len(p.len, b, p.S);
+    const long long wid = (long long)blockIdx.x * (CC_THREADS / 32) + (threadIdx.x >> 5);
+    if (wid == 0 && p.len_out) {
+        const int count = ca_count(p.accepted, b, p.A, p.T, p.S - n);
+        if (lane == 0) p.len_out[b] = n + count;
+    }
+    if (wid >= (long long)p.A * p.Hkv) return;
+    const int h = (int)(wid / p.A), i = (int)(wid % p.A);
+    if (ca_count(p.accepted, b, p.A, p.T, min(i + 1, p.S - n)) <= i) return;
+    const int t = p.accepted ? __ldg(p.accepted + (long long)b * p.A + i) : i;
+    const long long row = n + i;
+    ca_copy_row<P>((char *)p.K + b * p.k.b + h * p.k.h + row * p.k.l, (const char *)p.Kd + b * p.kd.b + h * p.kd.h + t * p.kd.l, p.row_bytes, lane);
+    ca_copy_row<P>((char *)p.V + b * p.v.b + h * p.v.h + row * p.v.l, (const char *)p.Vd + b * p.vd.b + h * p.vd.h + t * p.vd.l, p.row_bytes, lane);
+    const long long at = ((long long)b * p.Hkv + h) * p.S + row;
+    if (lane == 0 && p.weights) p.weights[at] = 0.0f;
+    if (lane == 0 && p.pos) p.pos[at] = (p.next_pos ? __ldg(p.next_pos + b) : n) + i;
+}
+
+// ---- eviction ------------------------------------------------------------------------------------------------------------
+struct CeParams {
+    void *K, *V, *K_out, *V_out;     // K_out == nullptr: in place
+    CaView k, v, ko, vo;             // strides in bytes
+    float *weights, *weights_out;
+    int *pos, *pos_out;
+    const int *len, *next_pos;
+    int *len_out, *kept;
+    int keep, sink, recent;
+    int B, Hkv, S, S_out, row_bytes;
+};
+
+// Weights as whole numbers of the same order: NaN lowest, -0 and 0 equal; protected rows are above all of them.
+__device__ __forceinline__ unsigned ce_rank(float w, bool held) {
+    if (held) return 0xffffffffu;
+    if (w != w) return 0u;
+    const unsigned u = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int CE_THREADS = 1024;
+constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS;
+inline size_t ce_smem_bytes(int S) { return (size_t)((S + 31) / 32) * 2 * sizeof(unsigned); }
+
+// Exclusive scan of one value per thread of the block.
+__device__ __forceinline__ int ce_scan(int x, int *s_warp, int *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int v = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += y;
+        }
+        s_warp[lane] = v;
+    }
+    __syncthreads();
+    if (total) *total = s_warp[31];
+    return (warp ? s_warp[warp - 1] : 0) + incl - x;
+}
+
+// One block per (sequence, head) finds the rows that stay and writes `kept`:
+//   the m-th largest rank by its digits from the top (three passes of a histogram over the rows of the prefix found so far),
+//   then two bit masks over the rows in shared memory - above that rank, equal to it; of the equal rows the first that there is room for stay -
+//   then, in place, the i-th freed row below m takes the i-th kept row from m on, found by its number among the mask's bits.
+__global__ void __launch_bounds__(CE_THREADS)
+ce_select_kernel(const CeParams p) {
+    extern __shared__ unsigned ce_masks[];
+    __shared__ int hist[CE_BINS], s_warp[32], s_first[CE_THREADS];
+    __shared__ unsigned s_digit;
+    __shared__ int s_above;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.y, h = blockIdx.x;
+    const int n = ca_len(p.len, b, p.S), m = min(n, p.keep);
+    const long long unit = (long long)b * p.Hkv + h;
+    int *kept = p.kept + unit * p.keep;
+    if (h == 0 && tid == 0 && p.len_out) p.len_out[b] = m;
+    for (int i = m + tid; i < p.keep; i += CE_THREADS) kept[i] = -1;
+    if (n <= p.keep) {
+        for (int i = tid; i < m; i += CE_THREADS) kept[i] = i;
+        return;
+    }
+    const float *w = p.weights + unit * p.S;
+    const int *pos = p.pos ? p.pos + unit * p.S : nullptr;
+    const long long recent = (long long)(p.next_pos ? p.next_pos[b] : n) - p.recent;
+    auto rank = [&](int r) {
+        const int at = pos ? pos[r] : r;
+        return ce_rank(w[r], at < p.sink || at >= recent);
+    };
+    unsigned prefix = 0;
+    int need = m;   // rows to take from those that share the prefix
+    for (int shift = 32 - CE_BITS;; shift = shift > CE_BITS ? shift - CE_BITS : 0) {
+        const int bits = shift == 0 ? 32 - 2 * CE_BITS : CE_BITS;
+        for (int i = tid; i < CE_BINS; i += CE_THREADS) hist[i] = 0;
+        __syncthreads();
+        for (int r0 = 0; r0 < n; r0 += CE_THREADS) {
+            const int r = r0 + tid;
+            const unsigned x = r < n ? rank(r) : 0u;
+            const bool in = r < n && (shift + bits == 32 || (x >> (shift + bits)) == (prefix >> (shift + bits)));
+            // equal digits are common (weights of 0): one addition per digit and warp
+            const unsigned d = in ? (x >> shift) & ((1u << bits) - 1) : 0xffffffffu;
+            const unsigned same = __match_any_sync(0xffffffffu, d);
+            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&hist[d], __popc(same));
+        }
+        __syncthreads();
+        // from the top digit down: the one in which the count reaches `need`; thread i has the digits 2 (1023 - i) + 1 and 2 (1023 - i)
+        const int hi = hist[2 * (CE_THREADS - 1 - tid) + 1], lo = hist[2 * (CE_THREADS - 1 - tid)];
+        const int before = ce_scan(hi + lo, s_warp, nullptr);
+        if (before < need && before + hi + lo >= need) {
+            const bool top = before + hi >= need;
+            s_digit = 2 * (CE_THREADS - 1 - tid) + (top ? 1 : 0);
+            s_above = before + (top ? 0 : hi);
+        }
+        __syncthreads();
+        prefix |= s_digit << shift;
+        need -= s_above;
+        __syncthreads();
+        if (shift == 0) break;
+    }
+    const int words = (n + 31) / 32;
+    unsigned *stays = ce_masks, *equal = ce_masks + words;
+    for (int r0 = 0; r0 < words * 32; r0 += CE_THREADS) {
+        const int r = r0 + tid;
+        if (r >= words * 32) break;   // (whole warps)
+        const unsigned x = r < n ? rank(r) : 0u;
+        const unsigned gt = __ballot_sync(0xffffffffu, r < n && x > prefix), eq = __ballot_sync(0xffffffffu, r < n && x == prefix);
+        if (lane == 0) { stays[r >> 5] = gt; equal[r >> 5] = eq; }
+    }
+    __syncthreads();
+    // each thread owns `per` words in a row
+    const int per = (words + CE_THREADS - 1) / CE_THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    int c = 0;
+    for (int i = w0; i < w1; ++i) c += __popc(equal[i]);
+    int room = need - ce_scan(c, s_warp, nullptr);
+    for (int i = w0; i < w1; ++i) {
+        unsigned eq = equal[i];
+        while (eq && room > 0) {
+            stays[i] |= eq & -eq;
+            eq &= eq - 1;
+            --room;
+        }
+    }
+    __syncthreads();
+    if (p.K_out) {   // in order
+        c = 0;
+        for (int i = w0; i < w1; ++i) c += __popc(stays[i]);
+        int at = ce_scan(c, s_warp, nullptr);
+        for (int i = w0; i < w1; ++i)
+            for (unsigned x = stays[i]; x; x &= x - 1) kept[at++] = 32 * i + __ffs(x) - 1;
+        return;
+    }
+    auto late = [&](int i) {   // rows from m on that stay, of word i
+        return 32 * i >= m ? stays[i] : 32 * i + 32 <= m ? 0u : stays[i] & ~((1u << (m - 32 * i)) - 1);
+    };
+    c = 0;
+    for (int i = w0; i < w1; ++i) c += __popc(late(i));
+    s_first[tid] = ce_scan(c, s_warp, nullptr);   // number of the first such row of this thread's words
+    c = 0;
+    for (int i = w0; i < w1; ++i) c += 32 * i >= m ? 0 : __popc(~stays[i] & (32 * i + 32 <= m ? 0xffffffffu : (1u << (m - 32 * i)) - 1));
+    int hole = ce_scan(c, s_warp, nullptr);
+    for (int i = w0; i < w1; ++i) {
+        for (int k = 0; k < 32 && 32 * i + k < m; ++k) {
+            const int r = 32 * i + k;
+            int from = r;
+            if (!(stays[i] >> k & 1)) {
+                int lo = 0, hi = CE_THREADS;   // the last thread whose first number is <= hole has that row
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_first[mid] <= hole) lo = mid; else hi = mid;
+                }
+                int left = hole - s_first[lo], x = lo * per;
+                while (left >= __popc(late(x))) left -= __popc(late(x++));
+                unsigned bitsx = late(x);
+                while (left--) bitsx &= bitsx - 1;
+                from = 32 * x + __ffs(bitsx) - 1;
+                ++hole;
+            }
+            kept[r] = from;
+        }
+    }
+}
+
+// Moves what `kept` says: a warp per row.  In place the sources are rows >= m and the targets rows < m, so that no move reads what another writes.
+template <typename P>
+__global__ void __launch_bounds__(CC_THREADS)
+ce_move_kernel(const CeParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, b = blockIdx.z, h = blockIdx.y;
+    const long long unit = (long long)b * p.Hkv + h;
+    const int i0 = (blockIdx.x * (CC_THREADS / 32) + (threadIdx.x >> 5)) * 32;
+    const int mine = i0 + lane < p.keep ? p.kept[unit * p.keep + i0 + lane] : -1;
+    const bool moves = mine >= 0 && (p.K_out || mine != i0 + lane);
+    for (unsigned todo = __ballot_sync(0xffffffffu, moves); todo; todo &= todo - 1) {
+        const int k = __ffs(todo) - 1;
+        const long long from = __shfl_sync(0xffffffffu, mine, k), to = i0 + k;
+        const CaView ko = p.K_out ? p.ko : p.k, vo = p.K_out ? p.vo : p.v;
+        ca_copy_row<P>((char *)(p.K_out ? p.K_out : p.K) + b * ko.b + h * ko.h + to * ko.l, (const char *)p.K + b * p.k.b + h * p.k.h + from * p.k.l, p.row_bytes, lane);
+        ca_copy_row<P>((char *)(p.K_out ? p.V_out : p.V) + b * vo.b + h * vo.h + to * vo.l, (const char *)p.V + b * p.v.b + h * p.v.h + from * p.v.l, p.row_bytes, lane);
+    }
+    if (moves) {
+        float *wo = p.K_out ? p.weights_out + unit * p.S_out : p.weights + unit * p.S;
+        wo[i0 + lane] = p.weights[unit * p.S + mine];
+        if (p.pos) (p.K_out ? p.pos_out + unit * p.S_out : p.pos + unit * p.S)[i0 + lane] = p.pos[unit * p.S + mine];
+    }
+}
+
+}  // namespace b200attn

@@ -257,6 +257,128 @@ int b200attn_forward_static(const float *Q, const float *K, const float *V, floa
                             int len_q, int len_k, int head_d, void *stream);
 const char *b200attn_static_last_error(void);
 
+/* ------------------------------------------------------------------------------------------ */
+/* A key/value cache: attention over it, and what keeps it                                     */
+/* ------------------------------------------------------------------------------------------ */
+
+/* The four calls below serve a decoder whose keys and values stay in a cache: tensors K and V [B,Hkv,S,D] with room for S
+ * rows (`capacity`) and a number of valid rows per sequence, length[b], in DEVICE memory.  Query heads share key heads in
+ * groups: query head h reads key head h / (num_heads / num_kv_heads).  One step of a program that drafts tokens:
+ *     b200attn_cache_attend    attention of the T new tokens over the cached rows and over each other (a tree of drafts)
+ *     (the program verifies the drafts)
+ *     b200attn_cache_commit    the accepted ones become rows of the cache, length[b] grows
+ *     b200attn_cache_weights   adds up, per cached row, the attention weight that the accepted tokens gave it
+ *     b200attn_cache_evict     once a cache exceeds its budget, the rows of least weight leave it
+ * An encoding of positions is applied by the caller before the call (b200attn_rope_k): keys are cached encoded.
+ *
+ * Common to all four.  They have no counterpart in the reference.  Tensors are views: the last dimension (D) is contiguous, the others have
+ * strides in elements, so a projection's output [B,T,heads,D] is passed as it is; pointers are aligned to the element size.  The
+ * other arrays are dense.  The work is enqueued on `stream` and waited for unless B200ATTN_FLAG_ASYNC is set.  Values that only the device
+ * knows cannot be refused by the host: a length outside [0, capacity] counts as the nearer of the two; rows behind the last valid one are
+ * neither read (whatever they hold, NaN included, has no effect) nor written.  Calls that share no tensors may be made at the same time from several threads and streams when each
+ * has a workspace of its own. */
+typedef struct b200attn_view {   /* a tensor [B, heads, rows, D] */
+    void *ptr;                   /* device pointer */
+    long long stride_b, stride_h, stride_l;   /* elements from one sequence, head, row to the next; not negative */
+} b200attn_view;
+
+/* out[b,h,t] = sum_j w_j V_j, w = softmax over the keys that token t sees of scale * Q[b,h,t] . K_j: the rows j < length[b] of the cache
+ * and, where Kd and Vd [B,Hkv,T,D] are given, the new tokens u with mask[b,t,u] != 0, or, without a mask, u <= t (a chain: the next token, or
+ * a prompt's next piece).  Without Kd and Vd the queries see the cache alone (cross attention to an encoder's states).
+ * lse[b,h,t] = log of the sum of exp(scale * Q . K_j), fp32.  A token that sees no key has out 0 and lse -inf.  Scores, softmax and
+ * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V.  A masked key and its value
+ * have no effect on a row, whatever they hold. */
+typedef struct b200attn_attend_args {
+    size_t struct_size;          /* sizeof(b200attn_attend_args) */
+    b200attn_view Q, K, V;       /* [B,Hq,T,D], [B,Hkv,S,D] */
+    b200attn_view Kd, Vd;        /* [B,Hkv,T,D]; ptr NULL in both: none */
+    b200attn_view out;           /* [B,Hq,T,D]; must not overlap an input */
+    float *lse;                  /* [B,Hq,T], or NULL */
+    const int *length;           /* [B] */
+    const unsigned char *mask;   /* [B,T,T], one byte each, or NULL */
+    long long mask_stride_b;     /* T*T, or 0 where all sequences share one mask */
+    int batch_sz, num_heads, num_kv_heads, len_new, capacity, head_d;   /* B, Hq, Hkv, T, S, D; D <= 256 */
+    int dtype;                   /* enum b200attn_dtype */
+    float scale;                 /* 0 means 1/sqrt(head_d) */
+    void *workspace;             /* device memory of b200attn_cache_attend_workspace bytes, 16-byte aligned; NULL: the library's own, with
+                                    the rules of b200attn_forward_ex for streams, threads and captures */
+    size_t workspace_bytes;
+    void *stream;
+    unsigned flags;              /* B200ATTN_FLAG_ASYNC, B200ATTN_FLAG_FORCE_GENERIC */
+} b200attn_attend_args;
+int b200attn_cache_attend(const b200attn_attend_args *args);
+/* Bytes of workspace that this call needs; needs no valid pointers.  0 and a message for b200attn_last_error() where the call would be refused. */
+size_t b200attn_cache_attend_workspace(const b200attn_attend_args *args);
+
+/* The i-th accepted token of sequence b, the new token t = accepted[b,i], becomes row length[b] + i: K and V of that row are copied from Kd and Vd
+ * [B,Hkv,T,D], weights[b,h,row] = 0, pos[b,h,row] = next_pos[b] + i.  The list ends at the first index outside [0, T) (pad it with -1) or after
+ * `max_accepted` entries; accepted NULL takes all T tokens in order.  Tokens that the cache has no room for are dropped.
+ * length_out[b] = length[b] + the number of rows written; the caches of all layers can be given the same `length`. */
+typedef struct b200attn_commit_args {
+    size_t struct_size;
+    b200attn_view K, V;          /* the cache, [B,Hkv,S,D] */
+    b200attn_view Kd, Vd;        /* [B,Hkv,T,D]; must not overlap the cache */
+    const int *length;           /* [B] */
+    int *length_out;             /* [B], not the array `length`; or NULL */
+    const int *accepted;         /* [B,max_accepted], or NULL */
+    int max_accepted;
+    float *weights;              /* [B,Hkv,S], or NULL */
+    int *pos;                    /* [B,Hkv,S], or NULL: the position in its text of each row's token */
+    const int *next_pos;         /* [B]: position of the first accepted token; NULL: length[b] (right while nothing has been evicted) */
+    int batch_sz, num_kv_heads, len_new, capacity, head_d, dtype;
+    void *stream;
+    unsigned flags;              /* B200ATTN_FLAG_ASYNC */
+} b200attn_commit_args;
+int b200attn_cache_commit(const b200attn_commit_args *args);
+
+/* weights[b,g,j] += sum over the accepted tokens and the query heads h of key head g of exp(scale * Q[b,h,t] . K[b,g,j] - lse[b,h,t]), where the i-th of
+ * the n accepted tokens of a sequence sees the rows j <= length[b] - n + i: the accepted tokens are the cache's last n rows (this call comes
+ * after the commit, `length` is the length after it), and Q and lse are those of the b200attn_cache_attend call before.  Sums in fp32, in an order that
+ * does not change from call to call.  `accepted` as above; a list longer than length[b] counts for its first length[b] entries; a token whose
+ * lse is -inf (it saw nothing) gave no weight. */
+typedef struct b200attn_weights_args {
+    size_t struct_size;
+    b200attn_view Q, K;          /* [B,Hq,T,D], [B,Hkv,S,D] */
+    const int *length;           /* [B] */
+    const float *lse;            /* [B,Hq,T] */
+    const int *accepted;         /* [B,max_accepted], or NULL */
+    int max_accepted;
+    float *weights;              /* [B,Hkv,S] */
+    int batch_sz, num_heads, num_kv_heads, len_new, capacity, head_d, dtype;   /* D <= 256 */
+    float scale;                 /* 0 means 1/sqrt(head_d) */
+    void *stream;
+    unsigned flags;              /* B200ATTN_FLAG_ASYNC, B200ATTN_FLAG_FORCE_GENERIC */
+} b200attn_weights_args;
+int b200attn_cache_weights(const b200attn_weights_args *args);
+
+/* Leaves m = min(length[b], keep) rows in each head of the cache: first the protected ones, then those of largest weight, among equals the
+ * lowest row (NaN is the least weight of all).  Protected are the tokens of the first `sink` positions and of the last `recent` ones: pos < sink or
+ * pos >= next_pos[b] - recent, with the row's index for pos and length[b] for next_pos where those are NULL.
+ * In place (K_out.ptr NULL) a row that stays does not move if its index is below m; the other kept rows fill the freed rows, both taken in
+ * order, so that a step's eviction moves few rows: rows do not stay in the order of their tokens, `pos` tells it.  Into another cache (K_out,
+ * V_out, weights_out and, with pos, pos_out given, capacity_out >= min(keep, capacity), no overlap) the kept rows are copied in order and this cache stays as it is.
+ * kept[b,h,i] = the former index of row i, -1 for i >= m.  length_out[b] = m. */
+typedef struct b200attn_evict_args {
+    size_t struct_size;
+    b200attn_view K, V;          /* [B,Hkv,S,D] */
+    float *weights;              /* [B,Hkv,S] */
+    int *pos;                    /* [B,Hkv,S], or NULL */
+    const int *length;           /* [B] */
+    const int *next_pos;         /* [B], or NULL */
+    int *length_out;             /* [B], not the array `length`; or NULL */
+    int *kept;                   /* [B,Hkv,keep] */
+    int keep, sink, recent;      /* keep >= 1, keep >= sink + recent */
+    b200attn_view K_out, V_out;  /* [B,Hkv,capacity_out,D], or ptr NULL: in place */
+    float *weights_out;          /* [B,Hkv,capacity_out] */
+    int *pos_out;                /* [B,Hkv,capacity_out] */
+    int capacity_out;
+    int batch_sz, num_kv_heads, capacity, head_d, dtype;   /* capacity <= B200ATTN_EVICT_MAX_ROWS */
+    void *stream;
+    unsigned flags;              /* B200ATTN_FLAG_ASYNC */
+} b200attn_evict_args;
+#define B200ATTN_EVICT_MAX_ROWS 524288
+int b200attn_cache_evict(const b200attn_evict_args *args);
+
 /* Fills a device buffer with the synthetic inputs the tests and the benchmark use: element i gets
  * a value drawn from splitmix64(seed*2^40 + tensor_id*2^36 + index0 + i); dist 0 = uniform[-1,1),
  * 1 = normal(0,1) by Box-Muller; stored as fp32 or rounded to bf16. */
