@@ -3,7 +3,7 @@
 #include <cstring>
 
 #include "host.h"
-#include "cache.cuh"
+#include "cache_tc.cuh"
 
 namespace b200attn {
 namespace {
@@ -134,6 +134,61 @@ int launch_attend(const CaParams &p, cudaStream_t st) {
     return B200ATTN_OK;
 }
 
+// The tensor-core kernel for these sizes: rows of a tile, tiles of a unit, ring.
+bool tc_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CtParams *out) {
+    if (a->dtype == B200ATTN_F32 || p.D % 8 != 0 || p.G > 128 || (a->flags & B200ATTN_FLAG_FORCE_GENERIC)) return false;
+    CtParams ct{};
+    ct.tpt = 128 / p.G;
+    ct.box_t = p.T < ct.tpt ? p.T : ct.tpt;
+    ct.rows8 = (p.G * ct.box_t + 7) & ~7;
+    ct.ng = (p.D + 63) / 64;
+    const int NT = p.D <= 128 && p.T > ct.tpt ? 2 : 1, TK = p.D <= 128 ? 128 : 64;
+    const size_t room = c.max_smem - 2048 - 1024, stage = (size_t)ct.ng * TK * 128;
+    // one row tile: the next unit's Q and the next key tile's P beside the present ones' where four stages remain
+    const int buffers[4][2] = {{2, 2}, {1, 2}, {2, 1}, {1, 1}};
+    for (int i = NT == 1 ? 0 : 3; i < 4; ++i) {
+        ct.nq = buffers[i][0]; ct.np = buffers[i][1];
+        const size_t front = ct_front_bytes(NT, ct.nq, ct.np, ct.ng, ct.rows8, TK);
+        ct.nst = front < room ? (int)((room - front) / stage) : 0;
+        if (ct.nst > CT_MAX_STAGES) ct.nst = CT_MAX_STAGES;
+        if (ct.nst >= (i < 3 ? 4 : 3)) break;
+    }
+    if (ct.nst < 3) return false;
+    share_out(p, NT * ct.tpt * p.G, TK, c.sm_count);
+    ct.a = p;
+    *out = ct;
+    return true;
+}
+bool tc_aligned(const b200attn_attend_args *a) {
+    auto fine = [&](const b200attn_view &v, long long h, long long l) {   // a dimension of size 1 has no stride to speak of; the others are not 0
+        b200attn_view x = v;
+        if (a->batch_sz == 1) x.stride_b = 8;
+        if (h == 1) x.stride_h = 8;
+        if (l == 1) x.stride_l = 8;
+        return aligned16(x, a->dtype) && x.stride_b > 0 && x.stride_h > 0 && x.stride_l > 0;
+    };
+    return fine(a->Q, a->num_heads, a->len_new) && fine(a->K, a->num_kv_heads, a->capacity) && fine(a->V, a->num_kv_heads, a->capacity) && fine(a->out, a->num_heads, a->len_new) &&
+           (a->Kd.ptr == nullptr || (fine(a->Kd, a->num_kv_heads, a->len_new) && fine(a->Vd, a->num_kv_heads, a->len_new)));
+}
+
+template <int NT, int TK, bool F16>
+int launch_tc(const CtParams &ct, const CUtensorMap (&m)[5], cudaStream_t st) {
+    const size_t smem = ct_front_bytes(NT, ct.nq, ct.np, ct.ng, ct.rows8, TK) + (size_t)ct.nst * ct.ng * TK * 128 + 1024;
+    int rc = raise_smem((const void *)ca_tc_kernel<NT, TK, F16>, smem);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_tc_kernel<NT, TK, F16>, dim3((unsigned)ct.a.grid), ct_threads(NT), smem, 1, st, m[0], m[1], m[2], m[3], m[4], ct));
+    return B200ATTN_OK;
+}
+template <bool F16>
+int launch_attend_tc(const CtParams &ct, const CUtensorMap (&m)[5], cudaStream_t st) {
+    const CaParams &p = ct.a;
+    int rc = p.TK == 64 ? launch_tc<1, 64, F16>(ct, m, st) : p.RT > ct.tpt * p.G ? launch_tc<2, 128, F16>(ct, m, st) : launch_tc<1, 128, F16>(ct, m, st);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    count_launches(2);
+    return B200ATTN_OK;
+}
+
 int attend(const b200attn_attend_args *a, size_t *need) {
     int rc = validate(a, need == nullptr);
     if (rc) return rc;
@@ -143,9 +198,22 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CaParams p{};
     fill(p, *a);
     p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    CtParams ct;
+    bool tc = tc_shape(a, c, p, &ct);
     share_out(p, CG_ROWS, CG_KEYS, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
-    const size_t bytes = attend_bytes(p);
+    // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
+    size_t bytes = attend_bytes(p);
+    if (tc && attend_bytes(ct.a) > bytes) bytes = attend_bytes(ct.a);
     if (need) { *need = bytes; return B200ATTN_OK; }
+    tc = tc && tc_aligned(a);
+    CUtensorMap m[5];
+    if (tc) {
+        memset(m, 0, sizeof m);
+        const CaParams &q = ct.a;
+        tc = ct_map_q(&m[0], q.Q, q.q, q.B, q.Hkv, q.G, q.T, q.D, ct.box_t) && ct_map_rows(&m[1], q.K, q.k, q.B, q.Hkv, q.S, q.D, q.TK) &&
+             ct_map_rows(&m[2], q.V, q.v, q.B, q.Hkv, q.S, q.D, q.TK) &&
+             (!q.drafts || (ct_map_rows(&m[3], q.Kd, q.kd, q.B, q.Hkv, q.T, q.D, q.TK) && ct_map_rows(&m[4], q.Vd, q.vd, q.B, q.Hkv, q.T, q.D, q.TK)));
+    }
     void *ws = a->workspace;
     if (ws) {
         if (a->workspace_bytes < bytes) return fail(B200ATTN_ERR_INVALID_ARG, "workspace_bytes is %zu, this call needs %zu", a->workspace_bytes, bytes);
@@ -153,11 +221,13 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     } else if ((rc = host_workspace(&c, bytes, st, &ws))) {
         return rc;
     }
-    p.part = (float *)ws;
-    p.entries = (int *)((char *)ws + bytes - (size_t)p.grid * 8 * sizeof(int));
-    rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, st) : launch_attend<__nv_bfloat16>(p, st);
+    CaParams &q = tc ? ct.a : p;
+    q.part = (float *)ws;
+    q.entries = (int *)((char *)ws + attend_bytes(q) - (size_t)q.grid * 8 * sizeof(int));
+    if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, m, st) : launch_attend_tc<false>(ct, m, st);
+    else rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, st) : launch_attend<__nv_bfloat16>(p, st);
     if (rc) return rc;
-    set_last_path("cache_generic");
+    set_last_path(tc ? "cache_tc" : "cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 

@@ -42,7 +42,7 @@ struct CaParams {
     unsigned spin_limit;
 };
 
-__host__ __device__ inline size_t ca_slot_floats(int RT, int D) { return (size_t)RT * (D + 2); }
+__host__ __device__ inline size_t ca_slot_floats(int RT, int D) { return ((size_t)RT * (D + 2) + 3) & ~(size_t)3; }
 
 // rows cached for a sequence
 __device__ __forceinline__ int ca_len(const int *len, int b, int S) { return min(max(__ldg(len + b), 0), S); }

@@ -1,0 +1,550 @@
+// Attention of new tokens over a cache on the 5th-generation tensor cores: bf16 / fp16, head_d a multiple of 8, at most 256, up to 128 query
+// heads a key head, 16-byte aligned rows.  The formulas and the sharing-out are those of cache.cuh.
+//
+// Rows (token t, query head g of the group: row t G + g) are the lanes of tensor memory, so the query heads that share a key head and the tokens of a
+// tree share every key tile: a tile of K and V is read once for up to 128 rows (ca_tc_kernel<1, ..>) or 256 (<2, ..>), and with one token and
+// four heads the MMAs compute 124 rows that nobody looks at - they are free: a tile of 128 keys (64 KB) takes 1.5 us from HBM at a 148th of its rate and
+// 0.55 us on the tensor cores.
+//   warp 0        one thread requests Q, K and V tiles by TMA through a ring of stages, in the order K_0 | K_1 V_0 | K_2 V_1 | ...
+//   warps 1, 2    one thread per row tile issues the MMAs: S = Q K^T, then O += P V once P is there
+//   warp 3        sees every V tile before the MMAs do: rows behind the cache's last are set to 0 (0 weight times NaN would be NaN); in a tile of
+//                 new tokens, which some rows see and others do not, values that are not finite are set to 0 and remembered
+//   warpgroups    a thread per row: scores into registers, the row's mask, running maximum and sum, P as 16-bit values to shared memory; at the end of a
+//                 unit O / l to the output or (O, m, l) to the workspace.  Values that warp 3 took out are added for the rows that see them.
+// The accumulator O stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 over the reference that its exponents are
+// taken against (m is that reference, so the result is exact; weights up to 2^8 stay inside fp16).  Rounding: P to the tensors' type; all else is fp32.
+// Warps of rows that do not exist only keep the hand-offs in step.  Every wait is bounded; one that expires sets the error word.
+#pragma once
+
+#include "cache.cuh"
+
+namespace b200attn {
+
+constexpr int CT_MAX_STAGES = 8;
+constexpr float CT_RESCALE_LOG2 = 8.0f;
+
+struct CtParams {
+    CaParams a;
+    int tpt, box_t;      // tokens of a row tile; tokens that a Q box has
+    int rows8;           // rows of a Q or P buffer: those of a box, whole groups of 8
+    int ng;              // groups of 64 columns
+    int nst, nq, np;     // ring stages, Q buffers, P buffers per row tile
+};
+
+constexpr int CT_SLOTS = 8;   // units of a CTA's range that its roles can be at: the ring lets the loading thread be four ahead
+
+struct CtSeg {           // a unit, or the part of it that is in this CTA's range
+    int b, h, rt, n;     // (n: rows cached)
+    int tile, end, ct;   // first and behind the last tile; tiles of cached keys
+    int whole;           // the whole unit; -1: no more units
+};
+
+struct CtBars {
+    uint64_t kv_full[CT_MAX_STAGES], kv_empty[CT_MAX_STAGES], ready[CT_MAX_STAGES];
+    uint64_t seg[CT_SLOTS];
+    uint64_t q_full[2], q_empty[2];
+    // per row tile, alternating from key tile to key tile: a wait by parity tells a phase from the one before it only
+    uint64_t s_full[2][2], s_read[2][2];   // scores are there / in registers
+    uint64_t p_full[2][2][2];              // each 64 keys of P
+    uint64_t o_done[2][2];                 // the MMAs over P have completed
+    uint64_t o_empty[2];
+};
+
+__device__ __forceinline__ void tma_load_5d(void *smem_dst, const CUtensorMap *tmap, int x, int y, int z, int w, int v, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+            smem_u32(smem_dst)),
+        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void ct_st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// A pair of 16-bit values with those that are not finite set to 0.
+template <bool F16>
+__device__ __forceinline__ uint32_t ct_finite(uint32_t w) {
+    constexpr uint32_t lo = F16 ? 0x00007c00u : 0x00007f80u, hi = lo << 16;
+    if ((w & lo) == lo) w &= 0xffff0000u;
+    if ((w & hi) == hi) w &= 0x0000ffffu;
+    return w;
+}
+template <bool F16> struct CtType { using T = __nv_bfloat16; };
+template <> struct CtType<true> { using T = __half; };
+
+// Bytes of shared memory in front of the ring: Q buffers, then P buffers.
+__host__ __device__ inline size_t ct_front_bytes(int NT, int nq, int np, int ng, int rows8, int TK) { return (size_t)NT * ((size_t)nq * ng + (size_t)np * (TK / 64)) * rows8 * 128; }
+
+#define CT_FAIL_AT(site, cond)                                                                          \
+    if (cond) {                                                                                         \
+        report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << (16 + (site))));     \
+        failed = true;                                                                                  \
+        break;                                                                                          \
+    }
+
+constexpr int ct_threads(int NT) { return 128 + NT * 128; }
+constexpr int CT_REGS_SMALL = 80, CT_REGS_LARGE = 208;   // NT = 2: 128 * 80 + 256 * 208 <= 384 * 168
+
+// NT: row tiles of 128 lanes per unit; TK: keys of a tile (64 where head_d is above 128, for stages of 32 KB).
+// Tensor memory: NT = 1: two score buffers at columns 0 and 128, O at 256; NT = 2: S_t at 128 t, O_t at 256 + 128 t.
+template <int NT, int TK, bool F16>
+__global__ void __launch_bounds__(ct_threads(NT), 1)
+ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+             const __grid_constant__ CUtensorMap tmKd, const __grid_constant__ CUtensorMap tmVd, const __grid_constant__ CtParams ct) {
+    using T = typename CtType<F16>::T;
+    extern __shared__ unsigned char ct_smem_raw[];
+    __shared__ CtBars bars;
+    __shared__ CaStart s_start;
+    __shared__ CtSeg s_seg[CT_SLOTS];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_bad[CT_SLOTS];     // warp 3: [unit of this CTA & 7] = that unit + 1 where its new values were not all finite
+    const CaParams &p = ct.a;
+    constexpr int NH = TK / 64;
+    const uint32_t raw_addr = smem_u32(ct_smem_raw);
+    unsigned char *smem = ct_smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ng = ct.ng, nst = ct.nst, nq = ct.nq;
+    const uint32_t slab = (uint32_t)ct.rows8 * 128u;        // 64 columns of a Q buffer, 64 keys of a P tile
+    const uint32_t stage = (uint32_t)ng * TK * 128u;        // a K or V tile: [ng groups][TK keys][128 B]
+    unsigned char *q_smem = smem;                           // [nq][NT][ng] slabs
+    unsigned char *p_smem = q_smem + (size_t)nq * NT * ng * slab;   // [NT][np][NH] slabs
+    // an MMA reads 128 rows from a slab's beginning on: behind the box's rows that is whatever follows, and only rows that nobody looks at depend on it
+    unsigned char *ring = p_smem + (size_t)NT * ct.np * NH * slab;
+    const uint32_t lim = p.spin_limit;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.kv_full[i], 1); mbar_init(&bars.kv_empty[i], NT + 1); mbar_init(&bars.ready[i], 1); }
+        for (int i = 0; i < CT_SLOTS; ++i) { mbar_init(&bars.seg[i], 1); s_bad[i] = 0; }
+        for (int i = 0; i < 2; ++i) { mbar_init(&bars.q_full[i], 1); mbar_init(&bars.q_empty[i], NT); }
+        for (int t = 0; t < 2; ++t) {
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars.s_full[t][b], 1); mbar_init(&bars.s_read[t][b], 4); mbar_init(&bars.o_done[t][b], 1);
+                for (int h = 0; h < 2; ++h) mbar_init(&bars.p_full[t][b][h], 4);
+            }
+            mbar_init(&bars.o_empty[t], 4);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+        if (p.drafts) { tma_prefetch_desc(&tmKd); tma_prefetch_desc(&tmVd); }
+    }
+    if (warp == 1) tmem_alloc(&tmem_slot, 512);
+    grid_dependency_wait();
+    if (warp == 2) {
+        const CaStart s = ca_locate(p, blockIdx.x);
+        if (lane == 0) s_start = s;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_launch_dependents();   // (not before the allocation: a dependent on this SM could take the columns and wait for this CTA to end)
+    const uint32_t tmem = tmem_slot;
+    bool failed = false;
+
+    if (warp < 4) {
+        if (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CT_REGS_SMALL));
+        if (warp == 0) {
+            if (elect_one()) {
+                CaWalk w;
+                w.start(p, s_start, blockIdx.x);
+                ca_entry(p, s_start, w, blockIdx.x);
+                int s = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                auto load = [&](bool v, int i) {   // tile i of the unit
+                    ok = ok && mbar_wait(&bars.kv_empty[s], ph ^ 1u, lim);
+                    if (!ok) return;
+                    mbar_expect_tx(&bars.kv_full[s], stage);
+                    const bool draft = i >= w.ct;
+                    const CUtensorMap *tm = draft ? (v ? &tmVd : &tmKd) : (v ? &tmV : &tmK);
+                    const int row = (draft ? i - w.ct : i) * TK;
+                    for (int g = 0; g < ng; ++g) tma_load_4d(ring + (size_t)s * stage + (size_t)g * (TK * 128), tm, g * 64, row, w.h, w.b, &bars.kv_full[s]);
+                    if (++s == nst) { s = 0; ph ^= 1u; }
+                };
+                int seg = 0;
+                for (; w.left > 0 && ok; ++seg, w.next(p)) {
+                    const int end = w.end();
+                    // (the slot's last unit is eight back: the ring has been handed back since by everybody who read it)
+                    s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, w.tile, end, w.ct, w.whole() ? 1 : 0};
+                    mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
+                    const int qi = nq == 2 ? seg & 1 : 0;
+                    ok = mbar_wait(&bars.q_empty[qi], (uint32_t)((nq == 2 ? seg >> 1 : seg) & 1) ^ 1u, lim);
+                    if (!ok) break;
+                    const int tok0 = w.rt * NT * ct.tpt, nt = NT == 2 && tok0 + ct.tpt < p.T ? 2 : 1;
+                    mbar_expect_tx(&bars.q_full[qi], (uint32_t)(nt * ng * p.G * ct.box_t) * 128u);
+                    for (int t = 0; t < nt; ++t)
+                        for (int g = 0; g < ng; ++g)
+                            tma_load_5d(q_smem + (size_t)((qi * NT + t) * ng + g) * slab, &tmQ, g * 64, 0, tok0 + t * ct.tpt, w.h, w.b, &bars.q_full[qi]);
+                    load(false, w.tile);
+                    for (int i = w.tile; i < end && ok; ++i) {
+                        if (i + 1 < end) load(false, i + 1);
+                        load(true, i);
+                    }
+                }
+                if (ok) {
+                    s_seg[seg & (CT_SLOTS - 1)].whole = -1;
+                    mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
+                } else {
+                    report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 16));
+                    failed = true;
+                }
+            }
+        } else if (warp == 3) {
+            // ---- every V tile before the MMAs see it ----
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            auto pass = [&](bool v, int i, int seg, int n, int nct) {
+                ok = ok && mbar_wait(&bars.kv_full[s], ph, lim);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                const bool draft = i >= nct;
+                unsigned char *tile = ring + (size_t)s * stage;
+                if (v && !draft && n - i * TK < TK) {
+                    const int first = max(n - i * TK, 0), per = (TK - first) * 8;   // 16-byte pieces of a group
+                    for (int g = 0; g < ng; ++g)
+                        for (int x = lane; x < per; x += 32) *reinterpret_cast<uint4 *>(tile + (size_t)g * (TK * 128) + first * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                } else if (v && draft) {
+                    const int per = min(TK, p.T - (i - nct) * TK) * 8;
+                    bool bad = false;
+                    for (int g = 0; g < ng; ++g)
+#pragma unroll 4
+                        for (int x = lane; x < per; x += 32) {
+                            uint4 *at = reinterpret_cast<uint4 *>(tile + (size_t)g * (TK * 128) + x * 16);
+                            const uint4 a = *at;
+                            const uint4 c = make_uint4(ct_finite<F16>(a.x), ct_finite<F16>(a.y), ct_finite<F16>(a.z), ct_finite<F16>(a.w));
+                            if (a.x != c.x || a.y != c.y || a.z != c.z || a.w != c.w) { *at = c; bad = true; }
+                        }
+                    if (__any_sync(0xffffffffu, bad)) {
+                        if (lane == 0) s_bad[seg & (CT_SLOTS - 1)] = seg + 1;
+                        fence_proxy_async_smem();
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&bars.ready[s]); mbar_arrive(&bars.kv_empty[s]); }
+                if (++s == nst) { s = 0; ph ^= 1u; }
+            };
+            for (int seg = 0; ok; ++seg) {
+                ok = mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const CtSeg w = s_seg[seg & (CT_SLOTS - 1)];
+                if (w.whole < 0) break;
+                pass(false, w.tile, seg, w.n, w.ct);
+                for (int i = w.tile; i < w.end && ok; ++i) {
+                    if (i + 1 < w.end) pass(false, i + 1, seg, w.n, w.ct);
+                    pass(true, i, seg, w.n, w.ct);
+                }
+            }
+            if (!ok) { report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 17)); failed = true; }
+        } else if (warp <= NT) {
+            if (elect_one()) {
+                const int t = warp - 1;
+                const int ks = (p.D + 15) >> 4;   // MMA steps of a score
+                const uint32_t id_qk = umma_idesc_16(128, TK, 0, 0, F16 ? 1 : 0), id_pv = umma_idesc_16(128, ks << 4, 0, 1, F16 ? 1 : 0);
+                const uint32_t pa = smem_u32(p_smem + (size_t)t * ct.np * NH * slab);
+                const uint32_t t_o = tmem + 256 + (NT == 2 ? t * 128 : 0);
+                int s = 0;
+                uint32_t ph = 0, gq = 0, gp = 0;   // key tiles so far: scores, products with V
+                int lu = 0;                        // units
+                bool ok = true;
+                uint32_t qa = 0;
+                int qi = 0;
+                auto qk = [&](bool last) {
+                    ok = ok && mbar_wait(&bars.kv_full[s], ph, lim);
+                    const uint32_t back = gq - (NT == 1 ? 2 : 1);   // the tile whose scores were where these go
+                    if (ok && gq >= (NT == 1 ? 2u : 1u)) ok = mbar_wait(&bars.s_read[t][back & 1], (back >> 1) & 1u, lim);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t ka = smem_u32(ring + (size_t)s * stage), t_s = tmem + (NT == 1 ? (gq & 1) : t) * 128;
+                    for (int g = 0; g < ng; ++g) {
+                        const uint64_t dq = umma_desc_k_sw128(qa + g * slab), dk = umma_desc_k_sw128(ka + g * (TK * 128));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (4 * g + k < ks) umma_bf16(t_s, dq + 2 * k, dk + 2 * k, id_qk, (g | k) != 0);
+                    }
+                    umma_commit(&bars.s_full[t][gq & 1]);
+                    umma_commit(&bars.kv_empty[s]);
+                    if (last) umma_commit(&bars.q_empty[qi]);
+                    ++gq;
+                    if (++s == nst) { s = 0; ph ^= 1u; }
+                };
+                for (int seg = 0; ok; ++seg) {
+                    ok = mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim);
+                    if (!ok) break;
+                    const CtSeg &w = s_seg[seg & (CT_SLOTS - 1)];
+                    if (w.whole < 0) break;
+                    const int first = w.tile, end = w.end;
+                    qi = nq == 2 ? seg & 1 : 0;
+                    ok = mbar_wait(&bars.q_full[qi], (uint32_t)((nq == 2 ? seg >> 1 : seg) & 1), lim);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (NT == 2 && (w.rt * NT + t) * ct.tpt >= p.T) {
+                        // no rows: the ring and the Q buffer are handed back in step with the other issuer, and the row threads are kept in step by a
+                        // tile's hand-offs without a tile
+                        mbar_arrive(&bars.q_empty[qi]);
+                        ok = mbar_wait(&bars.o_empty[t], (uint32_t)(lu & 1) ^ 1u, lim);
+                        if (ok && gq > 0) ok = mbar_wait(&bars.s_read[t][(gq - 1) & 1], ((gq - 1) >> 1) & 1u, lim);
+                        if (!ok) break;
+                        mbar_arrive(&bars.s_full[t][gq & 1]);
+                        for (int h = 0; h < NH; ++h) ok = ok && mbar_wait(&bars.p_full[t][gp & 1][h], (gp >> 1) & 1u, lim);
+                        if (!ok) break;
+                        mbar_arrive(&bars.o_done[t][gp & 1]);
+                        ++gq; ++gp; ++lu;
+                        for (int i = 0; i < 2 * (end - first) && ok; ++i) {
+                            ok = mbar_wait(&bars.kv_full[s], ph, lim);
+                            if (!ok) break;
+                            mbar_arrive(&bars.kv_empty[s]);
+                            if (++s == nst) { s = 0; ph ^= 1u; }
+                        }
+                        continue;
+                    }
+                    qa = smem_u32(q_smem + (size_t)(qi * NT + t) * ng * slab);
+                    qk(first + 1 == end);
+                    for (int i = first; i < end && ok; ++i, ++gp) {
+                        if (i + 1 < end) qk(i + 2 == end);
+                        ok = ok && mbar_wait(&bars.ready[s], ph, lim);   // V_i
+                        if (ok && i == first) ok = mbar_wait(&bars.o_empty[t], (uint32_t)(lu & 1) ^ 1u, lim);
+                        const uint32_t va = smem_u32(ring + (size_t)s * stage), pb = pa + (ct.np == 2 ? (gp & 1) * NH * slab : 0u);
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) {
+                            ok = ok && mbar_wait(&bars.p_full[t][gp & 1][h], (gp >> 1) & 1u, lim);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint64_t dp = umma_desc_k_sw128(pb + h * slab);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma_bf16(t_o, dp + 2 * k, umma_desc_mn_sw128(va + (4 * h + k) * 2048, TK * 128), id_pv, (i > first || h != 0 || k != 0) ? 1u : 0u);
+                        }
+                        if (!ok) break;
+                        umma_commit(&bars.o_done[t][gp & 1]);
+                        umma_commit(&bars.kv_empty[s]);
+                        if (++s == nst) { s = 0; ph ^= 1u; }
+                    }
+                    ++lu;
+                }
+                if (!ok) { report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 18)); failed = true; }
+            }
+        }
+    } else {
+        if (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CT_REGS_LARGE));
+        // ---- softmax and epilogue of row tile t; thread = row (tensor-memory lane) ----
+        const int t = (warp - 4) >> 2, q = warp & 3, row = 32 * q + lane;
+        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+        const uint32_t to = tl + 256u + (NT == 2 ? t * 128u : 0u);
+        const uint32_t prow = smem_u32(p_smem + (size_t)t * ct.np * NH * slab) + (uint32_t)row * 128u, sw = (uint32_t)(row & 7);
+        const float sl2 = p.scale_log2;
+        uint32_t g = 0;   // key tiles so far
+        uint32_t r[TK / 32][32];
+        auto pv_done = [&](uint32_t x) { return mbar_wait(&bars.o_done[t][x & 1], (x >> 1) & 1u, lim); };
+        for (int seg = 0; !failed; ++seg) {
+            CT_FAIL_AT(7, !mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim));
+            const CtSeg &w = s_seg[seg & (CT_SLOTS - 1)];
+            if (w.whole < 0) break;
+            const int tok0 = (w.rt * NT + t) * ct.tpt, rows = min(ct.tpt, p.T - tok0) * p.G;
+            if (NT == 2 && rows <= 0) {   // a tile's hand-offs (above)
+                CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&bars.s_read[t][g & 1]);
+                    for (int h = 0; h < NH; ++h) mbar_arrive(&bars.p_full[t][g & 1][h]);
+                }
+                CT_FAIL_AT(6, !pv_done(g));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.o_empty[t]);
+                ++g;
+                continue;
+            }
+            const bool act = 32 * q < rows;       // the same for a warp
+            const bool mine = row < rows;
+            const int tok = min(tok0 + row / p.G, p.T - 1);
+            float m_ref = -INFINITY, l = 0.0f;
+            const int first = w.tile, end = w.end, nct = w.ct;
+            for (int i = first; i < end; ++i, ++g) {
+                const bool draft = i >= nct;
+                const int j0 = (draft ? i - nct : i) * TK;
+                const bool part = draft || i + 1 == nct;   // (the same for every thread) keys that may not be there, or not be seen
+                uint32_t see[TK / 32];
+                if (part && act) {
+                    const int valid = !draft ? w.n - j0 : p.mask ? 0 : tok - j0 + 1;
+#pragma unroll
+                    for (int x = 0; x < TK / 32; ++x) see[x] = valid >= 32 * (x + 1) ? 0xffffffffu : valid <= 32 * x ? 0u : (1u << (valid - 32 * x)) - 1u;
+                    if (draft && p.mask && mine) {
+                        const unsigned char *mrow = p.mask + w.b * p.mask_b + (long long)tok * p.T + j0;
+                        const int n = min(TK, p.T - j0);
+#pragma unroll
+                        for (int x = 0; x < TK / 32; ++x) {
+                            uint32_t bits = 0;
+#pragma unroll 8
+                            for (int k = 0; k < 32; ++k)
+                                if (32 * x + k < n) bits |= (__ldg(mrow + 32 * x + k) != 0 ? 1u : 0u) << k;
+                            see[x] = bits;
+                        }
+                    }
+                }
+                CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                tc_fence_after();
+                const uint32_t ts = tl + (NT == 1 ? (g & 1) : t) * 128u;
+                if (act) {
+#pragma unroll
+                    for (int x = 0; x < TK / 32; ++x) tmem_ld32(ts + 32 * x, r[x]);
+                    tmem_ld_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.s_read[t][g & 1]);   // these scores may be overwritten
+                if (act) {
+                    if (part) {
+#pragma unroll
+                        for (int x = 0; x < TK / 32; ++x)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (!(see[x] >> k & 1u)) r[x][k] = 0xff800000u;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+#pragma unroll
+                        for (int x = 0; x < TK / 32; ++x) mx[(x + (TK == 64 ? 2 * (k & 1) : 0)) & 3] = fmaxf(mx[(x + (TK == 64 ? 2 * (k & 1) : 0)) & 3], __uint_as_float(r[x][k]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                    if (i == first) {
+                        m_ref = top;
+                    } else {
+                        const bool need = mine && top > m_ref + CT_RESCALE_LOG2;
+                        if (__any_sync(0xffffffffu, need)) {
+                            CT_FAIL_AT(4, !pv_done(g - 1));
+                            tc_fence_after();
+                            const float m_new = need ? top : m_ref;
+                            const float f = need ? fast_exp2(m_ref - m_new) : 1.0f;   // (0 where the row had seen nothing)
+                            uint32_t o[16];
+                            for (int c = 0; c < p.D; c += 16) {
+                                tmem_ld16(to + c, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tmem_st16(to + c, o);
+                            }
+                            tmem_st_wait();
+                            l *= f;
+                            m_ref = m_new;
+                        }
+                    }
+                }
+                const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;   // a row that has seen nothing: every score is -inf
+                if (g >= (uint32_t)ct.np) CT_FAIL_AT(5, !pv_done(g - ct.np));   // the MMAs have read what was in this P buffer
+                const uint32_t pw = prow + (ct.np == 2 ? (g & 1) * NH * slab : 0u);
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    if (act) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int e = 8 * (c & 3) + 2 * k;
+                                const float e0 = fast_exp2(fmaf(__uint_as_float(r[2 * h + (c >> 2)][e]), sl2, neg)), e1 = fast_exp2(fmaf(__uint_as_float(r[2 * h + (c >> 2)][e + 1]), sl2, neg));
+                                sum0 += e0; sum1 += e1;
+                                pk[k] = pack_16x2(e0, e1, F16);
+                            }
+                            if (row < ct.rows8) ct_st_shared_v4(pw + h * slab + ((((uint32_t)c) ^ sw) << 4), pk[0], pk[1], pk[2], pk[3]);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.p_full[t][g & 1][h]);
+                }
+                l += sum0 + sum1;
+            }
+            if (failed) break;
+            // ---- epilogue of the unit ----
+            CT_FAIL_AT(6, !pv_done(g - 1));
+            tc_fence_after();
+            if (act) {
+                const bool whole = w.whole != 0, bad = s_bad[seg & (CT_SLOTS - 1)] == seg + 1;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int hq = w.h * p.G + row % p.G;
+                float *prt = p.part + ((size_t)blockIdx.x * 2 + (seg == 0 ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
+                const int urow = t * ct.tpt * p.G + row;   // row of the unit
+                T *o = ca_row<T>(p.O, p.o, w.b, hq, tok);
+                for (int c = 0; c < p.D; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(to + c, v);
+                    tmem_ld_wait();
+                    if (bad && mine) {   // values that are not finite, for the rows that see them
+                        for (int j = max(first - nct, 0) * TK; j < min(p.T, (end - nct) * TK); ++j) {
+                            if (p.mask ? p.mask[w.b * p.mask_b + (long long)tok * p.T + j] == 0 : j > tok) continue;
+                            const T *vd = ca_row<T>(p.Vd, p.vd, w.b, w.h, j);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const float x = c + k < p.D ? to_f32(vd[c + k]) : 0.0f;
+                                if (!(fabsf(x) < INFINITY)) v[k] = __float_as_uint(__uint_as_float(v[k]) + x);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; k += 8) {
+                        if (!mine || c + k >= p.D) break;
+                        if (whole) {
+                            uint4 x;
+                            x.x = pack_16x2(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv, F16);
+                            x.y = pack_16x2(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv, F16);
+                            x.z = pack_16x2(__uint_as_float(v[k + 4]) * inv, __uint_as_float(v[k + 5]) * inv, F16);
+                            x.w = pack_16x2(__uint_as_float(v[k + 6]) * inv, __uint_as_float(v[k + 7]) * inv, F16);
+                            *reinterpret_cast<uint4 *>(o + c + k) = x;
+                        } else {
+                            float4 *d = reinterpret_cast<float4 *>(prt + (size_t)urow * p.D + c + k);
+                            d[0] = make_float4(__uint_as_float(v[k]), __uint_as_float(v[k + 1]), __uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]));
+                            d[1] = make_float4(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5]), __uint_as_float(v[k + 6]), __uint_as_float(v[k + 7]));
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (mine) {
+                    if (!whole) {
+                        prt[(size_t)p.RT * p.D + 2 * urow] = m_ref;
+                        prt[(size_t)p.RT * p.D + 2 * urow + 1] = l;
+                    } else if (p.lse) {
+                        p.lse[((long long)w.b * p.Hq + hq) * p.T + tok] = l == 0.0f ? -INFINITY : (m_ref + log2f(l)) * 0.69314718055994531f;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.o_empty[t]);
+        }
+    }
+
+    if (failed) for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // let copies and MMAs in flight drain
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, 512);
+}
+#undef CT_FAIL_AT
+
+// ---- host: tensor maps ----------------------------------------------------------------------------------------------------
+// [B, heads, rows, D] as {D, rows, heads, B}, boxes of 64 columns x `box_rows`; what lies outside reads as 0.  A dimension of size 1 has no stride to speak of.
+inline bool ct_map_rows(CUtensorMap *m, const void *base, const CaView &v, int B, int H, long long L, int D, int box_rows) {
+    PFN_tmapEncodeTiled enc = tmap_encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
+    cuuint64_t st[3] = {(cuuint64_t)(L == 1 ? 512 : v.l * 2), (cuuint64_t)(H == 1 ? 512 : v.h * 2), (cuuint64_t)(B == 1 ? 512 : v.b * 2)};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Q [B, Hkv * G, T, D] as {D, G, T, Hkv, B}: a box of G x box_t rows is a row tile, row t G + g.
+inline bool ct_map_q(CUtensorMap *m, const void *base, const CaView &v, int B, int Hkv, int G, int T, int D, int box_t) {
+    PFN_tmapEncodeTiled enc = tmap_encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[5] = {(cuuint64_t)D, (cuuint64_t)G, (cuuint64_t)T, (cuuint64_t)Hkv, (cuuint64_t)B};
+    cuuint64_t st[4] = {(cuuint64_t)(G == 1 ? 512 : v.h * 2), (cuuint64_t)(T == 1 ? 512 : v.l * 2), (cuuint64_t)(Hkv == 1 ? 512 : v.h * G * 2),
+                        (cuuint64_t)(B == 1 ? 512 : v.b * 2)};
+    cuuint32_t box[5] = {64, (cuuint32_t)G, (cuuint32_t)box_t, 1, 1}, es[5] = {1, 1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace b200attn
