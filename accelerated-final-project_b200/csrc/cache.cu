@@ -3,7 +3,7 @@
 #include <cstring>
 
 #include "host.h"
-#include "cache_tc.cuh"
+#include "cache_narrow.cuh"
 
 namespace b200attn {
 namespace {
@@ -159,6 +159,23 @@ bool tc_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CtPa
     *out = ct;
     return true;
 }
+// The kernel for up to 64 rows a key head.
+bool narrow_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CnParams *out) {
+    if (a->dtype == B200ATTN_F32 || p.D % 8 != 0 || p.R > 64 || (a->flags & B200ATTN_FLAG_FORCE_GENERIC)) return false;
+    CnParams cn{};
+    cn.ng = (p.D + 63) / 64;
+    cn.nh = (cn.ng + 1) / 2;
+    cn.gp = cn.ng < 2 ? 1 : 2;
+    const int N = p.R <= 16 ? 16 : p.R <= 32 ? 32 : 64, cols = 2 * N + 2 * cn.nh * N;
+    for (cn.tmem_cols = 32; cn.tmem_cols < cols; cn.tmem_cols *= 2) {}
+    const size_t room = c.max_smem - 4096 - 1024, front = cn_front_bytes(N, cn.ng);
+    cn.nst = (int)((room - front) / ((size_t)cn.gp * CN_GROUP));
+    if (cn.nst > CT_MAX_STAGES) cn.nst = CT_MAX_STAGES;
+    share_out(p, p.R, CN_TK, c.sm_count);
+    cn.a = p;
+    *out = cn;
+    return true;
+}
 bool tc_aligned(const b200attn_attend_args *a) {
     auto fine = [&](const b200attn_view &v, long long h, long long l) {   // a dimension of size 1 has no stride to speak of; the others are not 0
         b200attn_view x = v;
@@ -189,6 +206,24 @@ int launch_attend_tc(const CtParams &ct, const CUtensorMap (&m)[5], cudaStream_t
     return B200ATTN_OK;
 }
 
+template <int N, bool F16>
+int launch_narrow(const CnParams &cn, const CUtensorMap (&m)[5], cudaStream_t st) {
+    const size_t smem = cn_front_bytes(N, cn.ng) + (size_t)cn.nst * cn.gp * CN_GROUP + 1024;
+    int rc = raise_smem((const void *)ca_narrow_kernel<N, F16>, smem);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_narrow_kernel<N, F16>, dim3((unsigned)cn.a.grid), CN_THREADS, smem, 1, st, m[0], m[1], m[2], m[3], m[4], cn));
+    return B200ATTN_OK;
+}
+template <bool F16>
+int launch_attend_narrow(const CnParams &cn, const CUtensorMap (&m)[5], cudaStream_t st) {
+    const CaParams &p = cn.a;
+    int rc = p.R <= 16 ? launch_narrow<16, F16>(cn, m, st) : p.R <= 32 ? launch_narrow<32, F16>(cn, m, st) : launch_narrow<64, F16>(cn, m, st);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    count_launches(2);
+    return B200ATTN_OK;
+}
+
 int attend(const b200attn_attend_args *a, size_t *need) {
     int rc = validate(a, need == nullptr);
     if (rc) return rc;
@@ -199,20 +234,23 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     fill(p, *a);
     p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
     CtParams ct;
-    bool tc = tc_shape(a, c, p, &ct);
+    CnParams cn;
+    bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
     share_out(p, CG_ROWS, CG_KEYS, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
     // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
     size_t bytes = attend_bytes(p);
-    if (tc && attend_bytes(ct.a) > bytes) bytes = attend_bytes(ct.a);
+    const size_t other = narrow ? attend_bytes(cn.a) : tc ? attend_bytes(ct.a) : 0;
+    if (other > bytes) bytes = other;
     if (need) { *need = bytes; return B200ATTN_OK; }
-    tc = tc && tc_aligned(a);
     CUtensorMap m[5];
-    if (tc) {
+    if (narrow || tc) {
+        const CaParams &q = narrow ? cn.a : ct.a;
         memset(m, 0, sizeof m);
-        const CaParams &q = ct.a;
-        tc = ct_map_q(&m[0], q.Q, q.q, q.B, q.Hkv, q.G, q.T, q.D, ct.box_t) && ct_map_rows(&m[1], q.K, q.k, q.B, q.Hkv, q.S, q.D, q.TK) &&
-             ct_map_rows(&m[2], q.V, q.v, q.B, q.Hkv, q.S, q.D, q.TK) &&
-             (!q.drafts || (ct_map_rows(&m[3], q.Kd, q.kd, q.B, q.Hkv, q.T, q.D, q.TK) && ct_map_rows(&m[4], q.Vd, q.vd, q.B, q.Hkv, q.T, q.D, q.TK)));
+        const bool maps = tc_aligned(a) && ct_map_q(&m[0], q.Q, q.q, q.B, q.Hkv, q.G, q.T, q.D, narrow ? q.T : ct.box_t) &&
+                          ct_map_rows(&m[1], q.K, q.k, q.B, q.Hkv, q.S, q.D, q.TK) && ct_map_rows(&m[2], q.V, q.v, q.B, q.Hkv, q.S, q.D, q.TK) &&
+                          (!q.drafts || (ct_map_rows(&m[3], q.Kd, q.kd, q.B, q.Hkv, q.T, q.D, q.TK) && ct_map_rows(&m[4], q.Vd, q.vd, q.B, q.Hkv, q.T, q.D, q.TK)));
+        narrow = narrow && maps;
+        tc = tc && maps;
     }
     void *ws = a->workspace;
     if (ws) {
@@ -221,13 +259,14 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     } else if ((rc = host_workspace(&c, bytes, st, &ws))) {
         return rc;
     }
-    CaParams &q = tc ? ct.a : p;
+    CaParams &q = narrow ? cn.a : tc ? ct.a : p;
     q.part = (float *)ws;
     q.entries = (int *)((char *)ws + attend_bytes(q) - (size_t)q.grid * 8 * sizeof(int));
-    if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, m, st) : launch_attend_tc<false>(ct, m, st);
+    if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, m, st) : launch_attend_narrow<false>(cn, m, st);
+    else if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, m, st) : launch_attend_tc<false>(ct, m, st);
     else rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, st) : launch_attend<__nv_bfloat16>(p, st);
     if (rc) return rc;
-    set_last_path(tc ? "cache_tc" : "cache_generic");
+    set_last_path(narrow ? "cache_narrow" : tc ? "cache_tc" : "cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 

@@ -16,6 +16,8 @@
 // Warps of rows that do not exist only keep the hand-offs in step.  Every wait is bounded; one that expires sets the error word.
 #pragma once
 
+#include <type_traits>
+
 #include "cache.cuh"
 
 namespace b200attn {
@@ -75,6 +77,52 @@ template <> struct CtType<true> { using T = __half; };
 
 // Bytes of shared memory in front of the ring: Q buffers, then P buffers.
 __host__ __device__ inline size_t ct_front_bytes(int NT, int nq, int np, int ng, int rows8, int TK) { return (size_t)NT * ((size_t)nq * ng + (size_t)np * (TK / 64)) * rows8 * 128; }
+
+// By one warp, on a V tile in shared memory ([groups][rows of 128 B]): rows from `first` on are set to 0 ...
+__device__ __forceinline__ void ct_clear_rows(unsigned char *tile, int groups, int rows, int first, int lane) {
+    const int per = (rows - first) * 8;   // 16-byte pieces of a group
+    for (int g = 0; g < groups; ++g)
+        for (int x = lane; x < per; x += 32) *reinterpret_cast<uint4 *>(tile + (size_t)g * rows * 128 + first * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+}
+// ... and values that are not finite among the first `n` rows are set to 0.  True where there were any.  The look at all of them is a multiply-add
+// with 0 per pair, whose sum stays 0 unless one is not finite (11 thousand clocks a tile of 128 x 128 became 1 thousand against comparing each).
+template <bool F16>
+__device__ __forceinline__ bool ct_take_out(unsigned char *tile, int groups, int rows, int n, int lane) {
+    using T2 = typename std::conditional<F16, __half2, __nv_bfloat162>::type;
+    const int per = n * 8;
+    uint32_t zero = 0;
+    T2 acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = *reinterpret_cast<T2 *>(&zero);
+    const T2 z = acc[0];
+    for (int g = 0; g < groups; ++g) {
+        const unsigned char *base = tile + (size_t)g * rows * 128;
+        for (int x0 = lane; x0 < per; x0 += 256) {
+            uint4 a[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) a[k] = x0 + 32 * k < per ? *reinterpret_cast<const uint4 *>(base + (x0 + 32 * k) * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                acc[0] = __hfma2(*reinterpret_cast<T2 *>(&a[k].x), z, acc[0]);
+                acc[1] = __hfma2(*reinterpret_cast<T2 *>(&a[k].y), z, acc[1]);
+                acc[2] = __hfma2(*reinterpret_cast<T2 *>(&a[k].z), z, acc[2]);
+                acc[3] = __hfma2(*reinterpret_cast<T2 *>(&a[k].w), z, acc[3]);
+            }
+        }
+    }
+    const T2 sum = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
+    const float2 f = F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&sum)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&sum));
+    if (!__any_sync(0xffffffffu, !(f.x + f.y == 0.0f))) return false;
+    for (int g = 0; g < groups; ++g)
+        for (int x = lane; x < per; x += 32) {
+            uint4 *at = reinterpret_cast<uint4 *>(tile + (size_t)g * rows * 128 + x * 16);
+            const uint4 a = *at;
+            *at = make_uint4(ct_finite<F16>(a.x), ct_finite<F16>(a.y), ct_finite<F16>(a.z), ct_finite<F16>(a.w));
+        }
+    fence_proxy_async_smem();
+    return true;
+}
 
 #define CT_FAIL_AT(site, cond)                                                                          \
     if (cond) {                                                                                         \
@@ -200,27 +248,8 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 if (!ok) return;
                 const bool draft = i >= nct;
                 unsigned char *tile = ring + (size_t)s * stage;
-                if (v && !draft && n - i * TK < TK) {
-                    const int first = max(n - i * TK, 0), per = (TK - first) * 8;   // 16-byte pieces of a group
-                    for (int g = 0; g < ng; ++g)
-                        for (int x = lane; x < per; x += 32) *reinterpret_cast<uint4 *>(tile + (size_t)g * (TK * 128) + first * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                } else if (v && draft) {
-                    const int per = min(TK, p.T - (i - nct) * TK) * 8;
-                    bool bad = false;
-                    for (int g = 0; g < ng; ++g)
-#pragma unroll 4
-                        for (int x = lane; x < per; x += 32) {
-                            uint4 *at = reinterpret_cast<uint4 *>(tile + (size_t)g * (TK * 128) + x * 16);
-                            const uint4 a = *at;
-                            const uint4 c = make_uint4(ct_finite<F16>(a.x), ct_finite<F16>(a.y), ct_finite<F16>(a.z), ct_finite<F16>(a.w));
-                            if (a.x != c.x || a.y != c.y || a.z != c.z || a.w != c.w) { *at = c; bad = true; }
-                        }
-                    if (__any_sync(0xffffffffu, bad)) {
-                        if (lane == 0) s_bad[seg & (CT_SLOTS - 1)] = seg + 1;
-                        fence_proxy_async_smem();
-                    }
-                }
+                if (v && !draft && n - i * TK < TK) ct_clear_rows(tile, ng, TK, max(n - i * TK, 0), lane);
+                if (v && draft && ct_take_out<F16>(tile, ng, TK, min(TK, p.T - (i - nct) * TK), lane) && lane == 0) s_bad[seg & (CT_SLOTS - 1)] = seg + 1;
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(&bars.ready[s]); mbar_arrive(&bars.kv_empty[s]); }
                 if (++s == nst) { s = 0; ph ^= 1u; }
