@@ -276,40 +276,40 @@ def _refuse(message):
     raise B200AttnError(_INVALID_ARG, message)
 
 
+# (a short call is bound by these functions, as above: 22 us of which the two launches take 5, one token over 777 cached rows, with the checks
+# spread over more attribute look-ups; shapes are compared as tuples, and what a function has allocated itself is not checked)
 def _view(t, name, shape, dtype, dev):
     """(address, strides of sequence, head and row) of a [B, heads, rows, D] tensor, after its checks."""
-    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 4:
-        _refuse(f"{name} must be a 4-dimensional {dtype} tensor on device {dev}")
-    if t.shape != shape:
-        _refuse(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
-    sb, sh, sl, sd = t.stride()
-    if sd != 1 and shape[3] != 1:
+    if t.dtype is dtype and t.get_device() == dev and t.shape == shape:
+        s = t.stride()
+        if s[3] == 1 or shape[3] == 1:
+            return t.data_ptr(), s[0], s[1], s[2]
         _refuse(f"the last dimension of {name} must be contiguous")
-    return t.data_ptr(), sb, sh, sl
+    _refuse(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on device {dev}, got {t.dtype}, {tuple(t.shape)} on {t.device}")
 
 
 def _dense(t, name, shape, dtype, dev):
     """Address of a dense tensor (0 for None), after its checks."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
-        _refuse(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on device {dev}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on device {dev}, got {t.dtype}, {tuple(t.shape)} on {t.device}")
 
 
 def _cache_shape(K):
     torch = _torch or _with_torch()
-    if not K.is_cuda or K.dim() != 4 or K.dtype not in _DTYPES:
+    shape, dev = K.shape, K.get_device()
+    if dev < 0 or len(shape) != 4 or K.dtype not in _DTYPES:
         _refuse("the cache must be a 4-dimensional float32, bfloat16 or float16 CUDA tensor [B, heads, rows, D]")
-    return torch, K.get_device(), K.shape
+    return torch, dev, shape
 
 
 def _call_on(dev, fn, packed):
-    torch = _torch
-    if dev == torch.cuda.current_device():
+    if dev == _torch._C._cuda_getDevice():
         status = fn(packed)
     else:
-        with torch.cuda.device(dev):
+        with _torch.cuda.device(dev):
             status = fn(packed)
     if status != OK:
         check(status)
@@ -325,6 +325,7 @@ def _elsewhere(stream, dev):
 
 
 _attend_ws = {}   # bytes of workspace by the sizes they depend on
+_NO_VIEWS = (0,) * 8
 
 
 def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=None, lse=None, stream=None, flags=0):
@@ -332,48 +333,58 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
     [B, Hkv, T, D] where mask [B or 1, T, T] (uint8 or bool) is not 0; without a mask token t sees the tokens u <= t; without Kd and Vd the cache alone
     (an encoder's states).  Tensors may be views whose last dimension is contiguous.  Returns (out [B, Hq, T, D], lse [B, Hq, T] float32)
     (b200attn_cache_attend).  The workspace comes from torch's allocator: calls on different streams do not share it."""
-    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
-    at = _elsewhere(stream, dev)
-    if at is not None:
+    torch, dev, k_shape = _cache_shape(K)
+    if stream is not None and (at := _elsewhere(stream, dev)) is not None:
         with torch.cuda.stream(at):
             return cache_attend(Q, K, V, length, Kd, Vd, mask, scale, out, lse, None, flags)
-    if Q.dim() != 4 or not Q.is_cuda:
-        _refuse("Q must be a 4-dimensional CUDA tensor [B, heads, new tokens, D]")
-    Hq, T = Q.shape[1], Q.shape[2]
-    dtype, q_shape = K.dtype, (B, Hq, T, D)
+    q_shape, dtype = Q.shape, K.dtype
+    if len(q_shape) != 4:
+        _refuse("Q must be a 4-dimensional tensor [B, heads, new tokens, D]")
+    B, Hkv, S, D = k_shape
+    _, Hq, T, _ = q_shape
+    q = _view(Q, "Q", (B, Hq, T, D), dtype, dev)
+    device = Q.device
     if out is None:
         out = torch.empty_like(Q)
+        s = out.stride()
+        o = out.data_ptr(), s[0], s[1], s[2]
+    else:
+        o = _view(out, "out", q_shape, dtype, dev)
     if lse is None:
-        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=Q.device)
-    if (Kd is None) != (Vd is None):
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        lse_at = lse.data_ptr()
+    else:
+        lse_at = _dense(lse, "lse", (B, Hq, T), torch.float32, dev)
+    if Kd is not None and Vd is not None:
+        d_shape = (B, Hkv, T, D)
+        d = *_view(Kd, "Kd", d_shape, dtype, dev), *_view(Vd, "Vd", d_shape, dtype, dev)
+    elif Kd is not None or Vd is not None:
         _refuse("Kd and Vd must be given together")
-    none = (0, 0, 0, 0)
+    else:
+        d = _NO_VIEWS
     mask_at = mask_b = 0
     if mask is not None:
+        m_shape = mask.shape
         if mask.dtype not in (torch.uint8, torch.bool) or mask.get_device() != dev or not mask.is_contiguous() or \
-                tuple(mask.shape) not in ((B, T, T), (1, T, T), (T, T)):
+                m_shape not in ((B, T, T), (1, T, T), (T, T)):
             _refuse(f"mask must be a contiguous uint8 or bool tensor of shape {(B, T, T)}, {(1, T, T)} or {(T, T)} on device {dev}")
-        mask_at, mask_b = mask.data_ptr(), T * T if mask.dim() == 3 and mask.shape[0] == B else 0
-    stream = torch._C._cuda_getCurrentRawStream(dev)
+        mask_at, mask_b = mask.data_ptr(), T * T if len(m_shape) == 3 and m_shape[0] == B else 0
     L = _lib or lib()
-    head = _view(Q, "Q", q_shape, dtype, dev) + _view(K, "K", K.shape, dtype, dev) + _view(V, "V", K.shape, dtype, dev) + \
-        (none + none if Kd is None else _view(Kd, "Kd", (B, Hkv, T, D), dtype, dev) + _view(Vd, "Vd", (B, Hkv, T, D), dtype, dev)) + \
-        _view(out, "out", q_shape, dtype, dev) + (_dense(lse, "lse", (B, Hq, T), torch.float32, dev),
-                                                  _dense(length, "length", (B,), torch.int32, dev), mask_at, mask_b,
-                                                  B, Hq, Hkv, T, S, D, _DTYPES[dtype], scale)
-    # the size goes by shapes, alignment and the device: kept per combination of them, it costs no second call
-    key = (dev, dtype, B, Hq, Hkv, T, S, D, Kd is None, mask is None, flags)
+    filled = *q, *_view(K, "K", k_shape, dtype, dev), *_view(V, "V", k_shape, dtype, dev), *d, *o, lse_at, _dense(length, "length", (B,), torch.int32, dev), \
+        mask_at, mask_b, B, Hq, Hkv, T, S, D, _DTYPES[dtype], scale
+    # the size goes by the shapes and the device: kept per combination of them, it costs no second call
+    key = dev, dtype, q_shape, k_shape, Kd is None, mask is None, flags
     need = _attend_ws.get(key)
     if need is None:
         with torch.cuda.device(dev):
-            need = L.b200attn_cache_attend_workspace(_pack_attend(*head, 0, 0, 0, flags))
+            need = L.b200attn_cache_attend_workspace(_pack_attend(*filled, 0, 0, 0, flags))
         if need == 0:
             _refuse(L.b200attn_last_error().decode())
         if len(_attend_ws) >= 4096:
             _attend_ws.clear()
         _attend_ws[key] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=Q.device)
-    _call_on(dev, L.b200attn_cache_attend, _pack_attend(*head, ws.data_ptr(), need, stream, flags))
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call_on(dev, L.b200attn_cache_attend, _pack_attend(*filled, ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(dev), flags))
     return out, lse
 
 
@@ -381,9 +392,9 @@ def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, ne
     """The accepted ones of T new tokens (accepted [B, A] int32, padded with -1; None: all) become rows of the cache from row length[b] on:
     K, V [B, Hkv, S, D] are written from Kd, Vd [B, Hkv, T, D], weights [B, Hkv, S] with 0, pos [B, Hkv, S] with next_pos[b] + i.  Returns the new
     lengths [B] (int32); `length` stays (b200attn_cache_commit)."""
-    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
-    at = _elsewhere(stream, dev)
-    if at is not None:
+    torch, dev, k_shape = _cache_shape(K)
+    B, Hkv, S, D = k_shape
+    if stream is not None and (at := _elsewhere(stream, dev)) is not None:
         with torch.cuda.stream(at):
             return cache_commit(K, V, length, Kd, Vd, accepted, weights, pos, next_pos, None, flags)
     if Kd.dim() != 4 or (accepted is not None and accepted.dim() != 2):
@@ -393,7 +404,7 @@ def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, ne
     out = torch.empty((B,), dtype=i32, device=K.device)
     stream = torch._C._cuda_getCurrentRawStream(dev)
     d_shape = (B, Hkv, T, D)
-    packed = _pack_commit(*_view(K, "K", K.shape, dtype, dev), *_view(V, "V", K.shape, dtype, dev), *_view(Kd, "Kd", d_shape, dtype, dev),
+    packed = _pack_commit(*_view(K, "K", k_shape, dtype, dev), *_view(V, "V", k_shape, dtype, dev), *_view(Kd, "Kd", d_shape, dtype, dev),
                           *_view(Vd, "Vd", d_shape, dtype, dev), _dense(length, "length", (B,), i32, dev), out.data_ptr(),
                           _dense(accepted, "accepted", (B, A), i32, dev), A, _dense(weights, "weights", (B, Hkv, S), torch.float32, dev),
                           _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev), B, Hkv, T, S, D, _DTYPES[dtype],
@@ -406,9 +417,9 @@ def cache_weights(Q, K, length, lse, weights, accepted=None, scale=0.0, stream=N
     """Adds to weights [B, Hkv, S] the attention weight that each cached row had from the accepted tokens, which are the cache's last rows by now:
     Q [B, Hq, T, D] and lse [B, Hq, T] are those of the cache_attend call, `length` and `accepted` those after and of cache_commit.  Returns
     `weights` (b200attn_cache_weights)."""
-    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
-    at = _elsewhere(stream, dev)
-    if at is not None:
+    torch, dev, k_shape = _cache_shape(K)
+    B, Hkv, S, D = k_shape
+    if stream is not None and (at := _elsewhere(stream, dev)) is not None:
         with torch.cuda.stream(at):
             return cache_weights(Q, K, length, lse, weights, accepted, scale, None, flags)
     if Q.dim() != 4 or (accepted is not None and accepted.dim() != 2):
@@ -418,7 +429,7 @@ def cache_weights(Q, K, length, lse, weights, accepted=None, scale=0.0, stream=N
     stream = torch._C._cuda_getCurrentRawStream(dev)
     if length is None or lse is None or weights is None:
         _refuse("length, lse and weights must be given")
-    packed = _pack_weights(*_view(Q, "Q", (B, Hq, T, D), dtype, dev), *_view(K, "K", K.shape, dtype, dev), _dense(length, "length", (B,), torch.int32, dev),
+    packed = _pack_weights(*_view(Q, "Q", (B, Hq, T, D), dtype, dev), *_view(K, "K", k_shape, dtype, dev), _dense(length, "length", (B,), torch.int32, dev),
                            _dense(lse, "lse", (B, Hq, T), torch.float32, dev), _dense(accepted, "accepted", (B, A), torch.int32, dev), A,
                            _dense(weights, "weights", (B, Hkv, S), torch.float32, dev), B, Hq, Hkv, T, S, D, _DTYPES[dtype], scale, stream, flags)
     _call_on(dev, (_lib or lib()).b200attn_cache_weights, packed)
@@ -429,9 +440,9 @@ def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_po
     """Leaves at most `keep` rows in each head of the cache: the tokens of the first `sink` and the last `recent` positions, then the rows of largest
     weight.  In place, or into another cache (K, V, weights, pos; pos None where `pos` is None).  Returns (kept [B, Hkv, keep] int32: the former index
     of each row or -1, the new lengths [B]); `length` stays (b200attn_cache_evict)."""
-    torch, dev, (B, Hkv, S, D) = _cache_shape(K)
-    at = _elsewhere(stream, dev)
-    if at is not None:
+    torch, dev, k_shape = _cache_shape(K)
+    B, Hkv, S, D = k_shape
+    if stream is not None and (at := _elsewhere(stream, dev)) is not None:
         with torch.cuda.stream(at):
             return cache_evict(K, V, length, weights, keep, sink, recent, pos, next_pos, into, kept, None, flags)
     dtype, i32, f32 = K.dtype, torch.int32, torch.float32
@@ -450,7 +461,7 @@ def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_po
         o_shape = (B, Hkv, So, D)
         target = _view(Ko, "K of `into`", o_shape, dtype, dev) + _view(Vo, "V of `into`", o_shape, dtype, dev) + (
             _dense(Wo, "weights of `into`", (B, Hkv, So), f32, dev), _dense(Po, "pos of `into`", (B, Hkv, So), i32, dev))
-    packed = _pack_evict(*_view(K, "K", K.shape, dtype, dev), *_view(V, "V", K.shape, dtype, dev), _dense(weights, "weights", (B, Hkv, S), f32, dev),
+    packed = _pack_evict(*_view(K, "K", k_shape, dtype, dev), *_view(V, "V", k_shape, dtype, dev), _dense(weights, "weights", (B, Hkv, S), f32, dev),
                          _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(length, "length", (B,), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev),
                          out.data_ptr(), _dense(kept, "kept", (B, Hkv, max(keep, 0)), i32, dev), keep, sink, recent, *target, So, B, Hkv, S, D,
                          _DTYPES[dtype], stream, flags)

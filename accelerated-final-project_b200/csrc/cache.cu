@@ -1,4 +1,5 @@
 // Entry points of the key/value cache (include/b200attn.h, "A key/value cache"): checks of the arguments, choice of the kernel, launches.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -56,8 +57,16 @@ bool aligned16(const b200attn_view &v, int dtype) {
     return (((uintptr_t)v.ptr | (uintptr_t)(v.stride_b * e) | (uintptr_t)(v.stride_h * e) | (uintptr_t)(v.stride_l * e)) & 15) == 0;
 }
 
-int raise_smem(const void *kern, size_t bytes) {
-    if (bytes > 48 * 1024) CU_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// Lets a kernel have all the shared memory there is, once per device (asking each time costs a short call half a microsecond).
+template <auto Kern>
+int raise_smem(const HostCall &c) {
+    static std::atomic<unsigned long long> done{0};
+    const unsigned long long bit = 1ull << (c.dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return B200ATTN_OK;
+    cudaFuncAttributes fa;
+    CU_TRY(cudaFuncGetAttributes(&fa, Kern));
+    CU_TRY(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(c.max_smem - fa.sharedSizeBytes)));
+    done.fetch_or(bit, std::memory_order_release);
     return B200ATTN_OK;
 }
 
@@ -118,18 +127,18 @@ void fill(CaParams &p, const b200attn_attend_args &a) {
 }
 
 template <typename T, int DB>
-int launch_generic(const CaParams &p, cudaStream_t st) {
+int launch_generic(const CaParams &p, const HostCall &c, cudaStream_t st) {
     const size_t smem = cg_smem_bytes(p.D);
-    int rc = raise_smem((const void *)ca_generic_kernel<T, DB>, smem);
+    int rc = raise_smem<ca_generic_kernel<T, DB>>(c);
     if (rc) return rc;
     CU_TRY(launch_dependent(ca_generic_kernel<T, DB>, dim3((unsigned)p.grid), CG_THREADS, smem, 1, st, p));
     return B200ATTN_OK;
 }
 template <typename T>
-int launch_attend(const CaParams &p, cudaStream_t st) {
-    int rc = p.D <= 64 ? launch_generic<T, 64>(p, st) : p.D <= 128 ? launch_generic<T, 128>(p, st) : launch_generic<T, 256>(p, st);
+int launch_attend(const CaParams &p, const HostCall &c, cudaStream_t st) {
+    int rc = p.D <= 64 ? launch_generic<T, 64>(p, c, st) : p.D <= 128 ? launch_generic<T, 128>(p, c, st) : launch_generic<T, 256>(p, c, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    CU_TRY(launch_dependent(ca_combine_kernel<T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
     count_launches(2);
     return B200ATTN_OK;
 }
@@ -189,37 +198,37 @@ bool tc_aligned(const b200attn_attend_args *a) {
 }
 
 template <int NT, int TK, bool F16>
-int launch_tc(const CtParams &ct, const CUtensorMap (&m)[5], cudaStream_t st) {
+int launch_tc(const CtParams &ct, const HostCall &c, const CUtensorMap (&m)[5], cudaStream_t st) {
     const size_t smem = ct_front_bytes(NT, ct.nq, ct.np, ct.ng, ct.rows8, TK) + (size_t)ct.nst * ct.ng * TK * 128 + 1024;
-    int rc = raise_smem((const void *)ca_tc_kernel<NT, TK, F16>, smem);
+    int rc = raise_smem<ca_tc_kernel<NT, TK, F16>>(c);
     if (rc) return rc;
     CU_TRY(launch_dependent(ca_tc_kernel<NT, TK, F16>, dim3((unsigned)ct.a.grid), ct_threads(NT), smem, 1, st, m[0], m[1], m[2], m[3], m[4], ct));
     return B200ATTN_OK;
 }
 template <bool F16>
-int launch_attend_tc(const CtParams &ct, const CUtensorMap (&m)[5], cudaStream_t st) {
+int launch_attend_tc(const CtParams &ct, const HostCall &c, const CUtensorMap (&m)[5], cudaStream_t st) {
     const CaParams &p = ct.a;
-    int rc = p.TK == 64 ? launch_tc<1, 64, F16>(ct, m, st) : p.RT > ct.tpt * p.G ? launch_tc<2, 128, F16>(ct, m, st) : launch_tc<1, 128, F16>(ct, m, st);
+    int rc = p.TK == 64 ? launch_tc<1, 64, F16>(ct, c, m, st) : p.RT > ct.tpt * p.G ? launch_tc<2, 128, F16>(ct, c, m, st) : launch_tc<1, 128, F16>(ct, c, m, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
     count_launches(2);
     return B200ATTN_OK;
 }
 
 template <int N, bool F16>
-int launch_narrow(const CnParams &cn, const CUtensorMap (&m)[5], cudaStream_t st) {
+int launch_narrow(const CnParams &cn, const HostCall &c, const CUtensorMap (&m)[5], cudaStream_t st) {
     const size_t smem = cn_front_bytes(N, cn.ng) + (size_t)cn.nst * cn.gp * CN_GROUP + 1024;
-    int rc = raise_smem((const void *)ca_narrow_kernel<N, F16>, smem);
+    int rc = raise_smem<ca_narrow_kernel<N, F16>>(c);
     if (rc) return rc;
     CU_TRY(launch_dependent(ca_narrow_kernel<N, F16>, dim3((unsigned)cn.a.grid), CN_THREADS, smem, 1, st, m[0], m[1], m[2], m[3], m[4], cn));
     return B200ATTN_OK;
 }
 template <bool F16>
-int launch_attend_narrow(const CnParams &cn, const CUtensorMap (&m)[5], cudaStream_t st) {
+int launch_attend_narrow(const CnParams &cn, const HostCall &c, const CUtensorMap (&m)[5], cudaStream_t st) {
     const CaParams &p = cn.a;
-    int rc = p.R <= 16 ? launch_narrow<16, F16>(cn, m, st) : p.R <= 32 ? launch_narrow<32, F16>(cn, m, st) : launch_narrow<64, F16>(cn, m, st);
+    int rc = p.R <= 16 ? launch_narrow<16, F16>(cn, c, m, st) : p.R <= 32 ? launch_narrow<32, F16>(cn, c, m, st) : launch_narrow<64, F16>(cn, c, m, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, (unsigned)((p.RT + 7) / 8)), CB_THREADS, 0, 1, st, p));
+    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
     count_launches(2);
     return B200ATTN_OK;
 }
@@ -262,9 +271,9 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CaParams &q = narrow ? cn.a : tc ? ct.a : p;
     q.part = (float *)ws;
     q.entries = (int *)((char *)ws + attend_bytes(q) - (size_t)q.grid * 8 * sizeof(int));
-    if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, m, st) : launch_attend_narrow<false>(cn, m, st);
-    else if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, m, st) : launch_attend_tc<false>(ct, m, st);
-    else rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, st) : launch_attend<__nv_bfloat16>(p, st);
+    if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, c, m, st) : launch_attend_narrow<false>(cn, c, m, st);
+    else if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, c, m, st) : launch_attend_tc<false>(ct, c, m, st);
+    else rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, c, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, c, st) : launch_attend<__nv_bfloat16>(p, c, st);
     if (rc) return rc;
     set_last_path(narrow ? "cache_narrow" : tc ? "cache_tc" : "cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
@@ -323,9 +332,9 @@ int commit(const b200attn_commit_args *a) {
 }
 
 template <typename T>
-int launch_weights(const CwParams &p, cudaStream_t st) {
+int launch_weights(const CwParams &p, const HostCall &c, cudaStream_t st) {
     const size_t smem = cg_smem_bytes(p.D);
-    int rc = raise_smem((const void *)cw_generic_kernel<T>, smem);
+    int rc = raise_smem<cw_generic_kernel<T>>(c);
     if (rc) return rc;
     CU_TRY(launch_dependent(cw_generic_kernel<T>, dim3((unsigned)((p.S + CG_KEYS - 1) / CG_KEYS), (unsigned)p.Hkv, (unsigned)p.B), CG_THREADS, smem, 1, st, p));
     count_launches(1);
@@ -357,7 +366,7 @@ int weights(const b200attn_weights_args *a) {
     p.A = A; p.B = a->batch_sz; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.G = G; p.T = a->len_new; p.S = a->capacity; p.D = a->head_d;
     p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_d) : a->scale) * 1.4426950408889634f;
     p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
-    rc = a->dtype == B200ATTN_F32 ? launch_weights<float>(p, st) : a->dtype == B200ATTN_F16 ? launch_weights<__half>(p, st) : launch_weights<__nv_bfloat16>(p, st);
+    rc = a->dtype == B200ATTN_F32 ? launch_weights<float>(p, c, st) : a->dtype == B200ATTN_F16 ? launch_weights<__half>(p, c, st) : launch_weights<__nv_bfloat16>(p, c, st);
     if (rc) return rc;
     set_last_path("cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
@@ -411,7 +420,7 @@ int evict(const b200attn_evict_args *a) {
     const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && p.row_bytes % 16 == 0 &&
                       (!into || (aligned16(a->K_out, a->dtype) && aligned16(a->V_out, a->dtype)));
     const size_t smem = ce_smem_bytes(p.S);
-    if ((rc = raise_smem((const void *)ce_select_kernel, smem))) return rc;
+    if ((rc = raise_smem<ce_select_kernel>(c))) return rc;
     CU_TRY(launch_dependent(ce_select_kernel, dim3((unsigned)p.Hkv, (unsigned)p.B), CE_THREADS, smem, 1, st, p));
     const int rows = CC_THREADS;   // of `kept` per block
     const dim3 grid((unsigned)((p.keep + (long long)rows - 1) / rows), (unsigned)p.Hkv, (unsigned)p.B);

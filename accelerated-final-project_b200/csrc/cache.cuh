@@ -168,63 +168,70 @@ __device__ __forceinline__ const T *ca_row(const void *base, const CaView &v, in
 }
 
 // ---- joining the parts of cut units ---------------------------------------------------------------------------------
-// Block (c, y): rows 8 y .. 8 y + 7 of the unit that entry c lists.  A row is taken by `per` warps that share its parts out, so that a row cut
-// over the whole chip (one sequence, one key head) does not wait for one part after the other.
-constexpr int CB_THREADS = 256;
+// Block (c, y): rows CB_ROWS y .. of the unit that entry c lists.  A row's warps first take all parts' (m, l), a part per lane, for the row's maximum and
+// sum; then the parts' accumulators with their weights, four requests in flight per column.  A row is taken by `per` warps that share its parts
+// out, so that a row cut over the whole chip (one sequence, one key head) does not wait for one part after the other.
+//   8 key heads x 4 rows in 7 parts each: 11 us with a dependent chain through (m, l, accumulator) of each part
+constexpr int CB_THREADS = 256, CB_ROWS = 16;
 
 template <typename T>
 __global__ void __launch_bounds__(CB_THREADS)
 ca_combine_kernel(const CaParams p) {
     __shared__ float s_acc[8][CA_MAX_D];
-    __shared__ float s_ml[8][2];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int *e = p.entries + (size_t)blockIdx.x * 8;
-    const int first = e[0];
+    const int4 e0 = *reinterpret_cast<const int4 *>(p.entries + (size_t)blockIdx.x * 8);
+    const int first = e0.x;
     if (first < 0) return;
-    const int slot0 = e[1], parts = e[2] - first + 1, b = e[3], h = e[4], rt = e[5];
-    const int rows = min(p.RT, p.R - rt * p.RT), row0 = blockIdx.y * 8;
-    if (row0 >= rows) return;
+    const int2 e1 = *reinterpret_cast<const int2 *>(p.entries + (size_t)blockIdx.x * 8 + 4);
+    const int slot0 = e0.y, parts = e0.z - first + 1, b = e0.w, h = e1.x, rt = e1.y;
+    const int rows = min(min(p.RT, p.R - rt * p.RT), (int)(blockIdx.y + 1) * CB_ROWS), row0 = blockIdx.y * CB_ROWS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = parts <= 12 ? 1 : parts <= 24 ? 2 : parts <= 48 ? 4 : 8;   // warps of a row
-    const size_t slot = ca_slot_floats(p.RT, p.D);
-    for (int r0 = 0; r0 < 8; r0 += 8 / per) {
-        const int row = row0 + r0 + warp / per;
+    const int per = parts <= 8 ? 1 : parts <= 16 ? 2 : parts <= 32 ? 4 : 8;   // warps of a row
+    const size_t slot = ca_slot_floats(p.RT, p.D), ml = (size_t)p.RT * p.D;
+    auto part = [&](int c) { return p.part + ((size_t)(first + c) * 2 + (c == 0 ? slot0 : 0)) * slot; };
+    for (int r0 = row0; r0 < rows; r0 += 8 / per) {
+        const int row = r0 + warp / per;
+        const bool mine = row < rows;
         float m = -INFINITY, l = 0.0f, acc[CA_MAX_D / 32];
 #pragma unroll
         for (int i = 0; i < CA_MAX_D / 32; ++i) acc[i] = 0.0f;
-        if (row < rows) {
-            for (int c = warp % per; c < parts; c += per) {
-                const float *ps = p.part + ((size_t)(first + c) * 2 + (c == 0 ? slot0 : 0)) * slot;
-                const float pm = ps[(size_t)p.RT * p.D + 2 * row], pl = ps[(size_t)p.RT * p.D + 2 * row + 1];
-                const float mn = fmaxf(m, pm);
-                const float f = mn == -INFINITY ? 0.0f : exp2f(m - mn), pf = mn == -INFINITY ? 0.0f : exp2f(pm - mn);
-                l = l * f + pl * pf;
-                m = mn;
+        if (mine) {
+            for (int c = lane; c < parts; c += 32) m = fmaxf(m, part(c)[ml + 2 * row]);
+            m = warp_max(m);
+            for (int c0 = 0; c0 < parts; c0 += 32) {
+                const int c = c0 + lane;
+                float w = 0.0f;
+                if (c < parts) {
+                    const float2 x = *reinterpret_cast<const float2 *>(part(c) + ml + 2 * row);
+                    w = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
+                    l += w * x.y;
+                }
+                const int n = min(32, parts - c0);
+#pragma unroll 4
+                for (int k = warp % per; k < n; k += per) {
+                    const float wk = __shfl_sync(0xffffffffu, w, k);
+                    const float *o = part(c0 + k) + (size_t)row * p.D;
 #pragma unroll
-                for (int i = 0; i < CA_MAX_D / 32; ++i)
-                    if (lane + 32 * i < p.D) acc[i] = acc[i] * f + ps[(size_t)row * p.D + lane + 32 * i] * pf;
+                    for (int i = 0; i < CA_MAX_D / 32; ++i)
+                        if (lane + 32 * i < p.D) acc[i] = fmaf(o[lane + 32 * i], wk, acc[i]);
+                }
             }
+            l = warp_sum(l);
         }
         if (per > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < CA_MAX_D / 32; ++i)
                 if (lane + 32 * i < p.D) s_acc[warp][lane + 32 * i] = acc[i];
-            if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
             __syncthreads();
             if (warp % per != 0) continue;
-            for (int w = warp + 1; w < warp + per; ++w) {
-                const float pm = s_ml[w][0], pl = s_ml[w][1], mn = fmaxf(m, pm);
-                const float f = mn == -INFINITY ? 0.0f : exp2f(m - mn), pf = mn == -INFINITY ? 0.0f : exp2f(pm - mn);
-                l = l * f + pl * pf;
-                m = mn;
+            for (int w = warp + 1; w < warp + per; ++w)
 #pragma unroll
                 for (int i = 0; i < CA_MAX_D / 32; ++i)
-                    if (lane + 32 * i < p.D) acc[i] = acc[i] * f + s_acc[w][lane + 32 * i] * pf;
-            }
+                    if (lane + 32 * i < p.D) acc[i] += s_acc[w][lane + 32 * i];
         }
-        if (row >= rows) continue;
+        if (!mine) continue;
         const int r = rt * p.RT + row, t = r / p.G, hq = h * p.G + r % p.G;
         T *o = ca_row<T>(p.O, p.o, b, hq, t);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -234,6 +241,7 @@ ca_combine_kernel(const CaParams p) {
         if (p.lse && lane == 0) p.lse[((long long)b * p.Hq + hq) * p.T + t] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
 }
+inline unsigned cb_blocks(const CaParams &p) { return (unsigned)(((p.RT < p.R ? p.RT : p.R) + CB_ROWS - 1) / CB_ROWS); }
 
 // ---- attention on the CUDA cores: every type, width and stride ---------------------------------------------------------
 // Units of 16 rows, tiles of 64 keys, 128 threads.  K and V pass through shared memory in fp32; a thread computes the scores of one key with
