@@ -107,8 +107,10 @@ int validate(const b200attn_attend_args *a, bool pointers) {
 // Workspace: the slots of cut units, then the entries.
 size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + (size_t)p.grid * 8 * sizeof(int); }
 
-void share_out(CaParams &p, int RT, int TK, int grid) {
-    p.RT = RT; p.TK = TK; p.grid = grid;
+#include <cstdlib>
+static int env_oh(int d) { const char *e = getenv("CA_OH"); return e ? atoi(e) : d; }
+void share_out(CaParams &p, int RT, int TK, int OH, int grid) {
+    p.RT = RT; p.TK = TK; p.OH = OH; p.grid = grid;
     p.nrt = (p.R + RT - 1) / RT;
     p.DT = 0;
     if (p.drafts)
@@ -163,7 +165,7 @@ bool tc_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CtPa
         if (ct.nst >= (i < 3 ? 4 : 3)) break;
     }
     if (ct.nst < 3) return false;
-    share_out(p, NT * ct.tpt * p.G, TK, c.sm_count);
+    share_out(p, NT * ct.tpt * p.G, TK, env_oh(4), c.sm_count);
     ct.a = p;
     *out = ct;
     return true;
@@ -180,7 +182,7 @@ bool narrow_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, 
     const size_t room = c.max_smem - 4096 - 1024, front = cn_front_bytes(N, cn.ng);
     cn.nst = (int)((room - front) / ((size_t)cn.gp * CN_GROUP));
     if (cn.nst > CT_MAX_STAGES) cn.nst = CT_MAX_STAGES;
-    share_out(p, p.R, CN_TK, c.sm_count);
+    share_out(p, p.R, CN_TK, env_oh(1), c.sm_count);
     cn.a = p;
     *out = cn;
     return true;
@@ -245,7 +247,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CtParams ct;
     CnParams cn;
     bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
-    share_out(p, CG_ROWS, CG_KEYS, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
+    share_out(p, CG_ROWS, CG_KEYS, env_oh(0), c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
     // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
     size_t bytes = attend_bytes(p);
     const size_t other = narrow ? attend_bytes(cn.a) : tc ? attend_bytes(ct.a) : 0;

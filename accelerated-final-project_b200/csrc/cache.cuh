@@ -6,7 +6,8 @@
 // One pass over the keys with a running maximum m and sum l: when m grows to m', l and the accumulator are multiplied by exp(m - m').
 // Parts over different keys join by the same rule.
 //
-// Sharing out: a unit is (sequence, key head, tile of RT rows); its items are the tiles of TK cached keys, then those of the new tokens' keys.
+// Sharing out: a unit is (sequence, key head, tile of RT rows); its items are the tiles of TK cached keys, then those of the new tokens' keys.  In front of
+// them stand OH items without work: what a unit's beginning and end cost a CTA, in tiles (short sequences would be taken for cheap otherwise).
 // The lengths are in device memory and differ, so no split can be chosen on the host: the items of all units, one after the other, are cut
 // into equal contiguous ranges, one per CTA, by each CTA for itself (a scan over the lengths).  A unit inside one range is finished there; one
 // that is cut leaves (accumulator, m, l) per row in the CTA's two slots of the workspace - only the first and the last unit of a range can be
@@ -32,7 +33,8 @@ struct CaParams {
     int B, Hq, Hkv, G, T, S, D;
     int R;               // rows of a key head: T * G
     int RT, nrt, TK;     // rows of a unit, units of a key head, keys of a tile
-    long long DT;        // items of new keys, summed over the units of a key head
+    int OH;              // items in front of a unit's tiles
+    long long DT;        // tiles of new keys, summed over the units of a key head
     int drafts;          // new keys are given
     int grid;            // CTAs that share the items out
     float scale_log2;    // scale * log2(e)
@@ -46,12 +48,12 @@ __host__ __device__ inline size_t ca_slot_floats(int RT, int D) { return ((size_
 
 // rows cached for a sequence
 __device__ __forceinline__ int ca_len(const int *len, int b, int S) { return min(max(__ldg(len + b), 0), S); }
-// items of cached keys (a call without new keys has one at least, so that every unit has an item)
+// tiles of cached keys (a call without new keys has one at least, so that every unit has a tile)
 __device__ __forceinline__ int ca_tiles(const CaParams &p, int n) {
     const int ct = (n + p.TK - 1) / p.TK;
     return p.drafts ? ct : max(ct, 1);
 }
-// items of new keys of unit rt: the last row of a chain sees its own token last
+// tiles of new keys of unit rt: the last row of a chain sees its own token last
 __host__ __device__ inline int ca_draft_tiles(int rt, int R, int RT, int G, int T, int TK, bool chain) {
     const long long end = (long long)(rt + 1) * RT;
     const int t = chain ? (int)(((end < R ? end : R) - 1) / G) + 1 : T;
@@ -71,7 +73,7 @@ __device__ __forceinline__ CaStart ca_locate(const CaParams &p, int c) {
     const int lane = threadIdx.x & 31;
     long long total = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-        long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * ca_tiles(p, ca_len(p.len, b0 + lane, p.S)) + p.DT) : 0;
+        long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * (p.OH + ca_tiles(p, ca_len(p.len, b0 + lane, p.S))) + p.DT) : 0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         total += x;
@@ -81,7 +83,7 @@ __device__ __forceinline__ CaStart ca_locate(const CaParams &p, int c) {
     const long long i0 = ca_range(total, s.grid, c);
     long long before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * ca_tiles(p, ca_len(p.len, b0 + lane, p.S)) + p.DT) : 0;
+        const long long x = b0 + lane < p.B ? (long long)p.Hkv * ((long long)p.nrt * (p.OH + ca_tiles(p, ca_len(p.len, b0 + lane, p.S))) + p.DT) : 0;
         long long incl = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -100,12 +102,18 @@ __device__ __forceinline__ CaStart ca_locate(const CaParams &p, int c) {
     return s;   // (not reached: i0 < total)
 }
 
-// The units of a CTA's range, one after the other; each role of a CTA keeps a walk of its own.
+// The units of a CTA's range, one after the other.
 struct CaWalk {
     long long left, u0;   // items left of the range; first item of the unit, counted over all
     int b, h, rt, n;      // the unit; rows cached
-    int tile, ct, nt;     // first item of this CTA in the unit; items of cached keys; all items
+    int at, ct, nt;       // first item of this CTA in the unit; tiles of cached keys; all tiles
     __device__ __forceinline__ void unit(const CaParams &p) { nt = ct + ca_draft_tiles(p, rt); }
+    __device__ __forceinline__ int tile(const CaParams &p) const { return max(at - p.OH, 0); }
+    __device__ __forceinline__ int end(const CaParams &p) const { return (int)min((long long)nt, at + left - p.OH); }
+    __device__ __forceinline__ bool whole(const CaParams &p) const { return at <= p.OH && at + left >= p.OH + nt; }
+    __device__ __forceinline__ void settle(const CaParams &p) {   // a range that ends before a unit's first tile has no part in it
+        if (at + left <= p.OH) left = 0;
+    }
     __device__ __forceinline__ void start(const CaParams &p, const CaStart &s, int c) {
         const long long i0 = ca_range(s.total, s.grid, c);
         left = c < s.grid ? ca_range(s.total, s.grid, c + 1) - i0 : 0;
@@ -113,24 +121,23 @@ struct CaWalk {
         b = s.b;
         n = ca_len(p.len, b, p.S);
         ct = ca_tiles(p, n);
-        const long long per = (long long)p.nrt * ct + p.DT;
+        const long long per = (long long)p.nrt * (p.OH + ct) + p.DT;
         h = (int)(s.rem / per);
         long long rem = s.rem % per;
         for (rt = 0;; ++rt) {
             unit(p);
-            if (rem < nt) break;
-            rem -= nt;
+            if (rem < p.OH + nt) break;
+            rem -= p.OH + nt;
         }
-        tile = (int)rem;
+        at = (int)rem;
         u0 = i0 - rem;
+        settle(p);
     }
-    __device__ __forceinline__ int end() const { return (int)min((long long)nt, tile + left); }
-    __device__ __forceinline__ bool whole() const { return tile == 0 && left >= nt; }
     __device__ __forceinline__ void next(const CaParams &p) {
-        left -= end() - tile;
+        left -= min(left, (long long)p.OH + nt - at);
         if (left == 0) return;
-        u0 += nt;
-        tile = 0;
+        u0 += p.OH + nt;
+        at = 0;
         if (++rt == p.nrt) {
             rt = 0;
             if (++h == p.Hkv) {
@@ -141,6 +148,7 @@ struct CaWalk {
             }
         }
         unit(p);
+        settle(p);
     }
 };
 
@@ -149,11 +157,11 @@ struct CaWalk {
 __device__ __forceinline__ void ca_entry(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
     int *e = p.entries + (size_t)c * 8;
     e[0] = -1;
-    if (w.left == 0 || w.tile == 0) return;
-    const int first = ca_cta_of(s.total, s.grid, w.u0);
-    if (ca_cta_of(s.total, s.grid, w.u0 + w.tile - 1) != first) return;
-    e[1] = ca_range(s.total, s.grid, first) == w.u0 ? 0 : 1;
-    e[2] = ca_cta_of(s.total, s.grid, w.u0 + w.nt - 1);
+    if (w.left == 0 || w.at <= p.OH) return;
+    const int first = ca_cta_of(s.total, s.grid, w.u0 + p.OH);
+    if (ca_cta_of(s.total, s.grid, w.u0 + w.at - 1) != first) return;
+    e[1] = ca_range(s.total, s.grid, first) >= w.u0 ? 0 : 1;
+    e[2] = ca_cta_of(s.total, s.grid, w.u0 + p.OH + w.nt - 1);
     e[3] = w.b; e[4] = w.h; e[5] = w.rt;
     e[0] = first;
 }
@@ -286,7 +294,7 @@ ca_generic_kernel(const CaParams p) {
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int r = 0; r < NR; ++r) acc[c][r] = 0.0f;
-        for (int tile = w.tile; tile < w.end(); ++tile) {
+        for (int tile = w.tile(p), end = w.end(p); tile < end; ++tile) {
             const bool draft = tile >= w.ct;
             const int j0 = (draft ? tile - w.ct : tile) * CG_KEYS, nk = min(CG_KEYS, (draft ? p.T : w.n) - j0);   // keys of the tile (0: an empty cache)
             __syncthreads();
@@ -358,7 +366,7 @@ ca_generic_kernel(const CaParams p) {
             }
         }
         __syncthreads();
-        const bool whole = w.whole();
+        const bool whole = w.whole(p);
         float *part = p.part + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {

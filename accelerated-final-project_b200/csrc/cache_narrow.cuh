@@ -130,15 +130,15 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             };
             int seg = 0;
             for (; w.left > 0 && ok; ++seg, w.next(p)) {
-                const int end = w.end(), qi = seg & 1;
-                s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, w.tile, end, w.ct, w.whole() ? 1 : 0};
+                const int first = w.tile(p), end = w.end(p), qi = seg & 1;
+                s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, first, end, w.ct, w.whole(p) ? 1 : 0};
                 mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
                 ok = mbar_wait(&bars.q_empty[qi], (uint32_t)(seg >> 1 & 1) ^ 1u, lim);
                 if (!ok) break;
                 mbar_expect_tx(&bars.q_full[qi], (uint32_t)(ng * p.R) * 128u);
                 for (int g = 0; g < ng; ++g) tma_load_5d(q_smem + (size_t)(qi * ng + g) * slab, &tmQ, g * 64, 0, 0, w.h, w.b, &bars.q_full[qi]);
-                load(false, w.tile);
-                for (int i = w.tile; i < end && ok; ++i) {
+                load(false, first);
+                for (int i = first; i < end && ok; ++i) {
                     if (i + 1 < end) load(false, i + 1);
                     load(true, i);
                 }

@@ -64,6 +64,29 @@ __device__ __forceinline__ void ct_st_shared_v4(uint32_t addr, uint32_t a, uint3
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Two fp32 operations in one instruction, and the largest of three values.
+__device__ __forceinline__ uint64_t ct_pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void ct_unpair(uint64_t x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t ct_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t ct_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ct_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // A pair of 16-bit values with those that are not finite set to 0.
 template <bool F16>
 __device__ __forceinline__ uint32_t ct_finite(uint32_t w) {
@@ -211,9 +234,9 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 };
                 int seg = 0;
                 for (; w.left > 0 && ok; ++seg, w.next(p)) {
-                    const int end = w.end();
+                    const int first = w.tile(p), end = w.end(p);
                     // (the slot's last unit is eight back: the ring has been handed back since by everybody who read it)
-                    s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, w.tile, end, w.ct, w.whole() ? 1 : 0};
+                    s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, first, end, w.ct, w.whole(p) ? 1 : 0};
                     mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
                     const int qi = nq == 2 ? seg & 1 : 0;
                     ok = mbar_wait(&bars.q_empty[qi], (uint32_t)((nq == 2 ? seg >> 1 : seg) & 1) ^ 1u, lim);
@@ -223,8 +246,8 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     for (int t = 0; t < nt; ++t)
                         for (int g = 0; g < ng; ++g)
                             tma_load_5d(q_smem + (size_t)((qi * NT + t) * ng + g) * slab, &tmQ, g * 64, 0, tok0 + t * ct.tpt, w.h, w.b, &bars.q_full[qi]);
-                    load(false, w.tile);
-                    for (int i = w.tile; i < end && ok; ++i) {
+                    load(false, first);
+                    for (int i = first; i < end && ok; ++i) {
                         if (i + 1 < end) load(false, i + 1);
                         load(true, i);
                     }
@@ -433,9 +456,13 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
+                    for (int k = 0; k < 32; k += 4)
 #pragma unroll
-                        for (int x = 0; x < TK / 32; ++x) mx[(x + (TK == 64 ? 2 * (k & 1) : 0)) & 3] = fmaxf(mx[(x + (TK == 64 ? 2 * (k & 1) : 0)) & 3], __uint_as_float(r[x][k]));
+                        for (int x = 0; x < TK / 32; ++x) {
+                            float &a = mx[2 * (x & 1)], &b = mx[2 * (x & 1) + 1];
+                            a = ct_max3(a, __uint_as_float(r[x][k]), __uint_as_float(r[x][k + 1]));
+                            b = ct_max3(b, __uint_as_float(r[x][k + 2]), __uint_as_float(r[x][k + 3]));
+                        }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
                     if (i == first) {
                         m_ref = top;
@@ -463,7 +490,8 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;   // a row that has seen nothing: every score is -inf
                 if (g >= (uint32_t)ct.np) CT_FAIL_AT(5, !pv_done(g - ct.np));   // the MMAs have read what was in this P buffer
                 const uint32_t pw = prow + (ct.np == 2 ? (g & 1) * NH * slab : 0u);
-                float sum0 = 0.0f, sum1 = 0.0f;
+                const uint64_t sl2_2 = ct_pair(sl2, sl2), neg_2 = ct_pair(neg, neg);
+                uint64_t sum = 0;   // a pair of sums
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
                     if (act) {
@@ -473,8 +501,11 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 const int e = 8 * (c & 3) + 2 * k;
-                                const float e0 = fast_exp2(fmaf(__uint_as_float(r[2 * h + (c >> 2)][e]), sl2, neg)), e1 = fast_exp2(fmaf(__uint_as_float(r[2 * h + (c >> 2)][e + 1]), sl2, neg));
-                                sum0 += e0; sum1 += e1;
+                                const uint32_t (&rr)[32] = r[2 * h + (c >> 2)];
+                                float e0, e1;
+                                ct_unpair(ct_fma2(ct_pair(__uint_as_float(rr[e]), __uint_as_float(rr[e + 1])), sl2_2, neg_2), e0, e1);
+                                e0 = fast_exp2(e0); e1 = fast_exp2(e1);
+                                sum = ct_add2(sum, ct_pair(e0, e1));
                                 pk[k] = pack_16x2(e0, e1, F16);
                             }
                             if (row < ct.rows8) ct_st_shared_v4(pw + h * slab + ((((uint32_t)c) ^ sw) << 4), pk[0], pk[1], pk[2], pk[3]);
@@ -484,6 +515,8 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_full[t][g & 1][h]);
                 }
+                float sum0, sum1;
+                ct_unpair(sum, sum0, sum1);
                 l += sum0 + sum1;
             }
             if (failed) break;
