@@ -5,6 +5,7 @@
 
 #include "host.h"
 #include "cache_narrow.cuh"
+#include "cache_weights.cuh"
 
 namespace b200attn {
 namespace {
@@ -55,6 +56,14 @@ CaView strides(const b200attn_view &v, long long unit = 1) { return CaView{v.str
 bool aligned16(const b200attn_view &v, int dtype) {
     const long long e = (long long)esize(dtype);
     return (((uintptr_t)v.ptr | (uintptr_t)(v.stride_b * e) | (uintptr_t)(v.stride_h * e) | (uintptr_t)(v.stride_l * e)) & 15) == 0;
+}
+
+// What tensor maps and 16-byte accesses take: rows on 16 bytes, strides that are not 0 (a dimension of size 1 has none to speak of).
+bool strides_fit(b200attn_view v, int dtype, int B, int H, int L) {
+    if (B == 1) v.stride_b = 8;
+    if (H == 1) v.stride_h = 8;
+    if (L == 1) v.stride_l = 8;
+    return aligned16(v, dtype) && v.stride_b > 0 && v.stride_h > 0 && v.stride_l > 0;
 }
 
 // Lets a kernel have all the shared memory there is, once per device (asking each time costs a short call half a microsecond).
@@ -188,13 +197,7 @@ bool narrow_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, 
     return true;
 }
 bool tc_aligned(const b200attn_attend_args *a) {
-    auto fine = [&](const b200attn_view &v, long long h, long long l) {   // a dimension of size 1 has no stride to speak of; the others are not 0
-        b200attn_view x = v;
-        if (a->batch_sz == 1) x.stride_b = 8;
-        if (h == 1) x.stride_h = 8;
-        if (l == 1) x.stride_l = 8;
-        return aligned16(x, a->dtype) && x.stride_b > 0 && x.stride_h > 0 && x.stride_l > 0;
-    };
+    auto fine = [&](const b200attn_view &v, int h, int l) { return strides_fit(v, a->dtype, a->batch_sz, h, l); };
     return fine(a->Q, a->num_heads, a->len_new) && fine(a->K, a->num_kv_heads, a->capacity) && fine(a->V, a->num_kv_heads, a->capacity) && fine(a->out, a->num_heads, a->len_new) &&
            (a->Kd.ptr == nullptr || (fine(a->Kd, a->num_kv_heads, a->len_new) && fine(a->Vd, a->num_kv_heads, a->len_new)));
 }
@@ -343,6 +346,34 @@ int launch_weights(const CwParams &p, const HostCall &c, cudaStream_t st) {
     return B200ATTN_OK;
 }
 
+// The tensor-core kernel where it takes the call: -1 where it does not.
+template <bool F16>
+int launch_weights_tc(const CxParams &cx, const HostCall &c, const CUtensorMap &m, size_t smem, cudaStream_t st) {
+    int rc = raise_smem<cw_tc_kernel<F16>>(c);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(cw_tc_kernel<F16>, dim3((unsigned)cx.grid), CX_THREADS, smem, 1, st, m, cx));
+    count_launches(1);
+    return B200ATTN_OK;
+}
+int weights_tc(const b200attn_weights_args *a, const CwParams &p, const HostCall &c, cudaStream_t st) {
+    if (a->dtype == B200ATTN_F32 || p.D % 8 != 0 || (a->flags & B200ATTN_FLAG_FORCE_GENERIC)) return -1;
+    if (!strides_fit(a->Q, a->dtype, a->batch_sz, a->num_heads, a->len_new) || !strides_fit(a->K, a->dtype, a->batch_sz, a->num_kv_heads, a->capacity)) return -1;
+    CxParams cx{};
+    cx.a = p;
+    cx.ng = (p.D + 63) / 64;
+    cx.grid = c.sm_count;
+    const size_t room = c.max_smem - 2048 - 1024, stage = (size_t)cx.ng * CX_TK * 128, row = (size_t)cx.ng * 128 + 8;
+    const long long rows = ((long long)p.A * p.G + 63) / 64 * 64;
+    const long long most = (long long)((room - 2 * stage) / row) / 64 * 64;   // beside two stages, the least that overlaps loads and products
+    cx.chunk = (int)(rows < most ? rows : most);
+    cx.nst = (int)((room - cx.chunk * row) / stage);
+    if (cx.nst > CT_MAX_STAGES) cx.nst = CT_MAX_STAGES;
+    CUtensorMap m;
+    if (!ct_map_rows(&m, p.K, p.k, p.B, p.Hkv, p.S, p.D, CX_TK)) return -1;
+    const size_t smem = cx.chunk * row + (size_t)cx.nst * stage + 1024;
+    return a->dtype == B200ATTN_F16 ? launch_weights_tc<true>(cx, c, m, smem, st) : launch_weights_tc<false>(cx, c, m, smem, st);
+}
+
 int weights(const b200attn_weights_args *a) {
     if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
     if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
@@ -368,6 +399,12 @@ int weights(const b200attn_weights_args *a) {
     p.A = A; p.B = a->batch_sz; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.G = G; p.T = a->len_new; p.S = a->capacity; p.D = a->head_d;
     p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_d) : a->scale) * 1.4426950408889634f;
     p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    rc = weights_tc(a, p, c, st);
+    if (rc == B200ATTN_OK) {
+        set_last_path("cache_tc");
+        return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
+    }
+    if (rc != -1) return rc;
     rc = a->dtype == B200ATTN_F32 ? launch_weights<float>(p, c, st) : a->dtype == B200ATTN_F16 ? launch_weights<__half>(p, c, st) : launch_weights<__nv_bfloat16>(p, c, st);
     if (rc) return rc;
     set_last_path("cache_generic");

@@ -37,12 +37,6 @@ struct CnBars {
 
 __host__ __device__ inline size_t cn_front_bytes(int N, int ng) { return (size_t)2 * N * 128 * (ng + 2); }   // two Q buffers, two P buffers
 
-__device__ __forceinline__ bool cn_any(bool x) {   // over the 128 softmax threads
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"((uint32_t)x) : "memory");
-    return any != 0;
-}
-__device__ __forceinline__ void cn_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ float cn_warp_max(float x) {
     float m;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
@@ -258,7 +252,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         auto pv_done = [&](uint32_t x) { return mbar_wait(&bars.o_done[x & 1], (x >> 1) & 1u, lim); };
         for (int seg = 0;; ++seg) {
             CN_FAIL_AT(7, !mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim));
-            if (cn_any(failed)) break;
+            if (ct_any(failed)) break;
             const CtSeg &w = s_seg[seg & (CT_SLOTS - 1)];
             if (w.whole < 0) break;
             const int first = w.tile, end = w.end, nct = w.ct;
@@ -311,8 +305,8 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (r + 3 >= R) d = -INFINITY;
                     top = fmaxf(fmaxf(top, fmaxf(a, b)), fmaxf(c, d));
                 }
-                if (cn_any(top > CT_RESCALE_LOG2 || failed)) {
-                    if (cn_any(failed)) { stop = true; break; }
+                if (ct_any(top > CT_RESCALE_LOG2 || failed)) {
+                    if (ct_any(failed)) { stop = true; break; }
                     // ---- new references where a row's maximum is beyond its own; what has been added up so far is rescaled ----
 #pragma unroll
                     for (int r = 0; r < N; ++r) {
@@ -320,7 +314,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const float m = cn_warp_max(x[r]);
                         if (lane == 0) s_red[q][r] = m;
                     }
-                    cn_sync();
+                    ct_sync();
                     if (tid < R) {
                         const float m = fmaxf(fmaxf(s_red[0][tid], s_red[1][tid]), fmaxf(s_red[2][tid], s_red[3][tid])) * sl2, old = s_neg[tid];
                         float f = 1.0f;
@@ -330,7 +324,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         }
                         s_f[tid] = f;
                     }
-                    cn_sync();
+                    ct_sync();
 #pragma unroll
                     for (int r = 0; r < N; ++r)
                         if (r < R) l[r] *= s_f[r];
@@ -370,7 +364,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.p_full[g & 1]);
             }
-            if (stop || cn_any(failed)) break;
+            if (stop || ct_any(failed)) break;
             // ---- the unit's sums, then its outputs ----
 #pragma unroll
             for (int r = 0; r < N; ++r) {
@@ -378,7 +372,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const float x = warp_sum(l[r]);
                 if (lane == 0) s_red[q][r] = x;
             }
-            cn_sync();
+            ct_sync();
             const bool whole = w.whole != 0, bad = s_bad[seg & (CT_SLOTS - 1)] == seg + 1;
             float *prt = p.part + ((size_t)blockIdx.x * 2 + (seg == 0 ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
             const int b = w.b, h = w.h;
@@ -395,7 +389,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             CN_FAIL_AT(6, !pv_done(g - 1));
             tc_fence_after();
-            cn_sync();
+            ct_sync();
             for (int c = 0; c < nh; ++c) {
                 // lane -> column: with 64 rows in the MMA, row d of the accumulator is in lane 32 (d / 16) + d % 16
                 const int d = p.D <= 64 ? (lane < 16 ? 16 * q + lane : p.D) : 128 * c + tid;

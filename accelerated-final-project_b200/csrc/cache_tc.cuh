@@ -60,6 +60,13 @@ __device__ __forceinline__ void tma_load_5d(void *smem_dst, const CUtensorMap *t
         : "memory");
 }
 
+__device__ __forceinline__ bool ct_any(bool x) {   // over the 128 threads of warps 4-7 (barrier 1)
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"((uint32_t)x) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void ct_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
 __device__ __forceinline__ void ct_st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
