@@ -348,10 +348,10 @@ int launch_weights(const CwParams &p, const HostCall &c, cudaStream_t st) {
 
 // The tensor-core kernel where it takes the call: -1 where it does not.
 template <bool F16>
-int launch_weights_tc(const CxParams &cx, const HostCall &c, const CUtensorMap &m, size_t smem, cudaStream_t st) {
+int launch_weights_tc(const CxParams &cx, const HostCall &c, const CUtensorMap (&m)[2], size_t smem, cudaStream_t st) {
     int rc = raise_smem<cw_tc_kernel<F16>>(c);
     if (rc) return rc;
-    CU_TRY(launch_dependent(cw_tc_kernel<F16>, dim3((unsigned)cx.grid), CX_THREADS, smem, 1, st, m, cx));
+    CU_TRY(launch_dependent(cw_tc_kernel<F16>, dim3((unsigned)cx.grid), CX_THREADS, smem, 1, st, m[0], m[1], cx));
     count_launches(1);
     return B200ATTN_OK;
 }
@@ -362,15 +362,30 @@ int weights_tc(const b200attn_weights_args *a, const CwParams &p, const HostCall
     cx.a = p;
     cx.ng = (p.D + 63) / 64;
     cx.grid = c.sm_count;
-    const size_t room = c.max_smem - 2048 - 1024, stage = (size_t)cx.ng * CX_TK * 128, row = (size_t)cx.ng * 128 + 8;
-    const long long rows = ((long long)p.A * p.G + 63) / 64 * 64;
-    const long long most = (long long)((room - 2 * stage) / row) / 64 * 64;   // beside two stages, the least that overlaps loads and products
-    cx.chunk = (int)(rows < most ? rows : most);
-    cx.nst = (int)((room - cx.chunk * row) / stage);
+    const long long room = (long long)c.max_smem - 2048 - 1024, stage = (long long)cx.ng * CX_TK * 128, row = cx.ng * 128 + 8, all = (long long)p.A * p.G;
+    // all tokens accepted: boxes of whole groups of 8 rows, up to 64 rows or one such group of them
+    int unit = CX_NB;   // a chunk is a multiple of this
+    if (!p.accepted && p.G <= 32) {
+        int t = 8;
+        while (t > 1 && p.G * (t / 2) % 8 == 0) t /= 2;
+        cx.box_t = p.G * t < CX_NB ? CX_NB / (p.G * t) * t : t;
+        unit = p.G * cx.box_t;
+    }
+    for (cx.nq = 2; cx.nq > 0; --cx.nq) {   // two buffers for Q where that leaves four stages; else what two stages, the least that overlaps loads and products, leave
+        const long long most = (room - (cx.nq == 2 ? 4 : 2) * stage) / (cx.nq * row) / CX_NB * CX_NB;   // rows of a buffer
+        const long long fits = most < unit ? 0 : most / unit * unit, rows = (all + unit - 1) / unit * unit;
+        if (cx.nq == 2 && rows > fits) continue;
+        if (fits == 0) return -1;
+        cx.chunk = (int)(rows < fits ? rows : fits);
+        break;
+    }
+    const long long pitch = (cx.chunk + CX_NB - 1) / CX_NB * CX_NB;
+    cx.nst = (int)((room - cx.nq * pitch * row) / stage);
     if (cx.nst > CT_MAX_STAGES) cx.nst = CT_MAX_STAGES;
-    CUtensorMap m;
-    if (!ct_map_rows(&m, p.K, p.k, p.B, p.Hkv, p.S, p.D, CX_TK)) return -1;
-    const size_t smem = cx.chunk * row + (size_t)cx.nst * stage + 1024;
+    CUtensorMap m[2];
+    memset(m, 0, sizeof m);
+    if (!ct_map_rows(&m[1], p.K, p.k, p.B, p.Hkv, p.S, p.D, CX_TK) || (cx.box_t && !ct_map_q(&m[0], p.Q, p.q, p.B, p.Hkv, p.G, p.T, p.D, cx.box_t))) return -1;
+    const size_t smem = (size_t)(cx.nq * pitch * row + cx.nst * stage + 1024);
     return a->dtype == B200ATTN_F16 ? launch_weights_tc<true>(cx, c, m, smem, st) : launch_weights_tc<false>(cx, c, m, smem, st);
 }
 

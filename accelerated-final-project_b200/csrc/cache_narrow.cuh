@@ -277,7 +277,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             tmem_ld_wait();
                         }
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) x[c + r] = there && c < R ? __uint_as_float(raw[r]) : -INFINITY;
+                        for (int r = 0; r < 16; ++r) x[c + r] = there && c + r < R ? __uint_as_float(raw[r]) : -INFINITY;
                     }
                 }
                 tc_fence_before();
@@ -296,14 +296,14 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 float top = -INFINITY;   // the largest score over its row's reference
 #pragma unroll
-                for (int r = 0; r < N; r += 4) {
-                    if (r >= R) break;
-                    const float4 n4 = *reinterpret_cast<const float4 *>(s_neg + r);
-                    float a = fmaf(x[r], sl2, n4.x), b = fmaf(x[r + 1], sl2, n4.y), c = fmaf(x[r + 2], sl2, n4.z), d = fmaf(x[r + 3], sl2, n4.w);
-                    if (r + 1 >= R) b = -INFINITY;
-                    if (r + 2 >= R) c = -INFINITY;
-                    if (r + 3 >= R) d = -INFINITY;
-                    top = fmaxf(fmaxf(top, fmaxf(a, b)), fmaxf(c, d));
+                for (int r0 = 0; r0 < N; r0 += 16) {   // (16 rows without a branch)
+                    if (r0 >= R) break;
+#pragma unroll
+                    for (int r = r0; r < r0 + 16; r += 4) {
+                        const float4 n4 = *reinterpret_cast<const float4 *>(s_neg + r);
+                        top = ct_max3(top, fmaf(x[r], sl2, n4.x), fmaf(x[r + 1], sl2, n4.y));
+                        top = ct_max3(top, fmaf(x[r + 2], sl2, n4.z), fmaf(x[r + 3], sl2, n4.w));
+                    }
                 }
                 if (ct_any(top > CT_RESCALE_LOG2 || failed)) {
                     if (ct_any(failed)) { stop = true; break; }
@@ -348,15 +348,17 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (g >= 2) CN_FAIL_AT(5, !pv_done(g - 2));   // the MMAs have read what was in this P buffer
                 const uint32_t pb = pw + (g & 1) * 2 * slab;
 #pragma unroll
-                for (int r = 0; r < N; r += 4) {
-                    if (r >= R) break;
-                    const float4 n4 = *reinterpret_cast<const float4 *>(s_neg + r);
-                    const float nn[4] = {n4.x, n4.y, n4.z, n4.w};
+                for (int r0 = 0; r0 < N; r0 += 8) {   // (8 rows without a branch)
+                    if (r0 >= R) break;
+                    const float4 na = *reinterpret_cast<const float4 *>(s_neg + r0), nb = *reinterpret_cast<const float4 *>(s_neg + r0 + 4);
+                    const float nn[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
+                    float e[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float e = fast_exp2(fmaf(x[r + k], sl2, nn[k]));
-                        l[r + k] += e;
-                        ct_st_shared_u16(pb + (r + k) * 128 + ((chunk ^ ((r + k) & 7)) << 4), pack_16(e, F16));
+                    for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(x[r0 + k], sl2, nn[k]));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        l[r0 + k] += e[k];
+                        ct_st_shared_u16(pb + (r0 + k) * 128 + ((chunk ^ k) << 4), pack_16(e[k], F16));
                     }
                 }
                 fence_proxy_async_smem();

@@ -3,32 +3,41 @@
 // lse is known, so there is no softmax to run: keys are the lanes of tensor memory, S^T [128 keys x rows] = K Q^T, and the thread of a key adds its
 // rows up in registers, in the order of the rows, and to the array once: no atomics, no exchange between threads.
 // The tiles of 128 keys of all (sequence, key head) pairs with accepted tokens are shared out evenly and contiguously over the CTAs (as in cache.cuh; a
-// tile needs no joining).  Per pair the accepted rows of Q are gathered once into shared memory (the list names tokens anywhere); more rows than fit
-// are taken in chunks, each over the CTA's tiles of the pair again.
-//   warp 0       the walk over the tiles; one thread requests K tiles by TMA
-//   warp 1       one thread issues the MMAs, 64 rows at a time into four buffers
-//   warps 4-7    gather Q, then a thread per key
+// tile needs no joining).  Per pair the accepted rows of Q are brought into shared memory once: by TMA where all new tokens are accepted, else gathered
+// (the list names tokens anywhere).  More rows than fit are taken in chunks, each over the CTA's tiles of the pair again.  Blocks of rows that see nothing
+// of a tile are left out.
+//   warp 0       the walk over the tiles; one thread requests K tiles (and Q) by TMA
+//   warp 1       one thread issues the MMAs, 64 rows at a time, into two buffers per summing warpgroup
+//   warps 2, 3   gather the next rows of Q beside the present ones (by the summing warps between two pairs: 61 against XX us, weights_step)
+//   warps 4-11   two warpgroups take the tiles in turn; a thread per key: its exponentials and their sum (bound by the latency of that chain: one
+//                warpgroup 54 us, weights_step)
 #pragma once
 
 #include "cache_tc.cuh"
 
 namespace b200attn {
 
-constexpr int CX_THREADS = 256, CX_TK = 128, CX_NB = 64;
+constexpr int CX_THREADS = 384, CX_TK = 128, CX_NB = 64;   // (64 rows a block)
 constexpr int CX_BUFS = 4;
 constexpr int CX_SLOTS = 16;   // pairs that the roles can be at: one per ring stage (up to 8) and score buffer, and two
 
 struct CxParams {
     CwParams a;
     int ng, nst;       // groups of 64 columns, ring stages
-    int chunk;         // rows of Q that shared memory holds: a multiple of 64
+    int chunk, nq;     // rows of Q that a buffer holds: a multiple of 64; buffers
+    int box_t;         // tokens of a Q box, a chunk is whole boxes of whole groups of 8 rows; 0: rows are gathered
     int grid;
+    // first row of a chunk [r0, ..) that sees something of tile t, down to whole blocks
+    __device__ __forceinline__ int first_row(int t, int seen_by_all, int r0) const {
+        const long long r = (long long)(t * CX_TK - seen_by_all) * a.G - r0;
+        return r <= 0 ? 0 : (int)(r / CX_NB * CX_NB);
+    }
 };
 struct CxSeg { int b, h, n, tile, end, count; };   // count -1: no more
 struct CxBars {
     uint64_t k_full[CT_MAX_STAGES], k_empty[CT_MAX_STAGES];
     uint64_t seg[CX_SLOTS];
-    uint64_t q_ready;
+    uint64_t q_full[2], q_empty[2];
     uint64_t s_full[CX_BUFS], s_read[CX_BUFS];
 };
 
@@ -40,7 +49,7 @@ __device__ __forceinline__ int cx_len(const CwParams &p, int b) {
 
 template <bool F16>
 __global__ void __launch_bounds__(CX_THREADS, 1)
-cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CxParams cx) {
+cw_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CxParams cx) {
     using T = typename CtType<F16>::T;
     extern __shared__ unsigned char ct_smem_raw[];
     __shared__ CxBars bars;
@@ -51,20 +60,23 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
     unsigned char *smem = ct_smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ng = cx.ng, nst = cx.nst, chunk = cx.chunk;
-    const uint32_t stage = (uint32_t)ng * CX_TK * 128u, slab = (uint32_t)chunk * 128u;
-    unsigned char *q_smem = smem;                                        // [ng][chunk rows][128 B]
-    unsigned char *ring = q_smem + (size_t)ng * slab;                    // [nst][ng][128 keys][128 B]
-    float *s_nl = reinterpret_cast<float *>(ring + (size_t)nst * stage); // [chunk]: minus lse, log2 units
-    int *s_i = reinterpret_cast<int *>(s_nl + chunk);                    // [chunk]: which accepted token
+    const int pitch = (chunk + CX_NB - 1) / CX_NB * CX_NB;                // rows of a Q buffer: whole blocks
+    const uint32_t stage = (uint32_t)ng * CX_TK * 128u, slab = (uint32_t)pitch * 128u;
+    unsigned char *q_smem = smem;                                        // [nq][ng][pitch rows][128 B]
+    unsigned char *ring = q_smem + (size_t)cx.nq * ng * slab;            // [nst][ng][128 keys][128 B]
+    float *s_nl = reinterpret_cast<float *>(ring + (size_t)nst * stage); // [nq][pitch]: minus lse, log2 units
+    int *s_i = reinterpret_cast<int *>(s_nl + cx.nq * pitch);            // [nq][pitch]: which accepted token; -1: one that saw nothing
+    __shared__ int s_skip[2];                                            // some row of the buffer saw nothing
     const uint32_t lim = p.spin_limit;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.k_full[i], 1); mbar_init(&bars.k_empty[i], 1); }
         for (int i = 0; i < CX_SLOTS; ++i) mbar_init(&bars.seg[i], 1);
-        mbar_init(&bars.q_ready, 4);
+        for (int i = 0; i < 2; ++i) { mbar_init(&bars.q_full[i], cx.box_t ? 3 : 2); mbar_init(&bars.q_empty[i], 8); s_skip[i] = 0; }
         for (int i = 0; i < CX_BUFS; ++i) { mbar_init(&bars.s_full[i], 1); mbar_init(&bars.s_read[i], 4); }
         mbar_fence_init();
         tma_prefetch_desc(&tmK);
+        if (cx.box_t) tma_prefetch_desc(&tmQ);
     }
     if (warp == 1) tmem_alloc(&tmem_slot, CX_BUFS * CX_NB);
     tc_fence_before();
@@ -107,7 +119,7 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
             before += __shfl_sync(0xffffffffu, incl, 31);
         }
         int s = 0, seg = 0;
-        uint32_t ph = 0;
+        uint32_t ph = 0, qn = 0;
         bool ok = true;
         while (at < i1 && ok) {
             const int n = cx_len(p, b), ct = (n + CX_TK - 1) / CX_TK;
@@ -121,7 +133,17 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
             }
             __syncwarp();
             if (elect_one()) {
-                for (int c = 0; c < chunks && ok; ++c)
+                for (int c = 0; c < chunks && ok; ++c, ++qn) {
+                    if (cx.box_t) {
+                        const uint32_t qb = cx.nq == 2 ? qn & 1 : 0;
+                        ok = mbar_wait(&bars.q_empty[qb], ((cx.nq == 2 ? qn >> 1 : qn) & 1u) ^ 1u, lim);
+                        if (!ok) break;
+                        const int boxes = (min(chunk, count * p.G - c * chunk) + p.G * cx.box_t - 1) / (p.G * cx.box_t);
+                        mbar_expect_tx(&bars.q_full[qb], (uint32_t)(boxes * ng * p.G * cx.box_t) * 128u);
+                        for (int k = 0; k < boxes; ++k)
+                            for (int g = 0; g < ng; ++g)
+                                tma_load_5d(q_smem + (size_t)(qb * ng + g) * slab + (size_t)k * p.G * cx.box_t * 128, &tmQ, g * 64, 0, c * (chunk / p.G) + k * cx.box_t, h, b, &bars.q_full[qb]);
+                    }
                     for (int i = tile; i < end && ok; ++i) {
                         ok = mbar_wait(&bars.k_empty[s], ph ^ 1u, lim);
                         if (!ok) break;
@@ -129,6 +151,7 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
                         for (int g = 0; g < ng; ++g) tma_load_4d(ring + (size_t)s * stage + (size_t)g * (CX_TK * 128), &tmK, g * 64, i * CX_TK, h, b, &bars.k_full[s]);
                         if (++s == nst) { s = 0; ph ^= 1u; }
                     }
+                }
             }
             __syncwarp();
             ok = __all_sync(0xffffffffu, ok);
@@ -148,7 +171,8 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
         if (elect_one()) {
             const int ks = (p.D + 15) >> 4;
             int s = 0;
-            uint32_t ph = 0, blk = 0, qn = 0;   // ring, blocks of 64 rows so far, gathered chunks so far
+            uint32_t ph = 0, qn = 0, tn = 0;   // ring; chunks, tiles so far
+            uint32_t blocks[2] = {0, 0};       // blocks of 64 rows so far, per summing warpgroup
             bool ok = true;
             for (int seg = 0; ok; ++seg) {
                 ok = mbar_wait(&bars.seg[seg & (CX_SLOTS - 1)], (uint32_t)(seg / CX_SLOTS) & 1u, lim);
@@ -157,19 +181,21 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
                 if (w.count < 0) break;
                 for (int r0 = 0; r0 < w.count * p.G && ok; r0 += chunk, ++qn) {
                     const int rows = min(chunk, w.count * p.G - r0);
-                    ok = mbar_wait(&bars.q_ready, qn & 1u, lim);
-                    for (int i = w.tile; i < w.end && ok; ++i) {
+                    const uint32_t qb = cx.nq == 2 ? qn & 1 : 0;
+                    ok = mbar_wait(&bars.q_full[qb], (cx.nq == 2 ? qn >> 1 : qn) & 1u, lim);
+                    for (int i = w.tile; i < w.end && ok; ++i, ++tn) {
+                        uint32_t blk = tn & 1 ? blocks[1] : blocks[0];
                         ok = mbar_wait(&bars.k_full[s], ph, lim);
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t ka = smem_u32(ring + (size_t)s * stage);
-                        for (int n0 = 0; n0 < rows; n0 += CX_NB, ++blk) {
-                            const uint32_t u = blk & (CX_BUFS - 1);
-                            ok = mbar_wait(&bars.s_read[u], (uint32_t)(blk / CX_BUFS & 1) ^ 1u, lim);
+                        for (int n0 = cx.first_row(i, w.n - w.count, r0); n0 < rows; n0 += CX_NB, ++blk) {
+                            const uint32_t u = 2 * (tn & 1) + (blk & 1);
+                            ok = mbar_wait(&bars.s_read[u], (blk >> 1 & 1u) ^ 1u, lim);
                             if (!ok) break;
                             tc_fence_after();
                             const uint32_t id = umma_idesc_16(128, min(CX_NB, (rows - n0 + 15) & ~15), 0, 0, F16 ? 1 : 0);
-                            const uint32_t qa = smem_u32(q_smem) + (uint32_t)n0 * 128u;
+                            const uint32_t qa = smem_u32(q_smem) + qb * ng * slab + (uint32_t)n0 * 128u;
                             for (int g = 0; g < ng; ++g) {
                                 const uint64_t dk = umma_desc_k_sw128(ka + g * (CX_TK * 128)), dq = umma_desc_k_sw128(qa + g * slab);
 #pragma unroll
@@ -179,6 +205,7 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
                             umma_commit(&bars.s_full[u]);
                         }
                         if (!ok) break;
+                        if (tn & 1) blocks[1] = blk; else blocks[0] = blk;
                         umma_commit(&bars.k_empty[s]);
                         if (++s == nst) { s = 0; ph ^= 1u; }
                     }
@@ -186,81 +213,149 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ Cx
             }
             if (!ok) { report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 17)); failed = true; }
         }
-    } else if (warp >= 4) {
+    } else if (warp < 4) {
+        // ---- gather: rows of Q as the MMAs read them, 16-byte pieces, eight requests in flight per thread ----
+        const int tid = threadIdx.x - 64;
+        uint32_t qn = 0;
+        bool ok = true;
+        const int pieces = ng * 8;
+        for (int seg = 0; ok; ++seg) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.seg[seg & (CX_SLOTS - 1)], (uint32_t)(seg / CX_SLOTS) & 1u, lim));
+            if (!ok) break;
+            const CxSeg w = s_seg[seg & (CX_SLOTS - 1)];
+            if (w.count < 0) break;
+            const int *list = p.accepted ? p.accepted + (long long)w.b * p.A : nullptr;
+            for (int r0 = 0; r0 < w.count * p.G; r0 += chunk, ++qn) {
+                const uint32_t qb = cx.nq == 2 ? qn & 1 : 0;
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_empty[qb], ((cx.nq == 2 ? qn >> 1 : qn) & 1u) ^ 1u, lim));
+                if (!ok) break;
+                unsigned char *dst = q_smem + (size_t)qb * ng * slab;
+                const int rows = min(chunk, w.count * p.G - r0), todo = cx.box_t ? 0 : ((rows + 15) & ~15) * pieces;   // (rows of zeros up to whole MMA columns)
+                for (int x0 = tid; x0 < todo; x0 += 64 * 8) {
+                    uint4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int x = x0 + 64 * k, r = x / pieces, c = x - r * pieces, rr = r0 + r, i = rr / p.G;
+                        v[k] = make_uint4(0, 0, 0, 0);
+                        if (r < rows && c * 8 < p.D)
+                            v[k] = *reinterpret_cast<const uint4 *>(ca_row<T>(p.Q, p.q, w.b, w.h * p.G + rr - i * p.G, list ? __ldg(list + i) : i) + c * 8);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int x = x0 + 64 * k, r = x / pieces, c = x - r * pieces;
+                        if (x < todo) *reinterpret_cast<uint4 *>(dst + (size_t)(c >> 3) * slab + (size_t)r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+                    }
+                }
+                const int padded = (rows + 31) & ~31;   // rows that do not exist see nothing
+                for (int x0 = tid; x0 < padded; x0 += 64 * 8) {
+                    float x[8];
+                    int at[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int rr = r0 + x0 + 64 * k;
+                        at[k] = rr / p.G;
+                        x[k] = x0 + 64 * k < rows ? p.lse[((long long)w.b * p.Hq + w.h * p.G + rr - at[k] * p.G) * p.T + (list ? __ldg(list + at[k]) : at[k])] : 0.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = x0 + 64 * k;
+                        if (r < padded) {
+                            s_nl[qb * pitch + r] = -1.4426950408889634f * x[k];
+                            s_i[qb * pitch + r] = x[k] == -INFINITY || r >= rows ? -1 : at[k];
+                            if (x[k] == -INFINITY) s_skip[qb] = (int)qn + 1;
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.q_full[qb]);
+            }
+        }
+        if (!ok) { if (lane == 0) report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 19)); failed = true; }
+    } else {
         const int q = warp & 3, tid = threadIdx.x & 127;
         const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
         const float sl2 = p.scale_log2;
-        uint32_t blk = 0;
+        const uint64_t sl2_2 = ct_pair(sl2, sl2);
+        const uint32_t wg = (warp - 4) >> 2;
+        uint32_t blk = 0, qn = 0, tn = 0;   // this warpgroup's blocks so far; chunks, tiles so far
         bool ok = true;
-        // (a thread whose wait has run out goes on through the barriers of the four warps until they all leave together, so that none waits for it there)
-        for (int seg = 0;; ++seg) {
-            ok = ok && mbar_wait(&bars.seg[seg & (CX_SLOTS - 1)], (uint32_t)(seg / CX_SLOTS) & 1u, lim);
-            if (ct_any(!ok)) { ok = false; break; }
+        for (int seg = 0; ok; ++seg) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.seg[seg & (CX_SLOTS - 1)], (uint32_t)(seg / CX_SLOTS) & 1u, lim));
+            if (!ok) break;
             const CxSeg w = s_seg[seg & (CX_SLOTS - 1)];
             if (w.count < 0) break;
             float *wrow = p.weights + ((long long)w.b * p.Hkv + w.h) * p.S;
-            for (int r0 = 0; r0 < w.count * p.G; r0 += chunk) {
+            for (int r0 = 0; r0 < w.count * p.G && ok; r0 += chunk, ++qn) {
                 const int rows = min(chunk, w.count * p.G - r0);
-                // ---- gather: the MMAs that read the rows before these have completed (their scores have been taken by every thread) ----
-                if (ct_any(!ok)) { ok = false; break; }
-                const int padded = (rows + 15) & ~15, pieces = ng * 8;   // rows of zeros up to whole MMA columns; 16-byte pieces of a row
-                for (int x = tid; x < padded * pieces; x += 128) {
-                    const int r = x / pieces, c = x % pieces, rr = r0 + r, i = rr / p.G;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < rows && c * 8 < p.D) {
-                        const int t = p.accepted ? __ldg(p.accepted + (long long)w.b * p.A + i) : i;
-                        v = *reinterpret_cast<const uint4 *>(ca_row<T>(p.Q, p.q, w.b, w.h * p.G + rr % p.G, t) + c * 8);
-                    }
-                    *reinterpret_cast<uint4 *>(q_smem + (size_t)(c >> 3) * slab + (size_t)r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-                }
-                for (int r = tid; r < rows; r += 128) {
-                    const int rr = r0 + r, i = rr / p.G, t = p.accepted ? __ldg(p.accepted + (long long)w.b * p.A + i) : i;
-                    const float x = p.lse[((long long)w.b * p.Hq + w.h * p.G + rr % p.G) * p.T + t];
-                    s_nl[r] = -1.4426950408889634f * x;
-                    s_i[r] = x == -INFINITY ? -1 : i;   // a token that saw nothing gave no weight
-                }
-                fence_proxy_async_smem();
-                ct_sync();
-                if (lane == 0) mbar_arrive(&bars.q_ready);
-                for (int t = w.tile; t < w.end; ++t) {
-                    const int j = t * CX_TK + tid, first = j - (w.n - w.count);   // the first accepted token that sees this key (<= 0: all do)
-                    const bool there = j < w.n;
-                    // rows of tokens that saw nothing, and keys behind the first accepted token, are looked at one by one
-                    const float old = there ? wrow[j] : 0.0f;
-                    const bool all = (t + 1) * CX_TK <= w.n - w.count;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int n0 = 0; n0 < rows; n0 += CX_NB, ++blk) {
-                        const uint32_t u = blk & (CX_BUFS - 1);
-                        ok = ok && mbar_wait(&bars.s_full[u], (uint32_t)(blk / CX_BUFS) & 1u, lim);
-                        ok = __all_sync(0xffffffffu, ok);
+                const uint32_t qb = cx.nq == 2 ? qn & 1 : 0;
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_full[qb], (cx.nq == 2 ? qn >> 1 : qn) & 1u, lim));
+                if (!ok) break;
+                const float *nl = s_nl + qb * pitch;
+                const int *si = s_i + qb * pitch;
+                const bool skip = s_skip[qb] == (int)qn + 1;
+                const int mine = w.tile + ((tn ^ wg) & 1);   // this warpgroup's first tile
+                tn += w.end - w.tile;
+                float next = mine < w.end && mine * CX_TK + tid < w.n ? wrow[mine * CX_TK + tid] : 0.0f;   // (asked for a tile ahead)
+                for (int t = mine; t < w.end && ok; t += 2) {
+                    const int j = t * CX_TK + tid, first = max(j - (w.n - w.count), 0);   // the first accepted token that sees this key
+                    const int n_first = cx.first_row(t, w.n - w.count, r0);
+                    const bool there = j < w.n && n_first < rows;
+                    const float old = next;
+                    if (t + 2 < w.end) next = j + 2 * CX_TK < w.n ? wrow[j + 2 * CX_TK] : 0.0f;
+                    const bool plain = !skip && (t + 1) * CX_TK <= w.n - w.count;         // every row sees every key of the tile
+                    uint64_t sum[2] = {0, 0};
+                    for (int n0 = n_first; n0 < rows && ok; n0 += CX_NB, ++blk) {
+                        const uint32_t u = 2 * wg + (blk & 1);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[u], blk >> 1 & 1u, lim));
+                        if (!ok) break;
                         tc_fence_after();
+                        uint32_t raw[CX_NB / 32][32];
 #pragma unroll
-                        for (int c = 0; c < CX_NB; c += 16) {
-                            if (n0 + c >= rows) break;
-                            uint32_t raw[16];
-                            tmem_ld16(tl + u * CX_NB + c, raw);
-                            tmem_ld_wait();
-                            const float4 *nl = reinterpret_cast<const float4 *>(s_nl + n0 + c);
-                            const int4 *si = reinterpret_cast<const int4 *>(s_i + n0 + c);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float4 l4 = nl[k];
-                                const int4 i4 = si[k];
-                                const int left = rows - (n0 + c + 4 * k), f = all ? 0 : max(first, 0);
-                                const float e0 = fast_exp2(fmaf(__uint_as_float(raw[4 * k]), sl2, l4.x)), e1 = fast_exp2(fmaf(__uint_as_float(raw[4 * k + 1]), sl2, l4.y));
-                                const float e2 = fast_exp2(fmaf(__uint_as_float(raw[4 * k + 2]), sl2, l4.z)), e3 = fast_exp2(fmaf(__uint_as_float(raw[4 * k + 3]), sl2, l4.w));
-                                if (0 < left && i4.x >= f) sum[0] += e0;
-                                if (1 < left && i4.y >= f) sum[1] += e1;
-                                if (2 < left && i4.z >= f) sum[2] += e2;
-                                if (3 < left && i4.w >= f) sum[3] += e3;
-                            }
-                        }
+                        for (int x = 0; x < CX_NB / 32; ++x)
+                            if (n0 + 32 * x < rows) tmem_ld32(tl + u * CX_NB + 32 * x, raw[x]);
+                        tmem_ld_wait();
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bars.s_read[u]);
+#pragma unroll
+                        for (int x = 0; x < CX_NB / 32; ++x) {   // (32 rows without a branch: one every 8 rows cost 27 clocks a row)
+                            if (n0 + 32 * x >= rows) break;
+                            const float4 *n4 = reinterpret_cast<const float4 *>(nl + n0 + 32 * x);
+                            float e[32];
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) {
+                                const float4 v = n4[k / 4];
+                                ct_unpair(ct_fma2(ct_pair(__uint_as_float(raw[x][k]), __uint_as_float(raw[x][k + 1])), sl2_2, ct_pair(v.x, v.y)), e[k], e[k + 1]);
+                                ct_unpair(ct_fma2(ct_pair(__uint_as_float(raw[x][k + 2]), __uint_as_float(raw[x][k + 3])), sl2_2, ct_pair(v.z, v.w)), e[k + 2], e[k + 3]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) e[k] = fast_exp2(e[k]);
+                            if (!plain || n0 + 32 * x + 32 > rows) {   // (the same for every thread)
+                                const int4 *i4 = reinterpret_cast<const int4 *>(si + n0 + 32 * x);
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4) {
+                                    const int4 v = i4[k / 4];
+                                    e[k] = v.x < first ? 0.0f : e[k];
+                                    e[k + 1] = v.y < first ? 0.0f : e[k + 1];
+                                    e[k + 2] = v.z < first ? 0.0f : e[k + 2];
+                                    e[k + 3] = v.w < first ? 0.0f : e[k + 3];
+                                }
+                            }
+#pragma unroll
+                            for (int k = 0; k < 32; k += 8) {
+                                sum[0] = ct_add2(sum[0], ct_add2(ct_pair(e[k], e[k + 1]), ct_pair(e[k + 2], e[k + 3])));
+                                sum[1] = ct_add2(sum[1], ct_add2(ct_pair(e[k + 4], e[k + 5]), ct_pair(e[k + 6], e[k + 7])));
+                            }
+                        }
                     }
-                    if (there && ok) wrow[j] = old + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    float a, c;
+                    ct_unpair(ct_add2(sum[0], sum[1]), a, c);
+                    if (there && ok) wrow[j] = old + (a + c);
                 }
+                if (!ok) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.q_empty[qb]);
             }
         }
         if (!ok) { if (lane == 0) report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 18)); failed = true; }
