@@ -327,7 +327,8 @@ int commit(const b200attn_commit_args *a) {
     p.A = a->accepted ? a->max_accepted : a->len_new;
     p.B = a->batch_sz; p.Hkv = a->num_kv_heads; p.T = a->len_new; p.S = a->capacity; p.row_bytes = (int)(D * e);
     const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && aligned16(a->Kd, a->dtype) && aligned16(a->Vd, a->dtype) && p.row_bytes % 16 == 0;
-    const long long blocks = ((long long)p.A * p.Hkv + CC_THREADS / 32 - 1) / (CC_THREADS / 32);
+    p.groups = (p.A + CC_ROWS - 1) / CC_ROWS;
+    const long long blocks = ((long long)p.groups * p.Hkv + CC_THREADS / 32 - 1) / (CC_THREADS / 32);
     if (blocks > 0x7fffffffll) return fail(B200ATTN_ERR_TOO_LARGE, "%lld rows to commit in a sequence are too many", (long long)p.A * p.Hkv);
     const dim3 grid((unsigned)blocks, (unsigned)p.B);
     CU_TRY(wide ? launch_dependent(cc_commit_kernel<uint4>, grid, CC_THREADS, 0, 1, st, p)
@@ -362,6 +363,7 @@ int weights_tc(const b200attn_weights_args *a, const CwParams &p, const HostCall
     cx.a = p;
     cx.ng = (p.D + 63) / 64;
     cx.grid = c.sm_count;
+    cx.oh = cx_overhead((long long)p.A * p.G);
     const long long room = (long long)c.max_smem - 2048 - 1024, stage = (long long)cx.ng * CX_TK * 128, row = cx.ng * 128 + 8, all = (long long)p.A * p.G;
     // all tokens accepted: boxes of whole groups of 8 rows, up to 64 rows or one such group of them
     int unit = CX_NB;   // a chunk is a multiple of this
@@ -473,9 +475,14 @@ int evict(const b200attn_evict_args *a) {
     p.B = a->batch_sz; p.Hkv = a->num_kv_heads; p.S = a->capacity; p.S_out = a->capacity_out; p.row_bytes = (int)(D * e);
     const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && p.row_bytes % 16 == 0 &&
                       (!into || (aligned16(a->K_out, a->dtype) && aligned16(a->V_out, a->dtype)));
-    const size_t smem = ce_smem_bytes(p.S);
+    // CTAs that share a head's rows: a cluster of up to 8, as many as fill the SMs, of 1024 rows each at least; their keys stay in shared memory where they fit
+    int cl = 1;
+    while (cl < 8 && (cl * 8192 * 6 < p.S || (2ll * cl * p.B * p.Hkv <= c.sm_count && cl * 1024 < p.S))) cl *= 2;
+    p.chunk_most = ((p.S + cl - 1) / cl + 31) & ~31;
+    p.cached = ce_smem_bytes(p.chunk_most, true) <= (c.max_smem - 24 * 1024) / (p.chunk_most <= 8192 ? 2 : 1);
+    const size_t smem = ce_smem_bytes(p.chunk_most, p.cached);
     if ((rc = raise_smem<ce_select_kernel>(c))) return rc;
-    CU_TRY(launch_dependent(ce_select_kernel, dim3((unsigned)p.Hkv, (unsigned)p.B), CE_THREADS, smem, 1, st, p));
+    CU_TRY(launch_dependent(ce_select_kernel, dim3((unsigned)(p.Hkv * cl), (unsigned)p.B), CE_THREADS, smem, cl, st, p));
     const int rows = CC_THREADS;   // of `kept` per block
     const dim3 grid((unsigned)((p.keep + (long long)rows - 1) / rows), (unsigned)p.Hkv, (unsigned)p.B);
     CU_TRY(wide ? launch_dependent(ce_move_kernel<uint4>, grid, CC_THREADS, 0, 1, st, p)

@@ -485,11 +485,32 @@ cw_generic_kernel(const CwParams p) {
 }
 
 // ---- rows from one place to another ------------------------------------------------------------------------------------
-// A warp copies a row of `bytes` bytes in pieces of type P (16 bytes, or an element where rows are not that aligned).
-template <typename P>
-__device__ __forceinline__ void ca_copy_row(void *dst, const void *src, int bytes, int lane) {
-    const int n = bytes / (int)sizeof(P);
-    for (int i = lane; i < n; i += 32) reinterpret_cast<P *>(dst)[i] = reinterpret_cast<const P *>(src)[i];
+// A warp copies `n` pairs of rows (of K and of V) of `bytes` bytes in pieces of type P (16 bytes, or an element where rows are not that aligned):
+// lanes share a row out as far as it has pieces, and four passes' pieces are in flight at once.  `at(i, ks, kd, vs, vd)` says where row i is and goes.
+template <typename P, typename At>
+__device__ __forceinline__ void ca_copy_rows(int n, int bytes, int lane, At at) {
+    const int pieces = bytes / (int)sizeof(P);
+    int L = 32;                       // lanes of a row
+    while (L > 1 && L / 2 >= pieces) L >>= 1;
+    const int per = 32 / L, sub = lane / L;
+    for (int i0 = 0; i0 < n; i0 += 4 * per) {
+        const P *ks[4], *vs[4];
+        P *kd[4], *vd[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * per + sub;
+            if (i < n) at(i, ks[u], kd[u], vs[u], vd[u]);
+        }
+        for (int c = lane % L; c < pieces; c += L) {
+            P k[4], v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * per + sub < n) { k[u] = ks[u][c]; v[u] = vs[u][c]; }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * per + sub < n) { kd[u][c] = k[u]; vd[u][c] = v[u]; }
+        }
+    }
 }
 
 struct CcParams {
@@ -500,10 +521,12 @@ struct CcParams {
     int *len_out, *pos;
     float *weights;
     int A, B, Hkv, T, S, row_bytes;
+    int groups;            // of CC_ROWS entries of a list
 };
-constexpr int CC_THREADS = 256;
+constexpr int CC_THREADS = 256, CC_ROWS = 16;
 
-// A warp per (head, accepted token), sequences along y: bound by memory where a prompt enters, else by the launch.
+// A warp per (head, 16 accepted tokens), sequences along y: bound by memory where a prompt enters, else by the launch.
+//   4 x 8 heads, 2000 tokens, fp32, head_d 64 (66 MB): 22 us with a warp per row
 template <typename P>
 __global__ void __launch_bounds__(CC_THREADS)
 cc_commit_kernel(const CcParams p) {
@@ -516,16 +539,23 @@ cc_commit_kernel(const CcParams p) {
         const int count = ca_count(p.accepted, b, p.A, p.T, p.S - n);
         if (lane == 0) p.len_out[b] = n + count;
     }
-    if (wid >= (long long)p.A * p.Hkv) return;
-    const int h = (int)(wid / p.A), i = (int)(wid % p.A);
-    if (ca_count(p.accepted, b, p.A, p.T, min(i + 1, p.S - n)) <= i) return;
-    const int t = p.accepted ? __ldg(p.accepted + (long long)b * p.A + i) : i;
-    const long long row = n + i;
-    ca_copy_row<P>((char *)p.K + b * p.k.b + h * p.k.h + row * p.k.l, (const char *)p.Kd + b * p.kd.b + h * p.kd.h + t * p.kd.l, p.row_bytes, lane);
-    ca_copy_row<P>((char *)p.V + b * p.v.b + h * p.v.h + row * p.v.l, (const char *)p.Vd + b * p.vd.b + h * p.vd.h + t * p.vd.l, p.row_bytes, lane);
-    const long long at = ((long long)b * p.Hkv + h) * p.S + row;
-    if (lane == 0 && p.weights) p.weights[at] = 0.0f;
-    if (lane == 0 && p.pos) p.pos[at] = (p.next_pos ? __ldg(p.next_pos + b) : n) + i;
+    if (wid >= (long long)p.groups * p.Hkv) return;
+    const int h = (int)(wid / p.groups), first = (int)(wid % p.groups) * CC_ROWS;
+    const int rows = ca_count(p.accepted, b, p.A, p.T, min(first + CC_ROWS, p.S - n)) - first;
+    if (rows <= 0) return;
+    const int *list = p.accepted ? p.accepted + (long long)b * p.A : nullptr;
+    char *K = (char *)p.K + b * p.k.b + h * p.k.h + (long long)(n + first) * p.k.l, *V = (char *)p.V + b * p.v.b + h * p.v.h + (long long)(n + first) * p.v.l;
+    const char *Kd = (const char *)p.Kd + b * p.kd.b + h * p.kd.h, *Vd = (const char *)p.Vd + b * p.vd.b + h * p.vd.h;
+    ca_copy_rows<P>(rows, p.row_bytes, lane, [&](int i, const P *&ks, P *&kd, const P *&vs, P *&vd) {
+        const long long t = list ? __ldg(list + first + i) : first + i;
+        ks = (const P *)(Kd + t * p.kd.l); kd = (P *)(K + i * p.k.l);
+        vs = (const P *)(Vd + t * p.vd.l); vd = (P *)(V + i * p.v.l);
+    });
+    if (lane < rows) {
+        const long long at = ((long long)b * p.Hkv + h) * p.S + n + first + lane;
+        if (p.weights) p.weights[at] = 0.0f;
+        if (p.pos) p.pos[at] = (p.next_pos ? __ldg(p.next_pos + b) : n) + first + lane;
+    }
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------------
@@ -538,6 +568,7 @@ struct CeParams {
     int *len_out, *kept;
     int keep, sink, recent;
     int B, Hkv, S, S_out, row_bytes;
+    int chunk_most, cached;          // rows of a CTA at the most; their ranks are kept in shared memory
 };
 
 // Weights as whole numbers of the same order: NaN lowest, -0 and 0 equal; protected rows are above all of them.
@@ -548,11 +579,12 @@ __device__ __forceinline__ unsigned ce_rank(float w, bool held) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int CE_THREADS = 1024;
-constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS;
-inline size_t ce_smem_bytes(int S) { return (size_t)((S + 31) / 32) * 2 * sizeof(unsigned); }
+constexpr int CE_THREADS = 512;
+constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS, CE_PER = CE_BINS / CE_THREADS;
+// per word of 32 rows: the mask of rows that stay, that of equal rank, a number; then 16 bits a row (the list of kept rows that move), then the ranks
+inline size_t ce_smem_bytes(int chunk, bool cached) { return (size_t)(chunk / 32) * 12 + (size_t)chunk * 2 + (cached ? (size_t)chunk * 4 : 0); }
 
-// Exclusive scan of one value per thread of the block.
+// Exclusive scan of one value per thread of the block, and its total.
 __device__ __forceinline__ int ce_scan(int x, int *s_warp, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = x;
@@ -564,140 +596,225 @@ __device__ __forceinline__ int ce_scan(int x, int *s_warp, int *total) {
     __syncthreads();
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    if (warp == 0) {
-        int v = s_warp[lane];
+    int before = 0, all = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += y;
-        }
-        s_warp[lane] = v;
+    for (int w = 0; w < CE_THREADS / 32; ++w) {
+        const int v = s_warp[w];
+        if (w < warp) before += v;
+        all += v;
     }
-    __syncthreads();
-    if (total) *total = s_warp[31];
-    return (warp ? s_warp[warp - 1] : 0) + incl - x;
+    *total = all;
+    return before + incl - x;
+}
+__device__ __forceinline__ int ce_remote(const void *p, uint32_t rank) {   // a 32-bit word of the same variable in another CTA of the cluster
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_to_rank(smem_u32(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ce_remote_u16(const void *p, uint32_t rank) {
+    unsigned short v;
+    asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(map_to_rank(smem_u32(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void ce_cluster_sync(uint32_t cl) {
+    if (cl > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
 }
 
-// One block per (sequence, head) finds the rows that stay and writes `kept`:
-//   the m-th largest rank by its digits from the top (three passes of a histogram over the rows of the prefix found so far),
-//   then two bit masks over the rows in shared memory - above that rank, equal to it; of the equal rows the first that there is room for stay -
-//   then, in place, the i-th freed row below m takes the i-th kept row from m on, found by its number among the mask's bits.
+// A cluster per (sequence, head), each CTA a piece of its rows, finds the rows that stay and writes `kept`:
+//   the m-th largest rank by its digits from the top: three histograms over the rows that share the prefix found so far, added up over the cluster;
+//   bit masks over the rows - above that rank, equal to it; of the equal rows the first that there is room for stay;
+//   into another cache: the numbers of the rows that stay are their new places.  In place: the kept rows from m on are listed by their number, and the i-th
+//   freed row below m takes the i-th of them, from the list of the CTA that has it.
+// Bound by latency: three passes over shared memory and some ten barriers.
+//   32 sequences x 8 heads, up to 4102 rows: 22 us with 1024 threads that read weights and positions anew in each pass; 4 x 8 heads, up to 32768 rows: 91 us
 __global__ void __launch_bounds__(CE_THREADS)
 ce_select_kernel(const CeParams p) {
-    extern __shared__ unsigned ce_masks[];
-    __shared__ int hist[CE_BINS], s_warp[32], s_first[CE_THREADS];
-    __shared__ unsigned s_digit;
-    __shared__ int s_above;
+    extern __shared__ unsigned ce_smem[];
+    __shared__ int hist[CE_BINS], s_warp[CE_THREADS / 32], s_count[4];
+    __shared__ int s_digit, s_above;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
+    uint32_t cl;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cl));
+    const uint32_t rank = cluster_ctarank();
+    const int h = blockIdx.x / cl;
     grid_launch_dependents();
     grid_dependency_wait();
-    const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.y, h = blockIdx.x;
     const int n = ca_len(p.len, b, p.S), m = min(n, p.keep);
     const long long unit = (long long)b * p.Hkv + h;
     int *kept = p.kept + unit * p.keep;
-    if (h == 0 && tid == 0 && p.len_out) p.len_out[b] = m;
-    for (int i = m + tid; i < p.keep; i += CE_THREADS) kept[i] = -1;
-    if (n <= p.keep) {
-        for (int i = tid; i < m; i += CE_THREADS) kept[i] = i;
+    if (h == 0 && rank == 0 && tid == 0 && p.len_out) p.len_out[b] = m;
+    for (int i = m + rank * CE_THREADS + tid; i < p.keep; i += cl * CE_THREADS) kept[i] = -1;
+    if (n <= p.keep) {   // (the same for the whole cluster)
+        for (int i = rank * CE_THREADS + tid; i < m; i += cl * CE_THREADS) kept[i] = i;
         return;
     }
-    const float *w = p.weights + unit * p.S;
-    const int *pos = p.pos ? p.pos + unit * p.S : nullptr;
+    const int chunk = min((int)(((n + cl - 1) / cl + 31) & ~31), p.chunk_most);   // rows of a CTA: whole words
+    const int lo = min((int)rank * chunk, n), rows = min(chunk, n - lo), words = (rows + 31) / 32;
+    unsigned *stays = ce_smem, *equal = stays + p.chunk_most / 32;
+    int *number = (int *)(equal + p.chunk_most / 32);
+    unsigned short *list = (unsigned short *)(number + p.chunk_most / 32);
+    unsigned *ranks = (unsigned *)(list + p.chunk_most);
+    const float *w = p.weights + unit * p.S + lo;
+    const int *pos = p.pos ? p.pos + unit * p.S + lo : nullptr;
     const long long recent = (long long)(p.next_pos ? p.next_pos[b] : n) - p.recent;
-    auto rank = [&](int r) {
-        const int at = pos ? pos[r] : r;
+    auto rank_of = [&](int r) {   // of row lo + r
+        const int at = pos ? pos[r] : lo + r;
         return ce_rank(w[r], at < p.sink || at >= recent);
     };
+    if (p.cached) {
+        for (int r0 = 0; r0 < rows; r0 += 4 * CE_THREADS) {
+            unsigned x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = r0 + k * CE_THREADS + tid < rows ? rank_of(r0 + k * CE_THREADS + tid) : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (r0 + k * CE_THREADS + tid < rows) ranks[r0 + k * CE_THREADS + tid] = x[k];
+        }
+    }
+    auto rank_at = [&](int r) { return p.cached ? ranks[r] : rank_of(r); };   // (a thread asks for the rows that it has written itself)
     unsigned prefix = 0;
     int need = m;   // rows to take from those that share the prefix
     for (int shift = 32 - CE_BITS;; shift = shift > CE_BITS ? shift - CE_BITS : 0) {
         const int bits = shift == 0 ? 32 - 2 * CE_BITS : CE_BITS;
         for (int i = tid; i < CE_BINS; i += CE_THREADS) hist[i] = 0;
         __syncthreads();
-        for (int r0 = 0; r0 < n; r0 += CE_THREADS) {
+        for (int r0 = 0; r0 < rows; r0 += CE_THREADS) {
             const int r = r0 + tid;
-            const unsigned x = r < n ? rank(r) : 0u;
-            const bool in = r < n && (shift + bits == 32 || (x >> (shift + bits)) == (prefix >> (shift + bits)));
-            // equal digits are common (weights of 0): one addition per digit and warp
-            const unsigned d = in ? (x >> shift) & ((1u << bits) - 1) : 0xffffffffu;
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&hist[d], __popc(same));
+            const unsigned x = r < rows ? rank_at(r) : 0u;
+            const bool in = r < rows && (shift + bits == 32 || (x >> (shift + bits)) == (prefix >> (shift + bits)));
+            const unsigned d = (x >> shift) & ((1u << bits) - 1);
+            // equal digits are common (weights of 0): those equal to the first lane's are added at once
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (who) {
+                const int leader = __ffs(who) - 1;
+                const unsigned d0 = __shfl_sync(0xffffffffu, d, leader), same = __ballot_sync(0xffffffffu, in && d == d0);
+                if (lane == leader) atomicAdd(&hist[d0], __popc(same));
+                if (in && d != d0) atomicAdd(&hist[d], 1);
+            }
         }
-        __syncthreads();
-        // from the top digit down: the one in which the count reaches `need`; thread i has the digits 2 (1023 - i) + 1 and 2 (1023 - i)
-        const int hi = hist[2 * (CE_THREADS - 1 - tid) + 1], lo = hist[2 * (CE_THREADS - 1 - tid)];
-        const int before = ce_scan(hi + lo, s_warp, nullptr);
-        if (before < need && before + hi + lo >= need) {
-            const bool top = before + hi >= need;
-            s_digit = 2 * (CE_THREADS - 1 - tid) + (top ? 1 : 0);
-            s_above = before + (top ? 0 : hi);
+        ce_cluster_sync(cl);
+        // thread i has the digits CE_BINS - 1 - CE_PER i downwards
+        int c[CE_PER], sum = 0;
+#pragma unroll
+        for (int k = 0; k < CE_PER; ++k) {
+            const int at = CE_BINS - 1 - CE_PER * tid - k;
+            c[k] = hist[at];
+            for (uint32_t o = 1; o < cl; ++o) c[k] += ce_remote(&hist[at], (rank + o) % cl);
+            sum += c[k];
         }
-        __syncthreads();
-        prefix |= s_digit << shift;
+        int all;
+        int before = ce_scan(sum, s_warp, &all);
+        if (before < need && before + sum >= need) {
+#pragma unroll
+            for (int k = 0; k < CE_PER; ++k) {
+                if (before < need && before + c[k] >= need) { s_digit = CE_BINS - 1 - CE_PER * tid - k; s_above = before; }
+                before += c[k];
+            }
+        }
+        ce_cluster_sync(cl);   // (and the histograms have been read by the others)
+        prefix |= (unsigned)s_digit << shift;
         need -= s_above;
-        __syncthreads();
         if (shift == 0) break;
+        __syncthreads();
     }
-    const int words = (n + 31) / 32;
-    unsigned *stays = ce_masks, *equal = ce_masks + words;
-    for (int r0 = 0; r0 < words * 32; r0 += CE_THREADS) {
-        const int r = r0 + tid;
-        if (r >= words * 32) break;   // (whole warps)
-        const unsigned x = r < n ? rank(r) : 0u;
-        const unsigned gt = __ballot_sync(0xffffffffu, r < n && x > prefix), eq = __ballot_sync(0xffffffffu, r < n && x == prefix);
-        if (lane == 0) { stays[r >> 5] = gt; equal[r >> 5] = eq; }
+    int equals = 0;
+    for (int i = warp; i < words; i += CE_THREADS / 32) {
+        const int r = 32 * i + lane;
+        // (with the ranks in shared memory this reads what other threads wrote: they have met since)
+        const unsigned x = r < rows ? rank_at(r) : 0u;
+        const unsigned gt = __ballot_sync(0xffffffffu, r < rows && x > prefix), eq = __ballot_sync(0xffffffffu, r < rows && x == prefix);
+        if (lane == 0) { stays[i] = gt; equal[i] = eq; }
     }
     __syncthreads();
-    // each thread owns `per` words in a row
-    const int per = (words + CE_THREADS - 1) / CE_THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-    int c = 0;
-    for (int i = w0; i < w1; ++i) c += __popc(equal[i]);
-    int room = need - ce_scan(c, s_warp, nullptr);
+    const int per = (words + CE_THREADS - 1) / CE_THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);   // words of this thread, in a row
+    for (int i = w0; i < w1; ++i) equals += __popc(equal[i]);
+    int all;
+    int mine = ce_scan(equals, s_warp, &all);
+    // numbers over the CTAs in front of this one: `slot` of s_count in each, which the caller's total goes into
+    auto in_front = [&](int total, int slot, int *sum) {
+        if (tid == 0) s_count[slot] = total;
+        ce_cluster_sync(cl);
+        int before = 0, every = 0;
+        for (uint32_t o = 0; o < cl; ++o) {
+            const int v = cl > 1 ? ce_remote(&s_count[slot], o) : s_count[slot];
+            if (o < rank) before += v;
+            every += v;
+        }
+        if (sum) *sum = every;
+        return before;
+    };
+    int room = need - in_front(all, 0, nullptr) - mine;
     for (int i = w0; i < w1; ++i) {
         unsigned eq = equal[i];
-        while (eq && room > 0) {
-            stays[i] |= eq & -eq;
-            eq &= eq - 1;
-            --room;
+        if (__popc(eq) <= room) {
+            stays[i] |= eq;
+            room -= __popc(eq);
+        } else {
+            for (; room > 0; --room) {
+                stays[i] |= eq & -eq;
+                eq &= eq - 1;
+            }
         }
     }
     __syncthreads();
-    if (p.K_out) {   // in order
-        c = 0;
-        for (int i = w0; i < w1; ++i) c += __popc(stays[i]);
-        int at = ce_scan(c, s_warp, nullptr);
-        for (int i = w0; i < w1; ++i)
-            for (unsigned x = stays[i]; x; x &= x - 1) kept[at++] = 32 * i + __ffs(x) - 1;
-        return;
-    }
-    auto late = [&](int i) {   // rows from m on that stay, of word i
-        return 32 * i >= m ? stays[i] : 32 * i + 32 <= m ? 0u : stays[i] & ~((1u << (m - 32 * i)) - 1);
+    // rows of word i below m
+    auto front = [&](int i) {
+        const int left = m - (lo + 32 * i);
+        return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
     };
-    c = 0;
-    for (int i = w0; i < w1; ++i) c += __popc(late(i));
-    s_first[tid] = ce_scan(c, s_warp, nullptr);   // number of the first such row of this thread's words
-    c = 0;
-    for (int i = w0; i < w1; ++i) c += 32 * i >= m ? 0 : __popc(~stays[i] & (32 * i + 32 <= m ? 0xffffffffu : (1u << (m - 32 * i)) - 1));
-    int hole = ce_scan(c, s_warp, nullptr);
+    const bool into = p.K_out != nullptr;
+    // the rows that are numbered: all that stay, or those of them from m on
+    int count = 0;
+    for (int i = w0; i < w1; ++i) count += __popc(into ? stays[i] : stays[i] & ~front(i));
+    mine = ce_scan(count, s_warp, &all);
     for (int i = w0; i < w1; ++i) {
-        for (int k = 0; k < 32 && 32 * i + k < m; ++k) {
-            const int r = 32 * i + k;
-            int from = r;
-            if (!(stays[i] >> k & 1)) {
-                int lo = 0, hi = CE_THREADS;   // the last thread whose first number is <= hole has that row
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (s_first[mid] <= hole) lo = mid; else hi = mid;
-                }
-                int left = hole - s_first[lo], x = lo * per;
-                while (left >= __popc(late(x))) left -= __popc(late(x++));
-                unsigned bitsx = late(x);
-                while (left--) bitsx &= bitsx - 1;
-                from = 32 * x + __ffs(bitsx) - 1;
-                ++hole;
-            }
-            kept[r] = from;
+        number[i] = mine;
+        mine += __popc(into ? stays[i] : stays[i] & ~front(i));
+    }
+    const int base = in_front(all, 1, nullptr);   // (a barrier: the numbers are there)
+    __syncthreads();
+    for (int i = warp; i < words; i += CE_THREADS / 32) {
+        const unsigned bits = into ? stays[i] : stays[i] & ~front(i);
+        if (bits >> lane & 1u) {
+            const int at = number[i] + __popc(bits & ((1u << lane) - 1u));
+            if (into) kept[base + at] = lo + 32 * i + lane;
+            else list[at] = (unsigned short)(32 * i + lane);
         }
     }
+    if (into) {
+        ce_cluster_sync(cl);   // (nobody leaves while its counts are being read)
+        return;
+    }
+    __syncthreads();
+    // freed rows: numbered, too
+    count = 0;
+    for (int i = w0; i < w1; ++i) count += __popc(~stays[i] & front(i));
+    mine = ce_scan(count, s_warp, &all);
+    for (int i = w0; i < w1; ++i) {
+        number[i] = mine;
+        mine += __popc(~stays[i] & front(i));
+    }
+    const int holes = in_front(all, 2, nullptr);   // (a barrier: all lists are there)
+    __syncthreads();
+    for (int i = warp; i < words; i += CE_THREADS / 32) {
+        const unsigned f = front(i), free = ~stays[i] & f;
+        if (f == 0) break;
+        if (f >> lane & 1u) {
+            int from = lo + 32 * i + lane;
+            if (free >> lane & 1u) {
+                int at = holes + number[i] + __popc(free & ((1u << lane) - 1u));
+                uint32_t o = 0;
+                for (;; ++o) {   // the CTA that has the at-th row that moves
+                    const int v = cl > 1 ? ce_remote(&s_count[1], o) : s_count[1];
+                    if (at < v || o + 1 == cl) break;
+                    at -= v;
+                }
+                from = (int)o * chunk + (cl > 1 ? ce_remote_u16(&list[at], o) : list[at]);
+            }
+            kept[lo + 32 * i + lane] = from;
+        }
+    }
+    ce_cluster_sync(cl);   // (nobody leaves while its list is being read)
 }
 
 // Moves what `kept` says: a warp per row.  In place the sources are rows >= m and the targets rows < m, so that no move reads what another writes.
@@ -711,13 +828,22 @@ ce_move_kernel(const CeParams p) {
     const int i0 = (blockIdx.x * (CC_THREADS / 32) + (threadIdx.x >> 5)) * 32;
     const int mine = i0 + lane < p.keep ? p.kept[unit * p.keep + i0 + lane] : -1;
     const bool moves = mine >= 0 && (p.K_out || mine != i0 + lane);
-    for (unsigned todo = __ballot_sync(0xffffffffu, moves); todo; todo &= todo - 1) {
-        const int k = __ffs(todo) - 1;
-        const long long from = __shfl_sync(0xffffffffu, mine, k), to = i0 + k;
-        const CaView ko = p.K_out ? p.ko : p.k, vo = p.K_out ? p.vo : p.v;
-        ca_copy_row<P>((char *)(p.K_out ? p.K_out : p.K) + b * ko.b + h * ko.h + to * ko.l, (const char *)p.K + b * p.k.b + h * p.k.h + from * p.k.l, p.row_bytes, lane);
-        ca_copy_row<P>((char *)(p.K_out ? p.V_out : p.V) + b * vo.b + h * vo.h + to * vo.l, (const char *)p.V + b * p.v.b + h * p.v.h + from * p.v.l, p.row_bytes, lane);
-    }
+    // the rows that move, closed up: lane i has the i-th of them
+    const unsigned todo = __ballot_sync(0xffffffffu, moves);
+    if (todo == 0) return;
+    const int to = __fns(todo, 0, lane + 1), from = __shfl_sync(0xffffffffu, mine, to >= 0 && to < 32 ? to : 0);
+    const CaView ko = p.K_out ? p.ko : p.k, vo = p.K_out ? p.vo : p.v;
+    char *Ko = (char *)(p.K_out ? p.K_out : p.K) + b * ko.b + h * ko.h + i0 * ko.l, *Vo = (char *)(p.K_out ? p.V_out : p.V) + b * vo.b + h * vo.h + i0 * vo.l;
+    const char *K = (const char *)p.K + b * p.k.b + h * p.k.h, *V = (const char *)p.V + b * p.v.b + h * p.v.h;
+    __shared__ int s_from[CC_THREADS], s_to[CC_THREADS];
+    s_from[threadIdx.x] = from;
+    s_to[threadIdx.x] = to;
+    __syncwarp();
+    const int *wf = s_from + (threadIdx.x & ~31), *wt = s_to + (threadIdx.x & ~31);
+    ca_copy_rows<P>(__popc(todo), p.row_bytes, lane, [&](int i, const P *&ks, P *&kd, const P *&vs, P *&vd) {
+        ks = (const P *)(K + wf[i] * p.k.l); kd = (P *)(Ko + wt[i] * ko.l);
+        vs = (const P *)(V + wf[i] * p.v.l); vd = (P *)(Vo + wt[i] * vo.l);
+    });
     if (moves) {
         float *wo = p.K_out ? p.weights_out + unit * p.S_out : p.weights + unit * p.S;
         wo[i0 + lane] = p.weights[unit * p.S + mine];

@@ -19,6 +19,9 @@ namespace b200attn {
 
 constexpr int CX_THREADS = 384, CX_TK = 128, CX_NB = 64;   // (64 rows a block)
 constexpr int CX_BUFS = 4;
+// What a pair's beginning and end cost a CTA, in tiles, as in cache.cuh: two tiles of a block of rows (none: a CTA with 20 short sequences took 62 us
+// where the others took 40, weights_step; two also where a tile has eleven blocks: 34 us instead of 28, weights_prompt).
+__host__ __device__ inline int cx_overhead(long long rows) { return rows <= CX_NB ? 2 : rows <= 2 * CX_NB ? 1 : 0; }
 constexpr int CX_SLOTS = 16;   // pairs that the roles can be at: one per ring stage (up to 8) and score buffer, and two
 
 struct CxParams {
@@ -26,7 +29,7 @@ struct CxParams {
     int ng, nst;       // groups of 64 columns, ring stages
     int chunk, nq;     // rows of Q that a buffer holds: a multiple of 64; buffers
     int box_t;         // tokens of a Q box, a chunk is whole boxes of whole groups of 8 rows; 0: rows are gathered
-    int grid;
+    int grid, oh;      // CTAs; items in front of a pair's tiles
     // first row of a chunk [r0, ..) that sees something of tile t, down to whole blocks
     __device__ __forceinline__ int first_row(int t, int seen_by_all, int r0) const {
         const long long r = (long long)(t * CX_TK - seen_by_all) * a.G - r0;
@@ -90,7 +93,10 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     if (warp == 0) {
         // ---- the walk: this CTA's range [i0, i1) of the tiles of all pairs ----
         long long total = 0;
-        auto items = [&](int b) { return b < p.B ? (long long)p.Hkv * ((cx_len(p, b) + CX_TK - 1) / CX_TK) : 0ll; };
+        auto items = [&](int b) {
+            const int ct = b < p.B ? (cx_len(p, b) + CX_TK - 1) / CX_TK : 0;
+            return ct > 0 ? (long long)p.Hkv * (cx.oh + ct) : 0ll;
+        };
         for (int b0 = 0; b0 < p.B; b0 += 32) {
             long long x = items(b0 + lane);
 #pragma unroll
@@ -122,9 +128,12 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         uint32_t ph = 0, qn = 0;
         bool ok = true;
         while (at < i1 && ok) {
-            const int n = cx_len(p, b), ct = (n + CX_TK - 1) / CX_TK;
-            if ((long long)p.Hkv * ct <= at - before) { before += (long long)p.Hkv * ct; ++b; continue; }
-            const int h = (int)((at - before) / ct), tile = (int)((at - before) % ct), end = (int)min((long long)ct, tile + (i1 - at));
+            const int n = cx_len(p, b), ct = (n + CX_TK - 1) / CX_TK, per = ct > 0 ? cx.oh + ct : 0;
+            if ((long long)p.Hkv * per <= at - before) { before += (long long)p.Hkv * per; ++b; continue; }
+            const int h = (int)((at - before) / per), from = (int)((at - before) % per), to = (int)min((long long)per, from + (i1 - at));
+            const int tile = max(from - cx.oh, 0), end = to - cx.oh;
+            at += to - from;
+            if (end <= tile) continue;   // (a range that ends in front of a pair's tiles)
             const int count = ca_count(p.accepted, b, p.A, p.T, n);
             const int chunks = (count * p.G + chunk - 1) / chunk;
             if (lane == 0) {
@@ -155,7 +164,6 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
             }
             __syncwarp();
             ok = __all_sync(0xffffffffu, ok);
-            at += end - tile;
             ++seg;
         }
         if (ok) {
