@@ -428,6 +428,19 @@ int weights(const b200attn_weights_args *a) {
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 
+template <typename P>
+int launch_evict(const CeParams &p, const HostCall &c, int cl, cudaStream_t st) {
+    int rc = raise_smem<ce_select_kernel<P>>(c);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ce_select_kernel<P>, dim3((unsigned)(p.Hkv * cl), (unsigned)p.B), CE_THREADS, ce_smem_bytes(p.chunk_most, p.cached), cl, st, p));
+    count_launches(1);
+    if (!p.K_out && p.S - p.keep <= CE_FEW) return B200ATTN_OK;
+    const int most = p.keep < p.S ? p.keep : p.S;
+    CU_TRY(launch_dependent(ce_move_kernel<P>, dim3((unsigned)((most + CC_THREADS - 1) / CC_THREADS), (unsigned)p.Hkv, (unsigned)p.B), CC_THREADS, 0, 1, st, p));
+    count_launches(1);
+    return B200ATTN_OK;
+}
+
 int evict(const b200attn_evict_args *a) {
     if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "args is NULL");
     if (a->struct_size != sizeof *a) return fail(B200ATTN_ERR_INVALID_ARG, "args->struct_size is %zu, expected %zu", a->struct_size, sizeof *a);
@@ -475,19 +488,15 @@ int evict(const b200attn_evict_args *a) {
     p.B = a->batch_sz; p.Hkv = a->num_kv_heads; p.S = a->capacity; p.S_out = a->capacity_out; p.row_bytes = (int)(D * e);
     const bool wide = aligned16(a->K, a->dtype) && aligned16(a->V, a->dtype) && p.row_bytes % 16 == 0 &&
                       (!into || (aligned16(a->K_out, a->dtype) && aligned16(a->V_out, a->dtype)));
-    // CTAs that share a head's rows: a cluster of up to 8, as many as fill the SMs, of 1024 rows each at least; their keys stay in shared memory where they fit
+    // CTAs that share a head's rows: a cluster of up to 8, as many as fill the SMs, of 4096 rows each at least (its barriers cost what 4096 rows do); one
+    // CTA where a step's few rows leave.  The ranks stay in shared memory where they fit.
     int cl = 1;
-    while (cl < 8 && (cl * 8192 * 6 < p.S || (2ll * cl * p.B * p.Hkv <= c.sm_count && cl * 1024 < p.S))) cl *= 2;
+    const bool step = !into && p.S - p.keep <= CE_PICK && ce_smem_bytes((p.S + 31) & ~31, true) <= c.max_smem - 24 * 1024;
+    while (!step && cl < 8 && (cl * 49152 < p.S || (2ll * cl * p.B * p.Hkv <= c.sm_count && cl * 4096 < p.S))) cl *= 2;
     p.chunk_most = ((p.S + cl - 1) / cl + 31) & ~31;
     p.cached = ce_smem_bytes(p.chunk_most, true) <= (c.max_smem - 24 * 1024) / (p.chunk_most <= 8192 ? 2 : 1);
-    const size_t smem = ce_smem_bytes(p.chunk_most, p.cached);
-    if ((rc = raise_smem<ce_select_kernel>(c))) return rc;
-    CU_TRY(launch_dependent(ce_select_kernel, dim3((unsigned)(p.Hkv * cl), (unsigned)p.B), CE_THREADS, smem, cl, st, p));
-    const int rows = CC_THREADS;   // of `kept` per block
-    const dim3 grid((unsigned)((p.keep + (long long)rows - 1) / rows), (unsigned)p.Hkv, (unsigned)p.B);
-    CU_TRY(wide ? launch_dependent(ce_move_kernel<uint4>, grid, CC_THREADS, 0, 1, st, p)
-                : e == 4 ? launch_dependent(ce_move_kernel<uint32_t>, grid, CC_THREADS, 0, 1, st, p) : launch_dependent(ce_move_kernel<uint16_t>, grid, CC_THREADS, 0, 1, st, p));
-    count_launches(2);
+    rc = wide ? launch_evict<uint4>(p, c, cl, st) : e == 4 ? launch_evict<uint32_t>(p, c, cl, st) : launch_evict<uint16_t>(p, c, cl, st);
+    if (rc) return rc;
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 

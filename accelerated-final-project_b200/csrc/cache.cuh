@@ -581,8 +581,13 @@ __device__ __forceinline__ unsigned ce_rank(float w, bool held) {
 
 constexpr int CE_THREADS = 512;
 constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS, CE_PER = CE_BINS / CE_THREADS;
-// per word of 32 rows: the mask of rows that stay, that of equal rank, a number; then 16 bits a row (the list of kept rows that move), then the ranks
-inline size_t ce_smem_bytes(int chunk, bool cached) { return (size_t)(chunk / 32) * 12 + (size_t)chunk * 2 + (cached ? (size_t)chunk * 4 : 0); }
+constexpr int CE_COPIES = 4;   // of the first histogram: most weights share a few of its digits, and additions to one word wait for each other
+constexpr size_t CE_HISTS = (size_t)(CE_COPIES + 2) * CE_BINS * 4;
+// the histograms; per word of 32 rows: the mask of rows that stay, that of equal rank, a number; 16 bits a row (the list of kept rows that move); the ranks
+inline size_t ce_smem_bytes(int chunk, bool cached) { return CE_HISTS + (size_t)(chunk / 32) * 12 + (size_t)chunk * 2 + (cached ? (size_t)chunk * 4 : 0); }
+// In place, up to this many rows a head move with ce_select_kernel itself; ce_move_kernel is not launched where the capacity allows no more.
+constexpr int CE_FEW = 128;
+constexpr int CE_PICK = 32;   // up to so many rows that leave are picked one by one
 
 // Exclusive scan of one value per thread of the block, and its total.
 __device__ __forceinline__ int ce_scan(int x, int *s_warp, int *total) {
@@ -611,6 +616,11 @@ __device__ __forceinline__ int ce_remote(const void *p, uint32_t rank) {   // a 
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_to_rank(smem_u32(p), rank)) : "memory");
     return v;
 }
+__device__ __forceinline__ int4 ce_remote4(const void *p, uint32_t rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_to_rank(smem_u32(p), rank)));
+    return v;
+}
 __device__ __forceinline__ int ce_remote_u16(const void *p, uint32_t rank) {
     unsigned short v;
     asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(map_to_rank(smem_u32(p), rank)) : "memory");
@@ -620,17 +630,42 @@ __device__ __forceinline__ void ce_cluster_sync(uint32_t cl) {
     if (cl > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
 }
 
+// By one whole warp: `n` rows of a head move, pairs[2 i] to pairs[2 i + 1] (in shared memory).  In place the sources are rows >= m and the targets
+// rows < m, so that no move reads what another writes.
+template <typename P>
+__device__ __forceinline__ void ce_move_rows(const CeParams &p, int b, int h, int n, const int *pairs) {
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)b * p.Hkv + h;
+    const CaView ko = p.K_out ? p.ko : p.k, vo = p.K_out ? p.vo : p.v;
+    char *Ko = (char *)(p.K_out ? p.K_out : p.K) + b * ko.b + h * ko.h, *Vo = (char *)(p.K_out ? p.V_out : p.V) + b * vo.b + h * vo.h;
+    const char *K = (const char *)p.K + b * p.k.b + h * p.k.h, *V = (const char *)p.V + b * p.v.b + h * p.v.h;
+    ca_copy_rows<P>(n, p.row_bytes, lane, [&](int i, const P *&ks, P *&kd, const P *&vs, P *&vd) {
+        const long long from = pairs[2 * i], to = pairs[2 * i + 1];
+        ks = (const P *)(K + from * p.k.l); kd = (P *)(Ko + to * ko.l);
+        vs = (const P *)(V + from * p.v.l); vd = (P *)(Vo + to * vo.l);
+    });
+    float *wo = p.K_out ? p.weights_out + unit * p.S_out : p.weights + unit * p.S;
+    int *po = p.K_out ? p.pos_out + unit * p.S_out : p.pos + unit * p.S;
+    for (int i = lane; i < n; i += 32) {
+        wo[pairs[2 * i + 1]] = p.weights[unit * p.S + pairs[2 * i]];
+        if (p.pos) po[pairs[2 * i + 1]] = p.pos[unit * p.S + pairs[2 * i]];
+    }
+}
+
 // A cluster per (sequence, head), each CTA a piece of its rows, finds the rows that stay and writes `kept`:
 //   the m-th largest rank by its digits from the top: three histograms over the rows that share the prefix found so far, added up over the cluster;
 //   bit masks over the rows - above that rank, equal to it; of the equal rows the first that there is room for stay;
 //   into another cache: the numbers of the rows that stay are their new places.  In place: the kept rows from m on are listed by their number, and the i-th
 //   freed row below m takes the i-th of them, from the list of the CTA that has it.
+// Where few rows leave, in place, they are picked one after the other instead: a reduction over the block each.
 // Bound by latency: three passes over shared memory and some ten barriers.
-//   32 sequences x 8 heads, up to 4102 rows: 22 us with 1024 threads that read weights and positions anew in each pass; 4 x 8 heads, up to 32768 rows: 91 us
-__global__ void __launch_bounds__(CE_THREADS)
+//   32 sequences x 8 heads, up to 4102 rows: 22 us with 1024 threads that read weights and positions anew in each pass, 19 with the ranks in shared memory, 23
+//   with two bits a round by counting; 4 x 8 heads, up to 32768 rows: 91, 33
+template <typename P>
+__global__ void __launch_bounds__(CE_THREADS, 2)
 ce_select_kernel(const CeParams p) {
-    extern __shared__ unsigned ce_smem[];
-    __shared__ int hist[CE_BINS], s_warp[CE_THREADS / 32], s_count[4];
+    extern __shared__ __align__(16) unsigned ce_smem[];
+    __shared__ int s_warp[CE_THREADS / 32], s_count[4], s_pairs[CE_FEW * 2];
     __shared__ int s_digit, s_above;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
     uint32_t cl;
@@ -650,58 +685,138 @@ ce_select_kernel(const CeParams p) {
     }
     const int chunk = min((int)(((n + cl - 1) / cl + 31) & ~31), p.chunk_most);   // rows of a CTA: whole words
     const int lo = min((int)rank * chunk, n), rows = min(chunk, n - lo), words = (rows + 31) / 32;
-    unsigned *stays = ce_smem, *equal = stays + p.chunk_most / 32;
+    int *hists = (int *)ce_smem;
+    unsigned *stays = ce_smem + CE_HISTS / 4, *equal = stays + p.chunk_most / 32;
     int *number = (int *)(equal + p.chunk_most / 32);
     unsigned short *list = (unsigned short *)(number + p.chunk_most / 32);
     unsigned *ranks = (unsigned *)(list + p.chunk_most);
     const float *w = p.weights + unit * p.S + lo;
     const int *pos = p.pos ? p.pos + unit * p.S + lo : nullptr;
-    const long long recent = (long long)(p.next_pos ? p.next_pos[b] : n) - p.recent;
+    const int recent = (int)max((long long)(p.next_pos ? p.next_pos[b] : n) - p.recent, -0x80000000ll);
     auto rank_of = [&](int r) {   // of row lo + r
         const int at = pos ? pos[r] : lo + r;
         return ce_rank(w[r], at < p.sink || at >= recent);
     };
+    const bool pick = cl == 1 && p.cached && !p.K_out && n - m <= CE_PICK;
+    if (pick)
+        for (int i = tid; i < m; i += CE_THREADS) kept[i] = i;   // (freed rows are put right below)
+    else
+        for (int i = tid; i < (CE_COPIES + 2) * CE_BINS / 4; i += CE_THREADS) reinterpret_cast<int4 *>(hists)[i] = make_int4(0, 0, 0, 0);
     if (p.cached) {
-        for (int r0 = 0; r0 < rows; r0 += 4 * CE_THREADS) {
-            unsigned x[4];
+        for (int r0 = tid; r0 < rows; r0 += 8 * CE_THREADS) {   // eight rows' requests in flight
+            float x[8];
+            int at[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = r0 + k * CE_THREADS + tid < rows ? rank_of(r0 + k * CE_THREADS + tid) : 0u;
+            for (int k = 0; k < 8; ++k) {
+                const int r = min(r0 + k * CE_THREADS, rows - 1);
+                x[k] = w[r];
+                at[k] = pos ? pos[r] : lo + r;
+            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (r0 + k * CE_THREADS + tid < rows) ranks[r0 + k * CE_THREADS + tid] = x[k];
+            for (int k = 0; k < 8; ++k)
+                if (r0 + k * CE_THREADS < rows) ranks[r0 + k * CE_THREADS] = ce_rank(x[k], at[k] < p.sink || at[k] >= recent);
         }
     }
     auto rank_at = [&](int r) { return p.cached ? ranks[r] : rank_of(r); };   // (a thread asks for the rows that it has written itself)
     unsigned prefix = 0;
     int need = m;   // rows to take from those that share the prefix
-    for (int shift = 32 - CE_BITS;; shift = shift > CE_BITS ? shift - CE_BITS : 0) {
-        const int bits = shift == 0 ? 32 - 2 * CE_BITS : CE_BITS;
-        for (int i = tid; i < CE_BINS; i += CE_THREADS) hist[i] = 0;
+    if (pick) {
+        // ---- a step's eviction: the row of least rank (of those, the last) leaves, n - m times ----
+        unsigned *gone = stays, least;
+        int *left = number, last;   // the rows that leave
+        for (int i = tid; i < words; i += CE_THREADS) gone[i] = 0;
         __syncthreads();
-        for (int r0 = 0; r0 < rows; r0 += CE_THREADS) {
-            const int r = r0 + tid;
-            const unsigned x = r < rows ? rank_at(r) : 0u;
-            const bool in = r < rows && (shift + bits == 32 || (x >> (shift + bits)) == (prefix >> (shift + bits)));
-            const unsigned d = (x >> shift) & ((1u << bits) - 1);
-            // equal digits are common (weights of 0): those equal to the first lane's are added at once
-            const unsigned who = __ballot_sync(0xffffffffu, in);
-            if (who) {
-                const int leader = __ffs(who) - 1;
-                const unsigned d0 = __shfl_sync(0xffffffffu, d, leader), same = __ballot_sync(0xffffffffu, in && d == d0);
-                if (lane == leader) atomicAdd(&hist[d0], __popc(same));
-                if (in && d != d0) atomicAdd(&hist[d], 1);
+        auto look = [&]() {   // at this thread's rows
+            least = 0xffffffffu;
+            last = -1;
+            for (int r = tid; r < rows; r += CE_THREADS)
+                if (ranks[r] <= least && !(gone[r >> 5] >> (r & 31) & 1u)) { least = ranks[r]; last = r; }
+        };
+        look();
+        uint2 *s_round = reinterpret_cast<uint2 *>(hists);   // [2][warps]
+        const int k = n - m;
+        for (int i = 0; i < k; ++i) {
+            const unsigned x = __reduce_min_sync(0xffffffffu, least);
+            const int r = __reduce_max_sync(0xffffffffu, least == x ? last : -1);
+            uint2 *at = s_round + (i & 1) * (CE_THREADS / 32);
+            if (lane == 0) at[warp] = make_uint2(x, (unsigned)r);
+            __syncthreads();
+            const uint2 v = at[lane % (CE_THREADS / 32)];
+            const unsigned y = __reduce_min_sync(0xffffffffu, v.x);
+            const int out = __reduce_max_sync(0xffffffffu, v.x == y ? (int)v.y : -1);
+            if (out % CE_THREADS == tid) {
+                atomicOr(&gone[out >> 5], 1u << (out & 31));
+                left[i] = out;
+                look();
             }
         }
-        ce_cluster_sync(cl);
-        // thread i has the digits CE_BINS - 1 - CE_PER i downwards
-        int c[CE_PER], sum = 0;
-#pragma unroll
-        for (int k = 0; k < CE_PER; ++k) {
-            const int at = CE_BINS - 1 - CE_PER * tid - k;
-            c[k] = hist[at];
-            for (uint32_t o = 1; o < cl; ++o) c[k] += ce_remote(&hist[at], (rank + o) % cl);
-            sum += c[k];
+        __syncthreads();
+        int holes = 0;
+        if (warp == 0) {
+            const int e = lane < k ? left[lane] : n;
+            int before = 0;
+            bool moves = lane < k;   // row m + lane stays, and moves
+            for (int j = 0; j < k; ++j) {
+                const int o = __shfl_sync(0xffffffffu, e, j);
+                if (o < e) ++before;
+                if (o == m + lane) moves = false;
+            }
+            const unsigned who = __ballot_sync(0xffffffffu, moves);
+            if (e < m) s_pairs[2 * before + 1] = e;
+            if (moves) s_pairs[2 * __popc(who & ((1u << lane) - 1u))] = m + lane;
+            if (lane == 0) s_count[0] = __popc(who);
         }
+        __syncthreads();
+        holes = s_count[0];
+        if (tid < holes) kept[s_pairs[2 * tid + 1]] = s_pairs[2 * tid];
+        const int each = (holes + CE_THREADS / 32 - 1) / (CE_THREADS / 32), k0 = warp * each, k1 = min(k0 + each, holes);
+        if (k0 < k1) ce_move_rows<P>(p, b, h, k1 - k0, s_pairs + 2 * k0);
+        return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? CE_BITS : 32 - 2 * CE_BITS, shift = pass < 2 ? 32 - (pass + 1) * CE_BITS : 0;
+        int *hist = hists + (pass == 0 ? 0 : CE_COPIES + pass - 1) * CE_BINS, *copy = hist + (pass == 0 ? (warp % CE_COPIES) * CE_BINS : 0);
+        for (int r0 = 0; r0 < rows; r0 += 4 * CE_THREADS) {
+            unsigned x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = r0 + k * CE_THREADS + tid < rows ? rank_at(r0 + k * CE_THREADS + tid) : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = r0 + k * CE_THREADS + tid < rows && (pass == 0 || ((x[k] ^ prefix) >> (shift + bits)) == 0);
+                const unsigned d = (x[k] >> shift) & ((1u << bits) - 1);
+                // equal digits are common (weights of 0): those equal to the first lane's are added at once
+                const unsigned who = __ballot_sync(0xffffffffu, in);
+                if (who == 0) continue;
+                const int leader = __ffs(who) - 1;
+                const unsigned d0 = __shfl_sync(0xffffffffu, d, leader), same = __ballot_sync(0xffffffffu, in && d == d0);
+                if (lane == leader) atomicAdd(&copy[d0], __popc(same));
+                if (in && d != d0) atomicAdd(&copy[d], 1);
+            }
+        }
+        // thread i has the digits CE_BINS - 1 - CE_PER i downwards
+        static_assert(CE_PER == 4, "a thread's bins are 16 bytes");
+        int4 *mine4 = reinterpret_cast<int4 *>(hist) + (CE_THREADS - 1 - tid);
+        if (pass == 0) {
+            __syncthreads();
+            int4 q = *mine4;
+#pragma unroll
+            for (int k = 1; k < CE_COPIES; ++k) {
+                const int4 v = mine4[k * CE_BINS / 4];
+                q.x += v.x; q.y += v.y; q.z += v.z; q.w += v.w;
+            }
+            *mine4 = q;
+        }
+        ce_cluster_sync(cl);
+        int4 q = *mine4;
+#pragma unroll
+        for (uint32_t o = 1; o < 8; ++o) {
+            if (o >= cl) break;
+            const int4 v = ce_remote4(mine4, (rank + o) % cl);
+            q.x += v.x; q.y += v.y; q.z += v.z; q.w += v.w;
+        }
+        const int c[CE_PER] = {q.w, q.z, q.y, q.x}, sum = q.x + q.y + q.z + q.w;
         int all;
         int before = ce_scan(sum, s_warp, &all);
         if (before < need && before + sum >= need) {
@@ -711,13 +826,12 @@ ce_select_kernel(const CeParams p) {
                 before += c[k];
             }
         }
-        ce_cluster_sync(cl);   // (and the histograms have been read by the others)
+        __syncthreads();
         prefix |= (unsigned)s_digit << shift;
         need -= s_above;
-        if (shift == 0) break;
-        __syncthreads();
     }
     int equals = 0;
+#pragma unroll 4
     for (int i = warp; i < words; i += CE_THREADS / 32) {
         const int r = 32 * i + lane;
         // (with the ranks in shared memory this reads what other threads wrote: they have met since)
@@ -773,6 +887,7 @@ ce_select_kernel(const CeParams p) {
     }
     const int base = in_front(all, 1, nullptr);   // (a barrier: the numbers are there)
     __syncthreads();
+#pragma unroll 4
     for (int i = warp; i < words; i += CE_THREADS / 32) {
         const unsigned bits = into ? stays[i] : stays[i] & ~front(i);
         if (bits >> lane & 1u) {
@@ -799,8 +914,9 @@ ce_select_kernel(const CeParams p) {
     for (int i = warp; i < words; i += CE_THREADS / 32) {
         const unsigned f = front(i), free = ~stays[i] & f;
         if (f == 0) break;
+        int from = -1;
         if (f >> lane & 1u) {
-            int from = lo + 32 * i + lane;
+            from = lo + 32 * i + lane;
             if (free >> lane & 1u) {
                 int at = holes + number[i] + __popc(free & ((1u << lane) - 1u));
                 uint32_t o = 0;
@@ -813,42 +929,41 @@ ce_select_kernel(const CeParams p) {
             }
             kept[lo + 32 * i + lane] = from;
         }
+        if (n - m <= CE_FEW && (free >> lane & 1u)) {
+            const int k = number[i] + __popc(free & ((1u << lane) - 1u));
+            s_pairs[2 * k] = from;
+            s_pairs[2 * k + 1] = lo + 32 * i + lane;
+        }
     }
-    ce_cluster_sync(cl);   // (nobody leaves while its list is being read)
+    ce_cluster_sync(cl);   // (nobody leaves while its list is being read; the pairs are there)
+    if (n - m <= CE_FEW) {
+        const int each = (all + CE_THREADS / 32 - 1) / (CE_THREADS / 32), k0 = warp * each, k1 = min(k0 + each, all);
+        if (k0 < k1) ce_move_rows<P>(p, b, h, k1 - k0, s_pairs + 2 * k0);
+    }
 }
 
-// Moves what `kept` says: a warp per row.  In place the sources are rows >= m and the targets rows < m, so that no move reads what another writes.
+// Moves what `kept` says: a warp per 32 rows.
 template <typename P>
 __global__ void __launch_bounds__(CC_THREADS)
 ce_move_kernel(const CeParams p) {
+    __shared__ int s_pairs[CC_THREADS * 2];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31, b = blockIdx.z, h = blockIdx.y;
-    const long long unit = (long long)b * p.Hkv + h;
-    const int i0 = (blockIdx.x * (CC_THREADS / 32) + (threadIdx.x >> 5)) * 32;
-    const int mine = i0 + lane < p.keep ? p.kept[unit * p.keep + i0 + lane] : -1;
-    const bool moves = mine >= 0 && (p.K_out || mine != i0 + lane);
-    // the rows that move, closed up: lane i has the i-th of them
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, h = blockIdx.y;
+    const int n = ca_len(p.len, b, p.S), m = min(n, p.keep), to = (blockIdx.x * (CC_THREADS / 32) + warp) * 32 + lane;
+    if (!p.K_out && n - m <= CE_FEW) return;   // (few rows have moved already)
+    const int from = to < m ? p.kept[((long long)b * p.Hkv + h) * p.keep + to] : -1;
+    const bool moves = from >= 0 && (p.K_out || from != to);
     const unsigned todo = __ballot_sync(0xffffffffu, moves);
     if (todo == 0) return;
-    const int to = __fns(todo, 0, lane + 1), from = __shfl_sync(0xffffffffu, mine, to >= 0 && to < 32 ? to : 0);
-    const CaView ko = p.K_out ? p.ko : p.k, vo = p.K_out ? p.vo : p.v;
-    char *Ko = (char *)(p.K_out ? p.K_out : p.K) + b * ko.b + h * ko.h + i0 * ko.l, *Vo = (char *)(p.K_out ? p.V_out : p.V) + b * vo.b + h * vo.h + i0 * vo.l;
-    const char *K = (const char *)p.K + b * p.k.b + h * p.k.h, *V = (const char *)p.V + b * p.v.b + h * p.v.h;
-    __shared__ int s_from[CC_THREADS], s_to[CC_THREADS];
-    s_from[threadIdx.x] = from;
-    s_to[threadIdx.x] = to;
-    __syncwarp();
-    const int *wf = s_from + (threadIdx.x & ~31), *wt = s_to + (threadIdx.x & ~31);
-    ca_copy_rows<P>(__popc(todo), p.row_bytes, lane, [&](int i, const P *&ks, P *&kd, const P *&vs, P *&vd) {
-        ks = (const P *)(K + wf[i] * p.k.l); kd = (P *)(Ko + wt[i] * ko.l);
-        vs = (const P *)(V + wf[i] * p.v.l); vd = (P *)(Vo + wt[i] * vo.l);
-    });
+    int *pairs = s_pairs + warp * 64;
     if (moves) {
-        float *wo = p.K_out ? p.weights_out + unit * p.S_out : p.weights + unit * p.S;
-        wo[i0 + lane] = p.weights[unit * p.S + mine];
-        if (p.pos) (p.K_out ? p.pos_out + unit * p.S_out : p.pos + unit * p.S)[i0 + lane] = p.pos[unit * p.S + mine];
+        const int i = __popc(todo & ((1u << lane) - 1u));
+        pairs[2 * i] = from;
+        pairs[2 * i + 1] = to;
     }
+    __syncwarp();
+    ce_move_rows<P>(p, b, h, __popc(todo), pairs);
 }
 
 }  // namespace b200attn
