@@ -114,7 +114,9 @@ int validate(const b200attn_attend_args *a, bool pointers) {
 }
 
 // Workspace: the slots of cut units, then the entries.
-size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + (size_t)p.grid * 8 * sizeof(int); }
+long long units(const CaParams &p) { return (long long)p.B * p.Hkv * p.nrt; }
+size_t entries_bytes(const CaParams &p) { return (size_t)(p.by_cta ? p.grid : units(p)) * 8 * sizeof(int); }
+size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + entries_bytes(p); }
 
 #include <cstdlib>
 static int env_oh(int d) { const char *e = getenv("CA_OH"); return e ? atoi(e) : d; }
@@ -122,6 +124,10 @@ void share_out(CaParams &p, int RT, int TK, int OH, int grid) {
     p.RT = RT; p.TK = TK; p.OH = OH; p.grid = grid;
     p.nrt = (p.R + RT - 1) / RT;
     p.DT = 0;
+    // few units are cut into many parts each, which a block's warps share out: then a block has as many rows as it can take at once
+    p.by_cta = units(p) > grid;
+    const long long parts = grid / units(p) + 1;
+    p.join_rows = p.by_cta ? 16 : parts <= 4 ? 8 : parts <= 8 ? 4 : parts <= 16 ? 2 : 1;
     if (p.drafts)
         for (int rt = 0; rt < p.nrt; ++rt) p.DT += ca_draft_tiles(rt, p.R, RT, p.G, p.T, TK, p.mask == nullptr);
 }
@@ -137,21 +143,27 @@ void fill(CaParams &p, const b200attn_attend_args &a) {
     p.scale_log2 = (a.scale == 0.0f ? 1.0f / sqrtf((float)a.head_d) : a.scale) * 1.4426950408889634f;
 }
 
-template <typename T, int DB>
-int launch_generic(const CaParams &p, const HostCall &c, cudaStream_t st) {
-    const size_t smem = cg_smem_bytes(p.D);
-    int rc = raise_smem<ca_generic_kernel<T, DB>>(c);
-    if (rc) return rc;
-    CU_TRY(launch_dependent(ca_generic_kernel<T, DB>, dim3((unsigned)p.grid), CG_THREADS, smem, 1, st, p));
+template <typename T>
+int launch_combine(const CaParams &p, cudaStream_t st) {
+    const dim3 grid((unsigned)(p.by_cta ? p.grid : units(p)), (unsigned)(((p.RT < p.R ? p.RT : p.R) + p.join_rows - 1) / p.join_rows));
+    CU_TRY(p.D <= 64 ? launch_dependent(ca_combine_kernel<T, 2>, grid, CB_THREADS, 0, 1, st, p)
+                     : p.D <= 128 ? launch_dependent(ca_combine_kernel<T, 4>, grid, CB_THREADS, 0, 1, st, p) : launch_dependent(ca_combine_kernel<T, 8>, grid, CB_THREADS, 0, 1, st, p));
+    count_launches(2);   // with the kernel whose parts these are
     return B200ATTN_OK;
 }
-template <typename T>
-int launch_attend(const CaParams &p, const HostCall &c, cudaStream_t st) {
-    int rc = p.D <= 64 ? launch_generic<T, 64>(p, c, st) : p.D <= 128 ? launch_generic<T, 128>(p, c, st) : launch_generic<T, 256>(p, c, st);
+template <typename T, int DB, bool FAST>
+int launch_generic(const CaParams &p, const HostCall &c, cudaStream_t st) {
+    const size_t smem = cg_smem_bytes(p.D);
+    int rc = raise_smem<ca_generic_kernel<T, DB, FAST>>(c);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
-    count_launches(2);
+    CU_TRY(launch_dependent(ca_generic_kernel<T, DB, FAST>, dim3((unsigned)p.grid), CG_THREADS, smem, 1, st, p));
     return B200ATTN_OK;
+}
+template <typename T, bool FAST>
+int launch_attend(const CaParams &p, const HostCall &c, cudaStream_t st) {
+    int rc = p.D <= 64 ? launch_generic<T, 64, FAST>(p, c, st) : p.D <= 128 ? launch_generic<T, 128, FAST>(p, c, st) : launch_generic<T, 256, FAST>(p, c, st);
+    if (rc) return rc;
+    return launch_combine<T>(p, st);
 }
 
 // The tensor-core kernel for these sizes: rows of a tile, tiles of a unit, ring.
@@ -215,9 +227,7 @@ int launch_attend_tc(const CtParams &ct, const HostCall &c, const CUtensorMap (&
     const CaParams &p = ct.a;
     int rc = p.TK == 64 ? launch_tc<1, 64, F16>(ct, c, m, st) : p.RT > ct.tpt * p.G ? launch_tc<2, 128, F16>(ct, c, m, st) : launch_tc<1, 128, F16>(ct, c, m, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
-    count_launches(2);
-    return B200ATTN_OK;
+    return launch_combine<typename CtType<F16>::T>(p, st);
 }
 
 template <int N, bool F16>
@@ -233,9 +243,7 @@ int launch_attend_narrow(const CnParams &cn, const HostCall &c, const CUtensorMa
     const CaParams &p = cn.a;
     int rc = p.R <= 16 ? launch_narrow<16, F16>(cn, c, m, st) : p.R <= 32 ? launch_narrow<32, F16>(cn, c, m, st) : launch_narrow<64, F16>(cn, c, m, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ca_combine_kernel<typename CtType<F16>::T>, dim3((unsigned)p.grid, cb_blocks(p)), CB_THREADS, 0, 1, st, p));
-    count_launches(2);
-    return B200ATTN_OK;
+    return launch_combine<typename CtType<F16>::T>(p, st);
 }
 
 int attend(const b200attn_attend_args *a, size_t *need) {
@@ -275,10 +283,11 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     }
     CaParams &q = narrow ? cn.a : tc ? ct.a : p;
     q.part = (float *)ws;
-    q.entries = (int *)((char *)ws + attend_bytes(q) - (size_t)q.grid * 8 * sizeof(int));
+    q.entries = (int *)((char *)ws + attend_bytes(q) - entries_bytes(q));
     if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, c, m, st) : launch_attend_narrow<false>(cn, c, m, st);
     else if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, c, m, st) : launch_attend_tc<false>(ct, c, m, st);
-    else rc = a->dtype == B200ATTN_F32 ? launch_attend<float>(p, c, st) : a->dtype == B200ATTN_F16 ? launch_attend<__half>(p, c, st) : launch_attend<__nv_bfloat16>(p, c, st);
+    else if (a->dtype == B200ATTN_F32) rc = p.D % 4 == 0 && tc_aligned(a) ? launch_attend<float, true>(p, c, st) : launch_attend<float, false>(p, c, st);
+    else rc = a->dtype == B200ATTN_F16 ? launch_attend<__half, false>(p, c, st) : launch_attend<__nv_bfloat16, false>(p, c, st);
     if (rc) return rc;
     set_last_path(narrow ? "cache_narrow" : tc ? "cache_tc" : "cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
@@ -337,12 +346,12 @@ int commit(const b200attn_commit_args *a) {
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 
-template <typename T>
+template <typename T, bool FAST>
 int launch_weights(const CwParams &p, const HostCall &c, cudaStream_t st) {
     const size_t smem = cg_smem_bytes(p.D);
-    int rc = raise_smem<cw_generic_kernel<T>>(c);
+    int rc = raise_smem<cw_generic_kernel<T, FAST>>(c);
     if (rc) return rc;
-    CU_TRY(launch_dependent(cw_generic_kernel<T>, dim3((unsigned)((p.S + CG_KEYS - 1) / CG_KEYS), (unsigned)p.Hkv, (unsigned)p.B), CG_THREADS, smem, 1, st, p));
+    CU_TRY(launch_dependent(cw_generic_kernel<T, FAST>, dim3((unsigned)((p.S + CG_KEYS - 1) / CG_KEYS), (unsigned)p.Hkv, (unsigned)p.B), CG_THREADS, smem, 1, st, p));
     count_launches(1);
     return B200ATTN_OK;
 }
@@ -422,7 +431,8 @@ int weights(const b200attn_weights_args *a) {
         return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
     }
     if (rc != -1) return rc;
-    rc = a->dtype == B200ATTN_F32 ? launch_weights<float>(p, c, st) : a->dtype == B200ATTN_F16 ? launch_weights<__half>(p, c, st) : launch_weights<__nv_bfloat16>(p, c, st);
+    if (a->dtype == B200ATTN_F32) rc = p.D % 4 == 0 && strides_fit(a->K, a->dtype, p.B, p.Hkv, p.S) ? launch_weights<float, true>(p, c, st) : launch_weights<float, false>(p, c, st);
+    else rc = a->dtype == B200ATTN_F16 ? launch_weights<__half, false>(p, c, st) : launch_weights<__nv_bfloat16, false>(p, c, st);
     if (rc) return rc;
     set_last_path("cache_generic");
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);

@@ -39,7 +39,9 @@ struct CaParams {
     int grid;            // CTAs that share the items out
     float scale_log2;    // scale * log2(e)
     float *part;         // [grid][2] slots of [RT][D] accumulators and [RT][2] (m in log2 units, l)
-    int *entries;        // [grid][8]: the cut unit whose first cut lies in front of this CTA (ca_entry)
+    int *entries;        // [8] words each: cut units (ca_entry_of_unit, ca_entry_of_cta)
+    int by_cta;          // ... per CTA, else per unit
+    int join_rows;       // rows that a block of ca_combine_kernel joins
     unsigned *err, *err_sys;
     unsigned spin_limit;
 };
@@ -152,9 +154,19 @@ struct CaWalk {
     }
 };
 
-// By one thread, for the first unit of a CTA's range: where that unit was cut by this range's beginning, and by none before it, its parts are
-// listed for ca_combine_kernel: {first CTA or -1, its slot, last CTA, b, h, rt}.  Every other part is in slot 0 of its CTA.
-__device__ __forceinline__ void ca_entry(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
+// What ca_combine_kernel goes by, {first CTA of a cut unit or -1, its slot, last CTA, b, h, rt}; every other part is in slot 0 of its CTA.  Kept per unit where
+// there are no more units than CTAs: written by the CTA with the unit's first tile, which calls this for each of its units ...
+__device__ __forceinline__ void ca_entry_of_unit(const CaParams &p, const CaStart &s, const CaWalk &w, int c, bool first_of_range) {
+    if (p.by_cta || w.tile(p) != 0) return;
+    int *e = p.entries + (((size_t)w.b * p.Hkv + w.h) * p.nrt + w.rt) * 8;
+    e[1] = first_of_range ? 0 : 1;
+    e[2] = ca_cta_of(s.total, s.grid, w.u0 + p.OH + w.nt - 1);
+    e[3] = w.b; e[4] = w.h; e[5] = w.rt;
+    e[0] = w.whole(p) ? -1 : c;
+}
+// ... else per CTA: by each CTA for the first unit of its range, which is listed where it was cut by this range's beginning and by none before it.
+__device__ __forceinline__ void ca_entry_of_cta(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
+    if (!p.by_cta) return;
     int *e = p.entries + (size_t)c * 8;
     e[0] = -1;
     if (w.left == 0 || w.at <= p.OH) return;
@@ -176,89 +188,151 @@ __device__ __forceinline__ const T *ca_row(const void *base, const CaView &v, in
 }
 
 // ---- joining the parts of cut units ---------------------------------------------------------------------------------
-// Block (c, y): rows CB_ROWS y .. of the unit that entry c lists.  A row's warps first take all parts' (m, l), a part per lane, for the row's maximum and
-// sum; then the parts' accumulators with their weights, four requests in flight per column.  A row is taken by `per` warps that share its parts
-// out, so that a row cut over the whole chip (one sequence, one key head) does not wait for one part after the other.
-//   8 key heads x 4 rows in 7 parts each: 11 us with a dependent chain through (m, l, accumulator) of each part
-constexpr int CB_THREADS = 256, CB_ROWS = 16;
+// Block (c, y): rows join_rows y .. of the unit that entry c lists.  A row is taken by `per` warps that share its parts out, so that a row cut over the whole
+// chip (one sequence, one key head) does not wait for one part after the other; a warp asks for its first four parts' accumulators before it knows their
+// weights, which it takes from all parts' (m, l), a part per lane.
+//   16 units x 7 rows in some 40 parts each: 40 us with 16 rows a block, one after the other; 8 x 4 rows in 7 parts: 11 us with a chain through the parts
+constexpr int CB_THREADS = 256;
 
-template <typename T>
+template <typename T, int NI>   // NI: columns of a lane
 __global__ void __launch_bounds__(CB_THREADS)
 ca_combine_kernel(const CaParams p) {
-    __shared__ float s_acc[8][CA_MAX_D];
+    __shared__ float s_acc[8][NI * 32];
     grid_launch_dependents();
     grid_dependency_wait();
     const int4 e0 = *reinterpret_cast<const int4 *>(p.entries + (size_t)blockIdx.x * 8);
+    const int2 e1 = *reinterpret_cast<const int2 *>(p.entries + (size_t)blockIdx.x * 8 + 4);
     const int first = e0.x;
     if (first < 0) return;
-    const int2 e1 = *reinterpret_cast<const int2 *>(p.entries + (size_t)blockIdx.x * 8 + 4);
     const int slot0 = e0.y, parts = e0.z - first + 1, b = e0.w, h = e1.x, rt = e1.y;
-    const int rows = min(min(p.RT, p.R - rt * p.RT), (int)(blockIdx.y + 1) * CB_ROWS), row0 = blockIdx.y * CB_ROWS;
+    const int row0 = blockIdx.y * p.join_rows, rows = min(min(p.RT, p.R - rt * p.RT), row0 + p.join_rows);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = parts <= 8 ? 1 : parts <= 16 ? 2 : parts <= 32 ? 4 : 8;   // warps of a row
+    const int per = parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8;   // warps of a row
     const size_t slot = ca_slot_floats(p.RT, p.D), ml = (size_t)p.RT * p.D;
     auto part = [&](int c) { return p.part + ((size_t)(first + c) * 2 + (c == 0 ? slot0 : 0)) * slot; };
     for (int r0 = row0; r0 < rows; r0 += 8 / per) {
-        const int row = r0 + warp / per;
-        const bool mine = row < rows;
-        float m = -INFINITY, l = 0.0f, acc[CA_MAX_D / 32];
+        const int row = min(r0 + warp / per, rows - 1), w0 = warp % per;
+        const bool mine = r0 + warp / per < rows;
+        float acc[NI], o[4][NI], m = -INFINITY, l = 0.0f;
+        auto ask = [&](int k0) {   // parts k0, k0 + per, ..
 #pragma unroll
-        for (int i = 0; i < CA_MAX_D / 32; ++i) acc[i] = 0.0f;
-        if (mine) {
-            for (int c = lane; c < parts; c += 32) m = fmaxf(m, part(c)[ml + 2 * row]);
-            m = warp_max(m);
-            for (int c0 = 0; c0 < parts; c0 += 32) {
-                const int c = c0 + lane;
-                float w = 0.0f;
-                if (c < parts) {
-                    const float2 x = *reinterpret_cast<const float2 *>(part(c) + ml + 2 * row);
-                    w = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
-                    l += w * x.y;
-                }
-                const int n = min(32, parts - c0);
-#pragma unroll 4
-                for (int k = warp % per; k < n; k += per) {
-                    const float wk = __shfl_sync(0xffffffffu, w, k);
-                    const float *o = part(c0 + k) + (size_t)row * p.D;
+            for (int u = 0; u < 4; ++u) {
+                const float *from = part(min(k0 + u * per, parts - 1)) + (size_t)row * p.D;
 #pragma unroll
-                    for (int i = 0; i < CA_MAX_D / 32; ++i)
-                        if (lane + 32 * i < p.D) acc[i] = fmaf(o[lane + 32 * i], wk, acc[i]);
+                for (int i = 0; i < NI; ++i) o[u][i] = lane + 32 * i < p.D ? from[lane + 32 * i] : 0.0f;
+            }
+        };
+        ask(w0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i] = 0.0f;
+        float2 x = make_float2(-INFINITY, 0.0f);   // of part `lane`
+        if (lane < parts) x = *reinterpret_cast<const float2 *>(part(lane) + ml + 2 * row);
+        m = x.x;
+        for (int c = lane + 32; c < parts; c += 32) m = fmaxf(m, part(c)[ml + 2 * row]);
+        m = warp_max(m);
+        for (int c0 = 0; c0 < parts; c0 += 32) {
+            if (c0 > 0) {
+                x = make_float2(-INFINITY, 0.0f);
+                if (c0 + lane < parts) x = *reinterpret_cast<const float2 *>(part(c0 + lane) + ml + 2 * row);
+            }
+            const float w = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
+            l += w * x.y;
+            for (int k0 = c0 + w0; k0 < min(c0 + 32, parts); k0 += 4 * per) {   // (32 is a multiple of 4 per)
+                if (k0 != w0) ask(k0);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int k = k0 + u * per;
+                    const float wk = __shfl_sync(0xffffffffu, w, (k - c0) & 31);
+                    if (k < parts) {
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) acc[i] = fmaf(o[u][i], wk, acc[i]);
+                    }
                 }
             }
-            l = warp_sum(l);
         }
+        l = warp_sum(l);
         if (per > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < CA_MAX_D / 32; ++i)
-                if (lane + 32 * i < p.D) s_acc[warp][lane + 32 * i] = acc[i];
+            for (int i = 0; i < NI; ++i) s_acc[warp][lane + 32 * i] = acc[i];
             __syncthreads();
-            if (warp % per != 0) continue;
+            if (w0 != 0) continue;
             for (int w = warp + 1; w < warp + per; ++w)
 #pragma unroll
-                for (int i = 0; i < CA_MAX_D / 32; ++i)
-                    if (lane + 32 * i < p.D) acc[i] += s_acc[w][lane + 32 * i];
+                for (int i = 0; i < NI; ++i) acc[i] += s_acc[w][lane + 32 * i];
         }
         if (!mine) continue;
         const int r = rt * p.RT + row, t = r / p.G, hq = h * p.G + r % p.G;
-        T *o = ca_row<T>(p.O, p.o, b, hq, t);
+        T *out = ca_row<T>(p.O, p.o, b, hq, t);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int i = 0; i < CA_MAX_D / 32; ++i)
-            if (lane + 32 * i < p.D) o[lane + 32 * i] = OutCvt<T>::one(acc[i] * inv);
+        for (int i = 0; i < NI; ++i)
+            if (lane + 32 * i < p.D) out[lane + 32 * i] = OutCvt<T>::one(acc[i] * inv);
         if (p.lse && lane == 0) p.lse[((long long)b * p.Hq + hq) * p.T + t] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
 }
-inline unsigned cb_blocks(const CaParams &p) { return (unsigned)(((p.RT < p.R ? p.RT : p.R) + CB_ROWS - 1) / CB_ROWS); }
 
 // ---- attention on the CUDA cores: every type, width and stride ---------------------------------------------------------
-// Units of 16 rows, tiles of 64 keys, 128 threads.  K and V pass through shared memory in fp32; a thread computes the scores of one key with
-// eight rows, then owns 16 outputs (8 rows of one column up to head_d 64, else 16 rows) per 128 columns.  Bound by FFMA and shared-memory reads.
+// Units of 16 rows, tiles of 64 keys, 128 threads.  K and V pass through shared memory in fp32: with FAST (fp32 rows on 16 bytes) by asynchronous copies, the
+// next tile's K under this one's softmax and products with V, its V under the next scores; else through registers.  A thread computes the scores of one
+// key with eight rows, then owns 16 outputs (8 rows of one column up to head_d 64, else 16 rows) per 128 columns.  Bound by shared-memory reads: nine of 16 bytes
+// per 32 multiply-adds of a score.
+//   2 x 8 heads, 7 tokens, 1501 and 2999 rows cached, head_d 64, fp32 (18.5 MB): 40 us with element-wise loads, one after the other
 constexpr int CG_ROWS = 16, CG_KEYS = 64, CG_THREADS = 128;
 __host__ __device__ inline int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
 inline size_t cg_smem_bytes(int D) { return ((size_t)(CG_ROWS + 2 * CG_KEYS) * cg_pitch(D) + CG_KEYS * (CG_ROWS + 4)) * sizeof(float); }
 
-template <typename T, int DB>   // DB: columns rounded up to 64, 128 or 256
+__device__ __forceinline__ void cg_copy16(float *dst, const void *src, bool there) {   // zeros where there is nothing to copy
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cg_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cg_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 64 rows of a head from row j0 on into `dst`, those from n on as zeros; the columns behind head_d are zero already where FAST.
+template <typename T, bool FAST>
+__device__ __forceinline__ void cg_load(float *dst, const void *base, const CaView &v, int b, int h, int j0, int n, int D, int S) {
+    const int pitch = cg_pitch(D), tid = threadIdx.x;
+    const T *rows = ca_row<T>(base, v, b, h, 0);
+    if (FAST) {
+        const int pieces = D >> 2;
+        for (int i = tid; i < CG_KEYS * pieces; i += CG_THREADS) {
+            const int j = i / pieces, c = i - j * pieces;
+            cg_copy16(dst + j * pitch + 4 * c, rows + min(j0 + j, S - 1) * v.l + 4 * c, j < n);
+        }
+        cg_commit();
+    } else {
+        for (int i0 = tid; i0 < CG_KEYS * pitch; i0 += 8 * CG_THREADS) {   // eight elements' requests in flight
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = i0 + k * CG_THREADS, j = i / pitch, d = i - j * pitch;
+                x[k] = i < CG_KEYS * pitch && j < n && d < D ? to_f32(rows[(j0 + j) * v.l + d]) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + k * CG_THREADS < CG_KEYS * pitch) dst[i0 + k * CG_THREADS] = x[k];
+        }
+    }
+}
+// Scores of a key's row with eight rows, four running sums each.
+__device__ __forceinline__ void cg_scores(const float *q, const float *k, int pitch, float (&s)[8]) {
+    float4 a[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) a[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int d = 0; d < pitch - 3; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4 *>(k + d);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float4 q4 = *reinterpret_cast<const float4 *>(q + r * pitch + d);
+            a[r].x = fmaf(q4.x, k4.x, a[r].x); a[r].y = fmaf(q4.y, k4.y, a[r].y);
+            a[r].z = fmaf(q4.z, k4.z, a[r].z); a[r].w = fmaf(q4.w, k4.w, a[r].w);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] = (a[r].x + a[r].y) + (a[r].z + a[r].w);
+}
+
+template <typename T, int DB, bool FAST>   // DB: columns rounded up to 64, 128 or 256
 __global__ void __launch_bounds__(CG_THREADS)
 ca_generic_kernel(const CaParams p) {
     extern __shared__ __align__(16) float cg_smem[];
@@ -268,6 +342,8 @@ ca_generic_kernel(const CaParams p) {
     float *qs = cg_smem, *ks = qs + CG_ROWS * pitch, *vs = ks + CG_KEYS * pitch, *ps = vs + CG_KEYS * pitch;   // ps [64 keys][16 rows + 4]
     constexpr int PP = CG_ROWS + 4;
     constexpr int NC = DB <= 128 ? 1 : 2, NR = DB <= 64 ? 8 : 16;
+    if (FAST)   // the columns behind head_d, once
+        for (int i = tid; i < 2 * CG_KEYS * (pitch - p.D); i += CG_THREADS) ks[i / (pitch - p.D) * pitch + p.D + i % (pitch - p.D)] = 0.0f;
     grid_launch_dependents();
     grid_dependency_wait();
     if (warp == 0) {
@@ -277,16 +353,30 @@ ca_generic_kernel(const CaParams p) {
     __syncthreads();
     CaWalk w;
     w.start(p, s_start, blockIdx.x);
-    if (tid == 0) ca_entry(p, s_start, w, blockIdx.x);
+    if (tid == 0) ca_entry_of_cta(p, s_start, w, blockIdx.x);
     const int col = DB <= 64 ? (tid & 63) : tid, rbase = DB <= 64 ? (tid >> 6) * 8 : 0;
     for (bool first = true; w.left > 0; first = false) {
-        const int row0 = w.rt * p.RT, rows = min(p.RT, p.R - row0);
+        const int row0 = w.rt * p.RT, rows = min(p.RT, p.R - row0), end = w.end(p);
+        if (tid == 0) ca_entry_of_unit(p, s_start, w, blockIdx.x, first);
+        auto keys = [&](int tile) { return min(CG_KEYS, tile >= w.ct ? p.T - (tile - w.ct) * CG_KEYS : w.n - tile * CG_KEYS); };   // (0: an empty cache)
+        auto load = [&](float *dst, bool v, int tile) {
+            const bool draft = tile >= w.ct;
+            cg_load<T, FAST>(dst, draft ? (v ? p.Vd : p.Kd) : (v ? p.V : p.K), draft ? (v ? p.vd : p.kd) : (v ? p.v : p.k), w.b, w.h, (draft ? tile - w.ct : tile) * CG_KEYS,
+                             keys(tile), p.D, draft ? p.T : p.S);
+        };
         __syncthreads();
-        for (int i = tid; i < CG_ROWS * pitch; i += CG_THREADS) {
-            const int r = i / pitch, d = i % pitch;
-            float x = 0.0f;
-            if (r < rows && d < p.D) x = to_f32(ca_row<T>(p.Q, p.q, w.b, w.h * p.G + (row0 + r) % p.G, (row0 + r) / p.G)[d]);
-            qs[i] = x;
+        load(ks, false, w.tile(p));
+        load(vs, true, w.tile(p));
+        for (int i0 = tid; i0 < CG_ROWS * pitch; i0 += 4 * CG_THREADS) {
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * CG_THREADS, r = i / pitch, d = i - r * pitch;
+                x[k] = r < rows && d < p.D ? to_f32(ca_row<T>(p.Q, p.q, w.b, w.h * p.G + (row0 + r) % p.G, (row0 + r) / p.G)[d]) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i0 + k * CG_THREADS < CG_ROWS * pitch) qs[i0 + k * CG_THREADS] = x[k];
         }
         if (tid < CG_ROWS) { s_m[tid] = -INFINITY; s_l[tid] = 0.0f; }
         float acc[NC][NR];
@@ -294,49 +384,34 @@ ca_generic_kernel(const CaParams p) {
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int r = 0; r < NR; ++r) acc[c][r] = 0.0f;
-        for (int tile = w.tile(p), end = w.end(p); tile < end; ++tile) {
+        for (int tile = w.tile(p); tile < end; ++tile) {
             const bool draft = tile >= w.ct;
-            const int j0 = (draft ? tile - w.ct : tile) * CG_KEYS, nk = min(CG_KEYS, (draft ? p.T : w.n) - j0);   // keys of the tile (0: an empty cache)
+            const int j0 = (draft ? tile - w.ct : tile) * CG_KEYS, nk = keys(tile);
+            cg_wait<1>();   // K; V may still be on its way
             __syncthreads();
-            for (int i = tid; i < CG_KEYS * pitch; i += CG_THREADS) {
-                const int j = i / pitch, d = i % pitch;
-                float x = 0.0f, y = 0.0f;
-                if (j < nk && d < p.D) {
-                    x = to_f32(draft ? ca_row<T>(p.Kd, p.kd, w.b, w.h, j0 + j)[d] : ca_row<T>(p.K, p.k, w.b, w.h, j0 + j)[d]);
-                    y = to_f32(draft ? ca_row<T>(p.Vd, p.vd, w.b, w.h, j0 + j)[d] : ca_row<T>(p.V, p.v, w.b, w.h, j0 + j)[d]);
-                }
-                ks[i] = x;
-                vs[i] = y;
-            }
-            __syncthreads();
-            {   // scores of key j with rows rb .. rb + 7, in log2 units; what a row does not see is -inf
+            {   // scores of key j with rows rb .. rb + 7; what a row does not see is -inf
                 const int j = tid & 63, rb = (tid >> 6) * 8;
-                float s[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) s[r] = 0.0f;
-                for (int d = 0; d < pitch - 3; d += 4) {
-                    const float4 k4 = *reinterpret_cast<const float4 *>(ks + j * pitch + d);
+                if (rb < rows) {   // (the same for a warp)
+                    float s[8];
+                    cg_scores(qs + rb * pitch, ks + j * pitch, pitch, s);
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        const float4 q4 = *reinterpret_cast<const float4 *>(qs + (rb + r) * pitch + d);
-                        s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
+                        bool see = j < nk && rb + r < rows;
+                        if (see && draft) {
+                            const int t = (row0 + rb + r) / p.G;
+                            see = p.mask ? p.mask[w.b * p.mask_b + (long long)t * p.T + j0 + j] != 0 : j0 + j <= t;
+                        }
+                        ps[j * PP + rb + r] = see ? s[r] : -INFINITY;
                     }
-                }
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    bool see = j < nk && rb + r < rows;
-                    if (see && draft) {
-                        const int t = (row0 + rb + r) / p.G;
-                        see = p.mask ? p.mask[w.b * p.mask_b + (long long)t * p.T + j0 + j] != 0 : j0 + j <= t;
-                    }
-                    ps[j * PP + rb + r] = see ? s[r] * p.scale_log2 : -INFINITY;
                 }
             }
             __syncthreads();
-            for (int r = warp; r < CG_ROWS; r += CG_THREADS / 32) {
+            if (tile + 1 < end) load(ks, false, tile + 1);
+            else if (FAST) cg_commit();   // (an empty group: the counts below stay the same)
+            for (int r = warp; r < rows; r += CG_THREADS / 32) {
                 const float a = ps[lane * PP + r], b = ps[(lane + 32) * PP + r], mo = s_m[r];
-                const float mn = fmaxf(mo, warp_max(fmaxf(a, b)));
-                const float ea = a == -INFINITY ? 0.0f : exp2f(a - mn), eb = b == -INFINITY ? 0.0f : exp2f(b - mn);
+                const float mn = fmaxf(mo, warp_max(fmaxf(a, b)) * p.scale_log2);
+                const float ea = a == -INFINITY ? 0.0f : exp2f(fmaf(a, p.scale_log2, -mn)), eb = b == -INFINITY ? 0.0f : exp2f(fmaf(b, p.scale_log2, -mn));
                 const float sum = warp_sum(ea + eb);
                 ps[lane * PP + r] = ea;
                 ps[(lane + 32) * PP + r] = eb;
@@ -347,25 +422,30 @@ ca_generic_kernel(const CaParams p) {
                     s_m[r] = mn;
                 }
             }
+            cg_wait<1>();   // V; the next K may still be on its way
             __syncthreads();
+            if (rbase < rows) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
+                for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int c = 0; c < NC; ++c) acc[c][r] *= s_f[rbase + r];
-            for (int j = 0; j < nk; ++j) {
-                float v[NC];
+                    for (int c = 0; c < NC; ++c) acc[c][r] *= s_f[rbase + r];
+                for (int j = 0; j < nk; ++j) {
+                    float v[NC], e[NR];
 #pragma unroll
-                for (int c = 0; c < NC; ++c) v[c] = col + 128 * c < pitch ? vs[j * pitch + col + 128 * c] : 0.0f;
+                    for (int c = 0; c < NC; ++c) v[c] = col + 128 * c < pitch ? vs[j * pitch + col + 128 * c] : 0.0f;
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float e = ps[j * PP + rbase + r];
-                    // a key that the row does not see weighs exactly 0; its value may be NaN
+                    for (int r = 0; r < NR; r += 4) *reinterpret_cast<float4 *>(e + r) = *reinterpret_cast<const float4 *>(ps + j * PP + rbase + r);
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) acc[c][r] = draft && e == 0.0f ? acc[c][r] : fmaf(e, v[c], acc[c][r]);
+                    for (int r = 0; r < NR; ++r)
+                        // a key that the row does not see weighs exactly 0; its value may be NaN
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) acc[c][r] = draft && e[r] == 0.0f ? acc[c][r] : fmaf(e[r], v[c], acc[c][r]);
                 }
             }
+            __syncthreads();
+            if (tile + 1 < end) load(vs, true, tile + 1);
+            else if (FAST) cg_commit();
         }
-        __syncthreads();
         const bool whole = w.whole(p);
         float *part = p.part + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
 #pragma unroll
@@ -425,7 +505,7 @@ struct CwParams {
 };
 
 // Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows.
-template <typename T>
+template <typename T, bool FAST>
 __global__ void __launch_bounds__(CG_THREADS)
 cw_generic_kernel(const CwParams p) {
     extern __shared__ __align__(16) float cg_smem[];
@@ -440,10 +520,9 @@ cw_generic_kernel(const CwParams p) {
     if (j0 >= n) return;
     const int count = ca_count(p.accepted, b, p.A, p.T, n);
     if (count == 0) return;
-    for (int i = tid; i < CG_KEYS * pitch; i += CG_THREADS) {
-        const int j = i / pitch, d = i % pitch;
-        ks[i] = j0 + j < n && d < p.D ? to_f32(ca_row<T>(p.K, p.k, b, h, j0 + j)[d]) : 0.0f;
-    }
+    if (FAST)
+        for (int i = tid; i < CG_KEYS * (pitch - p.D); i += CG_THREADS) ks[i / (pitch - p.D) * pitch + p.D + i % (pitch - p.D)] = 0.0f;
+    cg_load<T, FAST>(ks, p.K, p.k, b, h, j0, min(CG_KEYS, n - j0), p.D, p.S);
     const int j = tid & 63, rb = (tid >> 6) * 8;
     float sum = 0.0f;
     for (int r0 = 0; r0 < count * p.G; r0 += CG_ROWS) {
@@ -455,24 +534,22 @@ cw_generic_kernel(const CwParams p) {
             s_i[tid] = x == -INFINITY ? -1 : i;   // a token that saw nothing gave no weight
             s_lse[tid] = x;
         }
-        for (int i = tid; i < CG_ROWS * pitch; i += CG_THREADS) {
-            const int r = r0 + i / pitch, d = i % pitch, a = r / p.G;
-            float x = 0.0f;
-            if (a < count && d < p.D) x = to_f32(ca_row<T>(p.Q, p.q, b, h * p.G + r % p.G, p.accepted ? p.accepted[(long long)b * p.A + a] : a)[d]);
-            qs[i] = x;
-        }
-        __syncthreads();
-        float s[8];
+        for (int i0 = tid; i0 < CG_ROWS * pitch; i0 += 4 * CG_THREADS) {
+            float x[4];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r] = 0.0f;
-        for (int d = 0; d < pitch - 3; d += 4) {
-            const float4 k4 = *reinterpret_cast<const float4 *>(ks + j * pitch + d);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const float4 q4 = *reinterpret_cast<const float4 *>(qs + (rb + r) * pitch + d);
-                s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * CG_THREADS, q = i / pitch, d = i - q * pitch, r = r0 + q, a = r / p.G;
+                x[k] = q < CG_ROWS && a < count && d < p.D ? to_f32(ca_row<T>(p.Q, p.q, b, h * p.G + r % p.G, p.accepted ? p.accepted[(long long)b * p.A + a] : a)[d]) : 0.0f;
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i0 + k * CG_THREADS < CG_ROWS * pitch) qs[i0 + k * CG_THREADS] = x[k];
         }
+        cg_wait<0>();
+        __syncthreads();
+        if (r0 + rb >= count * p.G) continue;   // (the same for a warp)
+        float s[8];
+        cg_scores(qs + rb * pitch, ks + j * pitch, pitch, s);
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const int i = s_i[rb + r];

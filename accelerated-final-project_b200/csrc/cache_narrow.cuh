@@ -105,7 +105,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (elect_one()) {
             CaWalk w;
             w.start(p, s_start, blockIdx.x);
-            ca_entry(p, s_start, w, blockIdx.x);
+            ca_entry_of_cta(p, s_start, w, blockIdx.x);
             int s = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -127,6 +127,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int first = w.tile(p), end = w.end(p), qi = seg & 1;
                 s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, first, end, w.ct, w.whole(p) ? 1 : 0};
                 mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
+                ca_entry_of_unit(p, s_start, w, blockIdx.x, seg == 0);
                 ok = mbar_wait(&bars.q_empty[qi], (uint32_t)(seg >> 1 & 1) ^ 1u, lim);
                 if (!ok) break;
                 mbar_expect_tx(&bars.q_full[qi], (uint32_t)(ng * p.R) * 128u);

@@ -225,7 +225,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
             if (elect_one()) {
                 CaWalk w;
                 w.start(p, s_start, blockIdx.x);
-                ca_entry(p, s_start, w, blockIdx.x);
+                ca_entry_of_cta(p, s_start, w, blockIdx.x);
                 int s = 0;
                 uint32_t ph = 0;
                 bool ok = true;
@@ -245,6 +245,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     // (the slot's last unit is eight back: the ring has been handed back since by everybody who read it)
                     s_seg[seg & (CT_SLOTS - 1)] = CtSeg{w.b, w.h, w.rt, w.n, first, end, w.ct, w.whole(p) ? 1 : 0};
                     mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
+                    ca_entry_of_unit(p, s_start, w, blockIdx.x, seg == 0);
                     const int qi = nq == 2 ? seg & 1 : 0;
                     ok = mbar_wait(&bars.q_empty[qi], (uint32_t)((nq == 2 ? seg >> 1 : seg) & 1) ^ 1u, lim);
                     if (!ok) break;
