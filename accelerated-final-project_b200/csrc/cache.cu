@@ -172,9 +172,10 @@ bool tc_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CtPa
     CtParams ct{};
     ct.tpt = 128 / p.G;
     ct.box_t = p.T < ct.tpt ? p.T : ct.tpt;
-    ct.rows8 = (p.G * ct.box_t + 7) & ~7;
     ct.ng = (p.D + 63) / 64;
-    const int NT = p.D <= 128 && p.T > ct.tpt ? 2 : 1, TK = p.D <= 128 ? 128 : 64;
+    const int NT = p.D <= 128 && p.T > ct.tpt ? 2 : 1;
+    ct.rows8 = NT == 2 ? 128 : (p.G * ct.box_t + 7) & ~7;
+    const int TK = p.D <= 128 ? 128 : 64;
     const size_t room = c.max_smem - 2048 - 1024, stage = (size_t)ct.ng * TK * 128;
     // one row tile: the next unit's Q and the next key tile's P beside the present ones' where four stages remain
     const int buffers[4][2] = {{2, 2}, {1, 2}, {2, 1}, {1, 1}};

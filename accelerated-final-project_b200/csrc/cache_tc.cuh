@@ -28,7 +28,7 @@ constexpr float CT_RESCALE_LOG2 = 8.0f;
 struct CtParams {
     CaParams a;
     int tpt, box_t;      // tokens of a row tile; tokens that a Q box has
-    int rows8;           // rows of a Q or P buffer: those of a box, whole groups of 8
+    int rows8;           // rows of a Q or P buffer: those of a box in whole groups of 8; 128 where a unit has two tiles
     int ng;              // groups of 64 columns
     int nst, nq, np;     // ring stages, Q buffers, P buffers per row tile
 };
@@ -425,8 +425,18 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 const bool draft = i >= nct;
                 const int j0 = (draft ? i - nct : i) * TK;
                 const bool part = draft || i + 1 == nct;   // (the same for every thread) keys that may not be there, or not be seen
+                if (!act) {   // a warp without rows keeps the hand-offs in step
+                    CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.s_read[t][g & 1]);
+                    if (g >= (uint32_t)ct.np) CT_FAIL_AT(5, !pv_done(g - ct.np));
+                    __syncwarp();
+                    if (lane == 0)
+                        for (int h = 0; h < NH; ++h) mbar_arrive(&bars.p_full[t][g & 1][h]);
+                    continue;
+                }
                 uint32_t see[TK / 32];
-                if (part && act) {
+                if (part) {
                     const int valid = !draft ? w.n - j0 : p.mask ? 0 : tok - j0 + 1;
 #pragma unroll
                     for (int x = 0; x < TK / 32; ++x) see[x] = valid >= 32 * (x + 1) ? 0xffffffffu : valid <= 32 * x ? 0u : (1u << (valid - 32 * x)) - 1u;
@@ -446,53 +456,49 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
                 tc_fence_after();
                 const uint32_t ts = tl + (NT == 1 ? (g & 1) : t) * 128u;
-                if (act) {
 #pragma unroll
-                    for (int x = 0; x < TK / 32; ++x) tmem_ld32(ts + 32 * x, r[x]);
-                    tmem_ld_wait();
-                }
+                for (int x = 0; x < TK / 32; ++x) tmem_ld32(ts + 32 * x, r[x]);
+                tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.s_read[t][g & 1]);   // these scores may be overwritten
-                if (act) {
-                    if (part) {
+                if (part) {
 #pragma unroll
-                        for (int x = 0; x < TK / 32; ++x)
+                    for (int x = 0; x < TK / 32; ++x)
 #pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!(see[x] >> k & 1u)) r[x][k] = 0xff800000u;
+                        for (int k = 0; k < 32; ++k)
+                            if (!(see[x] >> k & 1u)) r[x][k] = 0xff800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < 32; k += 4)
+#pragma unroll
+                    for (int x = 0; x < TK / 32; ++x) {
+                        float &a = mx[2 * (x & 1)], &b = mx[2 * (x & 1) + 1];
+                        a = ct_max3(a, __uint_as_float(r[x][k]), __uint_as_float(r[x][k + 1]));
+                        b = ct_max3(b, __uint_as_float(r[x][k + 2]), __uint_as_float(r[x][k + 3]));
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                if (i == first) {
+                    m_ref = top;
+                } else {
+                    const bool need = mine && top > m_ref + CT_RESCALE_LOG2;
+                    if (__any_sync(0xffffffffu, need)) {
+                        CT_FAIL_AT(4, !pv_done(g - 1));
+                        tc_fence_after();
+                        const float m_new = need ? top : m_ref;
+                        const float f = need ? fast_exp2(m_ref - m_new) : 1.0f;   // (0 where the row had seen nothing)
+                        uint32_t o[16];
+                        for (int c = 0; c < p.D; c += 16) {
+                            tmem_ld16(to + c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-#pragma unroll
-                        for (int x = 0; x < TK / 32; ++x) {
-                            float &a = mx[2 * (x & 1)], &b = mx[2 * (x & 1) + 1];
-                            a = ct_max3(a, __uint_as_float(r[x][k]), __uint_as_float(r[x][k + 1]));
-                            b = ct_max3(b, __uint_as_float(r[x][k + 2]), __uint_as_float(r[x][k + 3]));
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st16(to + c, o);
                         }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                    if (i == first) {
-                        m_ref = top;
-                    } else {
-                        const bool need = mine && top > m_ref + CT_RESCALE_LOG2;
-                        if (__any_sync(0xffffffffu, need)) {
-                            CT_FAIL_AT(4, !pv_done(g - 1));
-                            tc_fence_after();
-                            const float m_new = need ? top : m_ref;
-                            const float f = need ? fast_exp2(m_ref - m_new) : 1.0f;   // (0 where the row had seen nothing)
-                            uint32_t o[16];
-                            for (int c = 0; c < p.D; c += 16) {
-                                tmem_ld16(to + c, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                tmem_st16(to + c, o);
-                            }
-                            tmem_st_wait();
-                            l *= f;
-                            m_ref = m_new;
-                        }
+                        tmem_st_wait();
+                        l *= f;
+                        m_ref = m_new;
                     }
                 }
                 const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;   // a row that has seen nothing: every score is -inf
@@ -502,24 +508,22 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 uint64_t sum = 0;   // a pair of sums
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
-                    if (act) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t pk[4];
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t pk[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int e = 8 * (c & 3) + 2 * k;
-                                const uint32_t (&rr)[32] = r[2 * h + (c >> 2)];
-                                float e0, e1;
-                                ct_unpair(ct_fma2(ct_pair(__uint_as_float(rr[e]), __uint_as_float(rr[e + 1])), sl2_2, neg_2), e0, e1);
-                                e0 = fast_exp2(e0); e1 = fast_exp2(e1);
-                                sum = ct_add2(sum, ct_pair(e0, e1));
-                                pk[k] = pack_16x2(e0, e1, F16);
-                            }
-                            if (row < ct.rows8) ct_st_shared_v4(pw + h * slab + ((((uint32_t)c) ^ sw) << 4), pk[0], pk[1], pk[2], pk[3]);
+                        for (int k = 0; k < 4; ++k) {
+                            const int e = 8 * (c & 3) + 2 * k;
+                            const uint32_t (&rr)[32] = r[2 * h + (c >> 2)];
+                            float e0, e1;
+                            ct_unpair(ct_fma2(ct_pair(__uint_as_float(rr[e]), __uint_as_float(rr[e + 1])), sl2_2, neg_2), e0, e1);
+                            e0 = fast_exp2(e0); e1 = fast_exp2(e1);
+                            sum = ct_add2(sum, ct_pair(e0, e1));
+                            pk[k] = pack_16x2(e0, e1, F16);
                         }
-                        fence_proxy_async_smem();
+                        if (NT == 2 || row < ct.rows8) ct_st_shared_v4(pw + h * slab + ((((uint32_t)c) ^ sw) << 4), pk[0], pk[1], pk[2], pk[3]);
                     }
+                    fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_full[t][g & 1][h]);
                 }
