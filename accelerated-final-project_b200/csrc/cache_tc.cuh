@@ -154,6 +154,32 @@ __device__ __forceinline__ bool ct_take_out(unsigned char *tile, int groups, int
     return true;
 }
 
+// By one whole warp, each lane with 128 bytes of a row, `at`: 4 x 4 blocks of 32-byte pieces are transposed among groups of four neighbouring lanes, then lane j of
+// a group stores piece j of each of the group's rows.  Only the first `rows` of a group's rows, and `bytes` of the 128, exist.
+__device__ __forceinline__ void ct_store_rows(unsigned char *at, uint32_t (&w)[32], int lane, int rows, int bytes) {
+    const int j = lane & 3;
+#pragma unroll
+    for (int M = 2; M >= 1; M >>= 1) {
+        const bool up = (j & M) != 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k & M) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t send = up ? w[8 * k + e] : w[8 * (k | M) + e];
+                const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, M);
+                if (up) w[8 * k + e] = recv; else w[8 * (k | M) + e] = recv;
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {   // the row of lane (group + m)
+        unsigned char *row = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), (lane & ~3) + m));
+        if (m < rows && j * 32 < bytes) *reinterpret_cast<uint4 *>(row + j * 32) = make_uint4(w[8 * m], w[8 * m + 1], w[8 * m + 2], w[8 * m + 3]);
+        if (m < rows && j * 32 + 16 < bytes) *reinterpret_cast<uint4 *>(row + j * 32 + 16) = make_uint4(w[8 * m + 4], w[8 * m + 5], w[8 * m + 6], w[8 * m + 7]);
+    }
+}
+
 #define CT_FAIL_AT(site, cond)                                                                          \
     if (cond) {                                                                                         \
         report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << (16 + (site))));     \
@@ -542,38 +568,40 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 float *prt = p.part + ((size_t)blockIdx.x * 2 + (seg == 0 ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
                 const int urow = t * ct.tpt * p.G + row;   // row of the unit
                 T *o = ca_row<T>(p.O, p.o, w.b, hq, tok);
-                for (int c = 0; c < p.D; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(to + c, v);
-                    tmem_ld_wait();
-                    if (bad && mine) {   // values that are not finite, for the rows that see them
-                        for (int j = max(first - nct, 0) * TK; j < min(p.T, (end - nct) * TK); ++j) {
-                            if (p.mask ? p.mask[w.b * p.mask_b + (long long)tok * p.T + j] == 0 : j > tok) continue;
-                            const T *vd = ca_row<T>(p.Vd, p.vd, w.b, w.h, j);
+                // 32 columns of a row: as fp32, 128 bytes of a part; two of them, as 16-bit values, 128 bytes of the output.  Lanes trade pieces so that a
+                // store covers whole lines of eight rows, not 16 bytes of 32 (7 us a unit of 128 columns).
+                uint32_t v[32];
+                if (whole) {
+                    uint32_t out[32];
+                    for (int c = 0; c < p.D; c += 64) {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                const float x = c + k < p.D ? to_f32(vd[c + k]) : 0.0f;
-                                if (!(fabsf(x) < INFINITY)) v[k] = __float_as_uint(__uint_as_float(v[k]) + x);
-                            }
-                        }
-                    }
+                        for (int x = 0; x < 2; ++x) {
+                            tmem_ld32(to + c + 32 * x, v);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int k = 0; k < 16; k += 8) {
-                        if (!mine || c + k >= p.D) break;
-                        if (whole) {
-                            uint4 x;
-                            x.x = pack_16x2(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv, F16);
-                            x.y = pack_16x2(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv, F16);
-                            x.z = pack_16x2(__uint_as_float(v[k + 4]) * inv, __uint_as_float(v[k + 5]) * inv, F16);
-                            x.w = pack_16x2(__uint_as_float(v[k + 6]) * inv, __uint_as_float(v[k + 7]) * inv, F16);
-                            *reinterpret_cast<uint4 *>(o + c + k) = x;
-                        } else {
-                            float4 *d = reinterpret_cast<float4 *>(prt + (size_t)urow * p.D + c + k);
-                            d[0] = make_float4(__uint_as_float(v[k]), __uint_as_float(v[k + 1]), __uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]));
-                            d[1] = make_float4(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5]), __uint_as_float(v[k + 6]), __uint_as_float(v[k + 7]));
+                            for (int k = 0; k < 16; ++k) out[16 * x + k] = pack_16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv, F16);
                         }
+                        ct_store_rows(reinterpret_cast<unsigned char *>(o + c), out, lane, rows - (row & ~3), (p.D - c) * 2);
                     }
+                } else {
+                    for (int c = 0; c < p.D; c += 32) {
+                        tmem_ld32(to + c, v);
+                        tmem_ld_wait();
+                        ct_store_rows(reinterpret_cast<unsigned char *>(prt + (size_t)urow * p.D + c), v, lane, rows - (row & ~3), (p.D - c) * 4);
+                    }
+                }
+                if (bad) {   // values that are not finite, for the rows that see them (the warp's lanes have written each other's rows)
                     __syncwarp();
+                    for (int j = max(first - nct, 0) * TK; mine && j < min(p.T, (end - nct) * TK); ++j) {
+                        if (p.mask ? p.mask[w.b * p.mask_b + (long long)tok * p.T + j] == 0 : j > tok) continue;
+                        const T *vd = ca_row<T>(p.Vd, p.vd, w.b, w.h, j);
+                        for (int d = 0; d < p.D; ++d) {
+                            const float x = to_f32(vd[d]);
+                            if (fabsf(x) < INFINITY) continue;
+                            if (whole) o[d] = OutCvt<T>::one(to_f32(o[d]) + x);
+                            else prt[(size_t)urow * p.D + d] += x;
+                        }
+                    }
                 }
                 if (mine) {
                     if (!whole) {
