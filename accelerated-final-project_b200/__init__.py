@@ -343,7 +343,6 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
     B, Hkv, S, D = k_shape
     _, Hq, T, _ = q_shape
     q = _view(Q, "Q", (B, Hq, T, D), dtype, dev)
-    device = Q.device
     if out is None:
         out = torch.empty_like(Q)
         s = out.stride()
@@ -351,7 +350,7 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
     else:
         o = _view(out, "out", q_shape, dtype, dev)
     if lse is None:
-        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        lse = Q.new_empty((B, Hq, T), dtype=torch.float32)
         lse_at = lse.data_ptr()
     else:
         lse_at = _dense(lse, "lse", (B, Hq, T), torch.float32, dev)
@@ -383,7 +382,7 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
         if len(_attend_ws) >= 4096:
             _attend_ws.clear()
         _attend_ws[key] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    ws = Q.new_empty((need + 1) // 2)   # (elements of 2 bytes at least)
     _call_on(dev, L.b200attn_cache_attend, _pack_attend(*filled, ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(dev), flags))
     return out, lse
 
@@ -401,11 +400,14 @@ def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, ne
         _refuse("Kd must be [B, heads, new tokens, D] and accepted [B, most accepted tokens]")
     T, dtype, i32 = Kd.shape[2], K.dtype, torch.int32
     A = 0 if accepted is None else accepted.shape[1]
-    out = torch.empty((B,), dtype=i32, device=K.device)
+    n = _dense(length, "length", (B,), i32, dev)
+    if n == 0:
+        _refuse("length must be given")
+    out = torch.empty_like(length)   # (half of the time of torch.empty)
     stream = torch._C._cuda_getCurrentRawStream(dev)
     d_shape = (B, Hkv, T, D)
     packed = _pack_commit(*_view(K, "K", k_shape, dtype, dev), *_view(V, "V", k_shape, dtype, dev), *_view(Kd, "Kd", d_shape, dtype, dev),
-                          *_view(Vd, "Vd", d_shape, dtype, dev), _dense(length, "length", (B,), i32, dev), out.data_ptr(),
+                          *_view(Vd, "Vd", d_shape, dtype, dev), n, out.data_ptr(),
                           _dense(accepted, "accepted", (B, A), i32, dev), A, _dense(weights, "weights", (B, Hkv, S), torch.float32, dev),
                           _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev), B, Hkv, T, S, D, _DTYPES[dtype],
                           stream, flags)
@@ -446,12 +448,16 @@ def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_po
         with torch.cuda.stream(at):
             return cache_evict(K, V, length, weights, keep, sink, recent, pos, next_pos, into, kept, None, flags)
     dtype, i32, f32 = K.dtype, torch.int32, torch.float32
-    if kept is None:
-        kept = torch.empty((B, Hkv, max(keep, 0)), dtype=i32, device=K.device)
-    out = torch.empty((B,), dtype=i32, device=K.device)
-    stream = torch._C._cuda_getCurrentRawStream(dev)
     if length is None or weights is None:
         _refuse("length and weights must be given")
+    n = _dense(length, "length", (B,), i32, dev)
+    if kept is None:
+        kept = length.new_empty((B, Hkv, max(keep, 0)))
+        kept_at = kept.data_ptr()
+    else:
+        kept_at = _dense(kept, "kept", (B, Hkv, max(keep, 0)), i32, dev)
+    out = torch.empty_like(length)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
     target, So = (0,) * 10, 0
     if into is not None:
         Ko, Vo, Wo, Po = into
@@ -462,8 +468,8 @@ def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_po
         target = _view(Ko, "K of `into`", o_shape, dtype, dev) + _view(Vo, "V of `into`", o_shape, dtype, dev) + (
             _dense(Wo, "weights of `into`", (B, Hkv, So), f32, dev), _dense(Po, "pos of `into`", (B, Hkv, So), i32, dev))
     packed = _pack_evict(*_view(K, "K", k_shape, dtype, dev), *_view(V, "V", k_shape, dtype, dev), _dense(weights, "weights", (B, Hkv, S), f32, dev),
-                         _dense(pos, "pos", (B, Hkv, S), i32, dev), _dense(length, "length", (B,), i32, dev), _dense(next_pos, "next_pos", (B,), i32, dev),
-                         out.data_ptr(), _dense(kept, "kept", (B, Hkv, max(keep, 0)), i32, dev), keep, sink, recent, *target, So, B, Hkv, S, D,
+                         _dense(pos, "pos", (B, Hkv, S), i32, dev), n, _dense(next_pos, "next_pos", (B,), i32, dev),
+                         out.data_ptr(), kept_at, keep, sink, recent, *target, So, B, Hkv, S, D,
                          _DTYPES[dtype], stream, flags)
     _call_on(dev, (_lib or lib()).b200attn_cache_evict, packed)
     return kept, out
