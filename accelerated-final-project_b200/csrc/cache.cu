@@ -118,8 +118,6 @@ long long units(const CaParams &p) { return (long long)p.B * p.Hkv * p.nrt; }
 size_t entries_bytes(const CaParams &p) { return (size_t)(p.by_cta ? p.grid : units(p)) * 8 * sizeof(int); }
 size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + entries_bytes(p); }
 
-#include <cstdlib>
-static int env_oh(int d) { const char *e = getenv("CA_OH"); return e ? atoi(e) : d; }
 void share_out(CaParams &p, int RT, int TK, int OH, int grid) {
     p.RT = RT; p.TK = TK; p.OH = OH; p.grid = grid;
     p.nrt = (p.R + RT - 1) / RT;
@@ -187,7 +185,7 @@ bool tc_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, CtPa
         if (ct.nst >= (i < 3 ? 4 : 3)) break;
     }
     if (ct.nst < 3) return false;
-    share_out(p, NT * ct.tpt * p.G, TK, env_oh(4), c.sm_count);
+    share_out(p, NT * ct.tpt * p.G, TK, CT_OH, c.sm_count);
     ct.a = p;
     *out = ct;
     return true;
@@ -204,7 +202,7 @@ bool narrow_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, 
     const size_t room = c.max_smem - 4096 - 1024, front = cn_front_bytes(N, cn.ng);
     cn.nst = (int)((room - front) / ((size_t)cn.gp * CN_GROUP));
     if (cn.nst > CT_MAX_STAGES) cn.nst = CT_MAX_STAGES;
-    share_out(p, p.R, CN_TK, env_oh(1), c.sm_count);
+    share_out(p, p.R, CN_TK, CN_OH, c.sm_count);
     cn.a = p;
     *out = cn;
     return true;
@@ -259,7 +257,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CtParams ct;
     CnParams cn;
     bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
-    share_out(p, CG_ROWS, CG_KEYS, env_oh(0), c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
+    share_out(p, CG_ROWS, CG_KEYS, CG_OH, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
     // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
     size_t bytes = attend_bytes(p);
     const size_t other = narrow ? attend_bytes(cn.a) : tc ? attend_bytes(ct.a) : 0;
@@ -439,11 +437,17 @@ int weights(const b200attn_weights_args *a) {
     return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
 }
 
+template <typename P, int THREADS>
+int launch_select(const CeParams &p, const HostCall &c, int cl, cudaStream_t st) {
+    int rc = raise_smem<ce_select_kernel<P, THREADS>>(c);
+    if (rc) return rc;
+    CU_TRY(launch_dependent(ce_select_kernel<P, THREADS>, dim3((unsigned)(p.Hkv * cl), (unsigned)p.B), THREADS, ce_smem_bytes(p.chunk_most, p.cached), cl, st, p));
+    return B200ATTN_OK;
+}
 template <typename P>
 int launch_evict(const CeParams &p, const HostCall &c, int cl, cudaStream_t st) {
-    int rc = raise_smem<ce_select_kernel<P>>(c);
+    int rc = cl > 1 ? launch_select<P, 1024>(p, c, cl, st) : launch_select<P, 512>(p, c, cl, st);
     if (rc) return rc;
-    CU_TRY(launch_dependent(ce_select_kernel<P>, dim3((unsigned)(p.Hkv * cl), (unsigned)p.B), CE_THREADS, ce_smem_bytes(p.chunk_most, p.cached), cl, st, p));
     count_launches(1);
     if (!p.K_out && p.S - p.keep <= CE_FEW) return B200ATTN_OK;
     const int most = p.keep < p.S ? p.keep : p.S;

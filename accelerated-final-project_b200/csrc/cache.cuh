@@ -279,6 +279,7 @@ ca_combine_kernel(const CaParams p) {
 // per 32 multiply-adds of a score.
 //   2 x 8 heads, 7 tokens, 1501 and 2999 rows cached, head_d 64, fp32 (18.5 MB): 40 us with element-wise loads, one after the other
 constexpr int CG_ROWS = 16, CG_KEYS = 64, CG_THREADS = 128;
+constexpr int CG_OH = 0;   // items in front of a unit's tiles (1: 72 us instead of 58, before the copies were asynchronous)
 __host__ __device__ inline int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
 inline size_t cg_smem_bytes(int D) { return ((size_t)(CG_ROWS + 2 * CG_KEYS) * cg_pitch(D) + CG_KEYS * (CG_ROWS + 4)) * sizeof(float); }
 
@@ -429,6 +430,7 @@ ca_generic_kernel(const CaParams p) {
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) acc[c][r] *= s_f[rbase + r];
+#pragma unroll 4
                 for (int j = 0; j < nk; ++j) {
                     float v[NC], e[NR];
 #pragma unroll
@@ -656,8 +658,7 @@ __device__ __forceinline__ unsigned ce_rank(float w, bool held) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int CE_THREADS = 512;
-constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS, CE_PER = CE_BINS / CE_THREADS;
+constexpr int CE_BITS = 11, CE_BINS = 1 << CE_BITS;
 constexpr int CE_COPIES = 4;   // of the first histogram: most weights share a few of its digits, and additions to one word wait for each other
 constexpr size_t CE_HISTS = (size_t)(CE_COPIES + 2) * CE_BINS * 4;
 // the histograms; per word of 32 rows: the mask of rows that stay, that of equal rank, a number; 16 bits a row (the list of kept rows that move); the ranks
@@ -667,6 +668,7 @@ constexpr int CE_FEW = 128;
 constexpr int CE_PICK = 32;   // up to so many rows that leave are picked one by one
 
 // Exclusive scan of one value per thread of the block, and its total.
+template <int CE_THREADS>
 __device__ __forceinline__ int ce_scan(int x, int *s_warp, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = x;
@@ -693,9 +695,9 @@ __device__ __forceinline__ int ce_remote(const void *p, uint32_t rank) {   // a 
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_to_rank(smem_u32(p), rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ int4 ce_remote4(const void *p, uint32_t rank) {
-    int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_to_rank(smem_u32(p), rank)));
+__device__ __forceinline__ int2 ce_remote2(const void *p, uint32_t rank) {
+    int2 v;
+    asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(map_to_rank(smem_u32(p), rank)));
     return v;
 }
 __device__ __forceinline__ int ce_remote_u16(const void *p, uint32_t rank) {
@@ -735,11 +737,12 @@ __device__ __forceinline__ void ce_move_rows(const CeParams &p, int b, int h, in
 //   into another cache: the numbers of the rows that stay are their new places.  In place: the kept rows from m on are listed by their number, and the i-th
 //   freed row below m takes the i-th of them, from the list of the CTA that has it.
 // Where few rows leave, in place, they are picked one after the other instead: a reduction over the block each.
-// Bound by latency: three passes over shared memory and some ten barriers.
+// Bound by latency: three passes over shared memory and some ten barriers; so a cluster's CTAs have 1024 threads (512: 48 us instead of 37 for 4 x 8 heads, up to 32768 rows), one that
+// shares its SM 512.
 //   32 sequences x 8 heads, up to 4102 rows: 22 us with 1024 threads that read weights and positions anew in each pass, 19 with the ranks in shared memory, 23
 //   with two bits a round by counting; 4 x 8 heads, up to 32768 rows: 91, 33
-template <typename P>
-__global__ void __launch_bounds__(CE_THREADS, 2)
+template <typename P, int CE_THREADS>
+__global__ void __launch_bounds__(CE_THREADS, 1024 / CE_THREADS)
 ce_select_kernel(const CeParams p) {
     extern __shared__ __align__(16) unsigned ce_smem[];
     __shared__ int s_warp[CE_THREADS / 32], s_count[4], s_pairs[CE_FEW * 2];
@@ -872,30 +875,36 @@ ce_select_kernel(const CeParams p) {
                 if (in && d != d0) atomicAdd(&copy[d], 1);
             }
         }
-        // thread i has the digits CE_BINS - 1 - CE_PER i downwards
-        static_assert(CE_PER == 4, "a thread's bins are 16 bytes");
-        int4 *mine4 = reinterpret_cast<int4 *>(hist) + (CE_THREADS - 1 - tid);
+        // thread i has the digits CE_BINS - 1 - CE_PER i downwards, in pairs
+        constexpr int CE_PER = CE_BINS / CE_THREADS, pairs = CE_PER / 2;
+        int2 *mine2 = reinterpret_cast<int2 *>(hist) + (CE_THREADS - 1 - tid) * pairs;
         if (pass == 0) {
             __syncthreads();
-            int4 q = *mine4;
 #pragma unroll
-            for (int k = 1; k < CE_COPIES; ++k) {
-                const int4 v = mine4[k * CE_BINS / 4];
-                q.x += v.x; q.y += v.y; q.z += v.z; q.w += v.w;
+            for (int i = 0; i < pairs; ++i) {
+                int2 q = mine2[i];
+#pragma unroll
+                for (int k = 1; k < CE_COPIES; ++k) { q.x += mine2[k * CE_BINS / 2 + i].x; q.y += mine2[k * CE_BINS / 2 + i].y; }
+                mine2[i] = q;
             }
-            *mine4 = q;
         }
         ce_cluster_sync(cl);
-        int4 q = *mine4;
+        int c[CE_PER], sum = 0;
 #pragma unroll
-        for (uint32_t o = 1; o < 8; ++o) {
-            if (o >= cl) break;
-            const int4 v = ce_remote4(mine4, (rank + o) % cl);
-            q.x += v.x; q.y += v.y; q.z += v.z; q.w += v.w;
+        for (int i = 0; i < pairs; ++i) {
+            int2 q = mine2[i];
+#pragma unroll
+            for (uint32_t o = 1; o < 8; ++o) {
+                if (o >= cl) break;
+                const int2 v = ce_remote2(mine2 + i, (rank + o) % cl);
+                q.x += v.x; q.y += v.y;
+            }
+            c[CE_PER - 1 - 2 * i] = q.x;
+            c[CE_PER - 2 - 2 * i] = q.y;
+            sum += q.x + q.y;
         }
-        const int c[CE_PER] = {q.w, q.z, q.y, q.x}, sum = q.x + q.y + q.z + q.w;
         int all;
-        int before = ce_scan(sum, s_warp, &all);
+        int before = ce_scan<CE_THREADS>(sum, s_warp, &all);
         if (before < need && before + sum >= need) {
 #pragma unroll
             for (int k = 0; k < CE_PER; ++k) {
@@ -920,7 +929,7 @@ ce_select_kernel(const CeParams p) {
     const int per = (words + CE_THREADS - 1) / CE_THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);   // words of this thread, in a row
     for (int i = w0; i < w1; ++i) equals += __popc(equal[i]);
     int all;
-    int mine = ce_scan(equals, s_warp, &all);
+    int mine = ce_scan<CE_THREADS>(equals, s_warp, &all);
     // numbers over the CTAs in front of this one: `slot` of s_count in each, which the caller's total goes into
     auto in_front = [&](int total, int slot, int *sum) {
         if (tid == 0) s_count[slot] = total;
@@ -957,7 +966,7 @@ ce_select_kernel(const CeParams p) {
     // the rows that are numbered: all that stay, or those of them from m on
     int count = 0;
     for (int i = w0; i < w1; ++i) count += __popc(into ? stays[i] : stays[i] & ~front(i));
-    mine = ce_scan(count, s_warp, &all);
+    mine = ce_scan<CE_THREADS>(count, s_warp, &all);
     for (int i = w0; i < w1; ++i) {
         number[i] = mine;
         mine += __popc(into ? stays[i] : stays[i] & ~front(i));
@@ -981,7 +990,7 @@ ce_select_kernel(const CeParams p) {
     // freed rows: numbered, too
     count = 0;
     for (int i = w0; i < w1; ++i) count += __popc(~stays[i] & front(i));
-    mine = ce_scan(count, s_warp, &all);
+    mine = ce_scan<CE_THREADS>(count, s_warp, &all);
     for (int i = w0; i < w1; ++i) {
         number[i] = mine;
         mine += __popc(~stays[i] & front(i));

@@ -25,6 +25,7 @@ struct CnParams {
     int tmem_cols;
 };
 constexpr int CN_THREADS = 256, CN_TK = 128;
+constexpr int CN_OH = 1;   // a unit's beginning and end, in tiles (0 / 1 / 3: 184.4 / 182.9 / 186.4 us for the call above)
 constexpr uint32_t CN_GROUP = CN_TK * 128u;   // 128 keys x 64 columns
 
 struct CnBars {

@@ -8,9 +8,10 @@
 // of a tile are left out.
 //   warp 0       the walk over the tiles; one thread requests K tiles (and Q) by TMA
 //   warp 1       one thread issues the MMAs, 64 rows at a time, into two buffers per summing warpgroup
-//   warps 2, 3   gather the next rows of Q beside the present ones (by the summing warps between two pairs: 61 against XX us, weights_step)
+//   warps 2, 3   gather the next rows of Q beside the present ones (61 us a call of 32 sequences, up to 6 tokens, 100 to 8000 rows, where the
+//                summing warps did it between two pairs; 49 so)
 //   warps 4-11   two warpgroups take the tiles in turn; a thread per key: its exponentials and their sum (bound by the latency of that chain: one
-//                warpgroup 54 us, weights_step)
+//                warpgroup was as fast with 24 rows, and 30 against 28 us with 700)
 #pragma once
 
 #include "cache_tc.cuh"
@@ -20,7 +21,7 @@ namespace b200attn {
 constexpr int CX_THREADS = 384, CX_TK = 128, CX_NB = 64;   // (64 rows a block)
 constexpr int CX_BUFS = 4;
 // What a pair's beginning and end cost a CTA, in tiles, as in cache.cuh: two tiles of a block of rows (none: a CTA with 20 short sequences took 62 us
-// where the others took 40, weights_step; two also where a tile has eleven blocks: 34 us instead of 28, weights_prompt).
+// where the others took 40; two also where a tile has eleven blocks: 34 us instead of 28).
 __host__ __device__ inline int cx_overhead(long long rows) { return rows <= CX_NB ? 2 : rows <= 2 * CX_NB ? 1 : 0; }
 constexpr int CX_SLOTS = 16;   // pairs that the roles can be at: one per ring stage (up to 8) and score buffer, and two
 
