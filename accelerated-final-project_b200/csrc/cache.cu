@@ -25,6 +25,11 @@ int check_dtype(int dtype) {
     return B200ATTN_OK;
 }
 
+int check_capacity(int capacity) {
+    if (capacity > (1 << 30)) return fail(B200ATTN_ERR_TOO_LARGE, "capacity must be at most 2^30 rows (got %d)", capacity);
+    return B200ATTN_OK;
+}
+
 int check_view(const char *name, const b200attn_view &v, int dtype) {
     if (v.ptr == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be non-NULL", name);
     if ((uintptr_t)v.ptr & (esize(dtype) - 1)) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be aligned to the element size", name);
@@ -90,6 +95,7 @@ int validate(const b200attn_attend_args *a, bool pointers) {
     if (rc) return rc;
     if (a->num_heads % a->num_kv_heads) return fail(B200ATTN_ERR_INVALID_ARG, "num_heads (%d) must be a multiple of num_kv_heads (%d)", a->num_heads, a->num_kv_heads);
     if (a->head_d > CA_MAX_D) return fail(B200ATTN_ERR_INVALID_ARG, "head_d must be at most %d (got %d)", CA_MAX_D, a->head_d);
+    if ((rc = check_capacity(a->capacity))) return rc;
     if ((long long)a->len_new * (a->num_heads / a->num_kv_heads) > (1ll << 30))
         return fail(B200ATTN_ERR_TOO_LARGE, "len_new times the query heads of a key head is %lld, at most 2^30 are taken", (long long)a->len_new * (a->num_heads / a->num_kv_heads));
     if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");
@@ -121,13 +127,18 @@ size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_fl
 void share_out(CaParams &p, int RT, int TK, int OH, int grid) {
     p.RT = RT; p.TK = TK; p.OH = OH; p.grid = grid;
     p.nrt = (p.R + RT - 1) / RT;
-    p.DT = 0;
     // few units are cut into many parts each, which a block's warps share out: then a block has as many rows as it can take at once
     p.by_cta = units(p) > grid;
     const long long parts = grid / units(p) + 1;
     p.join_rows = p.by_cta ? 16 : parts <= 4 ? 8 : parts <= 8 ? 4 : parts <= 16 ? 2 : 1;
-    if (p.drafts)
-        for (int rt = 0; rt < p.nrt; ++rt) p.DT += ca_draft_tiles(rt, p.R, RT, p.G, p.T, TK, p.mask == nullptr);
+}
+// Of the kernel that runs: the tiles of new keys of a key head's units.
+void count_drafts(CaParams &p) {
+    p.DT = 0;
+    if (!p.drafts) return;
+    if (p.mask) p.DT = (long long)p.nrt * ca_draft_tiles(0, p.R, p.RT, p.G, p.T, p.TK, false);
+    else
+        for (int rt = 0; rt < p.nrt; ++rt) p.DT += ca_draft_tiles(rt, p.R, p.RT, p.G, p.T, p.TK, true);
 }
 
 void fill(CaParams &p, const b200attn_attend_args &a) {
@@ -281,6 +292,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
         return rc;
     }
     CaParams &q = narrow ? cn.a : tc ? ct.a : p;
+    count_drafts(q);
     q.part = (float *)ws;
     q.entries = (int *)((char *)ws + attend_bytes(q) - entries_bytes(q));
     if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, c, m, st) : launch_attend_narrow<false>(cn, c, m, st);
@@ -312,6 +324,7 @@ int commit(const b200attn_commit_args *a) {
     int rc = check_dtype(a->dtype);
     if (rc || (rc = check_grid(a->batch_sz, a->num_kv_heads))) return rc;
     if (a->head_d > (1 << 20)) return fail(B200ATTN_ERR_TOO_LARGE, "head_d must be at most 2^20 (got %d)", a->head_d);
+    if ((rc = check_capacity(a->capacity))) return rc;
     const long long B = a->batch_sz, H = a->num_kv_heads, T = a->len_new, S = a->capacity, D = a->head_d;
     if ((rc = check_view("K", a->K, a->dtype)) || (rc = check_view("V", a->V, a->dtype)) || (rc = check_view("Kd", a->Kd, a->dtype)) || (rc = check_view("Vd", a->Vd, a->dtype)) ||
         (rc = check_written("K", a->K, B, H, S, D)) || (rc = check_written("V", a->V, B, H, S, D)) || (rc = check_accepted(a->accepted, a->max_accepted)))
@@ -409,6 +422,7 @@ int weights(const b200attn_weights_args *a) {
     if (rc || (rc = check_grid(a->batch_sz, a->num_kv_heads))) return rc;
     if (a->num_heads % a->num_kv_heads) return fail(B200ATTN_ERR_INVALID_ARG, "num_heads (%d) must be a multiple of num_kv_heads (%d)", a->num_heads, a->num_kv_heads);
     if (a->head_d > CA_MAX_D) return fail(B200ATTN_ERR_INVALID_ARG, "head_d must be at most %d (got %d)", CA_MAX_D, a->head_d);
+    if ((rc = check_capacity(a->capacity))) return rc;
     const int A = a->accepted ? a->max_accepted : a->len_new, G = a->num_heads / a->num_kv_heads;
     if ((long long)A * G > (1ll << 30)) return fail(B200ATTN_ERR_TOO_LARGE, "accepted tokens times the query heads of a key head are %lld, at most 2^30 are taken", (long long)A * G);
     if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");

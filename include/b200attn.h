@@ -189,7 +189,9 @@ const char *b200attn_last_error(void);
  * "tc_fused" (bf16 / fp16, head_d 64, 128, 192 or 256, more than 64 queries: one kernel, scores in tensor
  * memory; an encoding is applied to copies of Q and K first, in one launch), "tc_bf16" (bf16 on the tensor cores, one-kernel
  * cluster pipeline) or "tc_decode" (bf16, up to 64 queries against a long K/V: key splits on the tensor cores
- * plus a combine kernel). */
+ * plus a combine kernel).  b200attn_cache_attend and b200attn_cache_weights name theirs, too: "cache_narrow" (16 bit, up to 64 rows a
+ * key head: keys as the lanes of tensor memory), "cache_tc" (16 bit, tensor cores) and "cache_generic" (CUDA cores: fp32, head_d that is not a multiple of
+ * 8, rows that do not begin on 16 bytes). */
 const char *b200attn_last_path(void);
 
 /* Number of kernel launches issued by this library in this process so far. */
@@ -275,7 +277,7 @@ const char *b200attn_static_last_error(void);
  * strides in elements, so a projection's output [B,T,heads,D] is passed as it is; pointers are aligned to the element size.  The
  * other arrays are dense.  The work is enqueued on `stream` and waited for unless B200ATTN_FLAG_ASYNC is set.  Values that only the device
  * knows cannot be refused by the host: a length outside [0, capacity] counts as the nearer of the two; rows behind the last valid one are
- * neither read (whatever they hold, NaN included, has no effect) nor written.  Calls that share no tensors may be made at the same time from several threads and streams when each
+ * neither read to any effect (whatever they hold, NaN included) nor written.  A capacity is at most 2^30 rows.  Calls that share no tensors may be made at the same time from several threads and streams when each
  * has a workspace of its own. */
 typedef struct b200attn_view {   /* a tensor [B, heads, rows, D] */
     void *ptr;                   /* device pointer */

@@ -67,7 +67,7 @@ def test_structures_have_the_header_s_sizes(pkg):
     ({"len_new": 0}, b"positive"), ({"capacity": 0}, b"positive"), ({"batch_sz": -1}, b"positive"), ({"num_heads": 6}, b"multiple"), ({"head_d": 257}, b"head_d"),
     ({"dtype": 7}, b"dtype"), ({"scale": -1.0}, b"scale"), ({"scale": float("nan")}, b"scale"), ({"scale": float("inf")}, b"scale"), ({"mask_stride_b": 4}, b"mask_stride_b"),
     ({"K_l": -64}, b"negative"), ({"out_l": 32}, b"overlap each other"), ({"out_h": 0}, b"overlap each other"), ({"out": P + 2}, b"overlap an input"), ({"out": 5 * P}, b"overlap an input"),
-    ({"len_new": 1 << 30}, b"2^30"),
+    ({"len_new": 1 << 30}, b"2^30"), ({"capacity": (1 << 30) + 1}, b"2^30"),
 ])
 def test_attend_refuses(pkg, over, word):
     rc, msg = status(pkg, "attend", attend_args(pkg, **over))

@@ -78,13 +78,35 @@ SHAPES = [
     (1, 40, 1, 4, 300, (290,), 64, "tree"),         # 40
     (1, 200, 1, 2, 100, (90,), 64, "tree"),         # more than a tile of rows for one token
     (40, 2, 1, 1, 100, tuple(range(0, 100, 7)), 64, "chain"),
+    (1, 16, 1, 4, 300, (299,), 256, "tree"),        # 64 rows a key head at the widest head
+    (2, 10, 1, 6, 300, (120, 299), 192, "chain"),
+    (1, 9, 1, 7, 200, (190,), 64, "tree"),          # 63 rows
+    (2, 8, 1, 12, 300, (300, 127), 128, "tree"),    # one tile of 96 rows
+    (3, 16, 2, 16, 300, (300, 0, 5), 64, "tree"),   # one of 128
+    (2, 100, 1, 1, 300, (300, 11), 128, "chain"),   # one token of 100 heads
+    (1, 126, 1, 3, 90, (77,), 80, "tree"),
+    (40, 16, 2, 16, 100, tuple(range(0, 100, 7)), 128, "tree"),   # many short sequences: several units a CTA
+    (37, 8, 2, 70, 50, tuple(range(0, 50, 3)), 128, "tree"),      # ... of two tiles, some of them without rows
+    (9, 5, 5, 300, 60, tuple(range(0, 60, 7)), 64, "chain"),
+    (30, 8, 4, 9, 200, tuple(range(0, 200, 13)), 256, "tree"),
 ]
+PATHS = ("cache_narrow", "cache_tc", "cache_generic")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s[:5])) + f"-{s[6]}-{s[7]}")
 def test_attend(pkg, cuda, shape, dtype):
     check_attend(pkg, Problem(dtype, *shape, seed=len(str(shape))))
+    B, Hq, Hkv, T, _, _, D, _ = shape
+    generic = dtype == "f32" or D % 8 or Hq // Hkv > 128
+    assert pkg.last_path() == PATHS[2 if generic else 0 if Hq // Hkv * T <= 64 else 1]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [SHAPES[4], SHAPES[5], SHAPES[8], SHAPES[13], SHAPES[24]], ids=lambda s: "-".join(map(str, s[:5])))
+def test_attend_without_the_tensor_cores(pkg, cuda, shape, dtype):
+    check_attend(pkg, Problem(dtype, *shape, seed=3), flags=pkg.FLAG_FORCE_GENERIC)
+    assert pkg.last_path() == "cache_generic"
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -244,6 +266,10 @@ def test_commit(pkg, cuda, dtype, D, token):
     (1, 1, 1, 1, 1, (1,), 64, 0), (3, 8, 2, 7, 300, (300, 5, 0), 128, 4), (2, 6, 2, 20, 260, (129, 64), 64, 20), (2, 4, 4, 150, 400, (400, 150), 128, 0),
     (1, 14, 2, 9, 200, (199,), 256, 5), (2, 4, 2, 5, 130, (128, 3), 96, 3), (2, 4, 2, 5, 130, (128, 3), 100, 5), (1, 64, 1, 30, 140, (135,), 64, 9),
     (1, 200, 1, 3, 140, (135,), 64, 2), (1, 2, 1, 3, 70, (66,), 33, 2), (2, 8, 1, 200, 300, (270, 290), 128, 0),
+    (1, 16, 2, 330, 700, (700,), 128, 0),        # 2640 rows a key head: in chunks, by TMA
+    (1, 12, 1, 150, 300, (290,), 256, 150),      # 1800, gathered
+    (1, 7, 1, 100, 300, (290,), 64, 0), (1, 40, 1, 30, 140, (135,), 64, 0), (2, 66, 2, 9, 140, (135, 9), 128, 0),
+    (30, 8, 2, 6, 260, tuple(range(1, 260, 17)), 128, 6),   # short pairs: several a CTA
 ], ids=lambda s: "-".join(map(str, s[:5])) + f"-{s[6]}-{s[7]}")
 def test_weights(pkg, cuda, shape, dtype):
     import torch
@@ -255,6 +281,8 @@ def test_weights(pkg, cuda, shape, dtype):
     if A:
         accepted = torch.stack([torch.randperm(T, device="cuda")[:A] for _ in range(B)]).to(torch.int32)
         accepted[B - 1, A - 1] = -1
+        if B > 4:
+            accepted[2::5, 0] = -1     # sequences that have accepted nothing
     w = torch.rand(B, Hkv, S, device="cuda")
     w[0, 0, S - 1] = math.nan if lengths[0] < S else 0.5     # behind the last row: stays as it is
     want, bound = ref.weights(p.Q, p.K, p.length, lse, w, accepted)
