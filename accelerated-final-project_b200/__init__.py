@@ -377,13 +377,13 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
     if need is None:
         with torch.cuda.device(dev):
             need = L.b200attn_cache_attend_workspace(_pack_attend(*filled, 0, 0, 0, flags))
-        if need == 0:
-            _refuse(L.b200attn_last_error().decode())
+        if need == 0 and (message := L.b200attn_last_error().decode()):
+            _refuse(message)
         if len(_attend_ws) >= 4096:
             _attend_ws.clear()
         _attend_ws[key] = need
-    ws = Q.new_empty((need + 1) // 2)   # (elements of 2 bytes at least)
-    _call_on(dev, L.b200attn_cache_attend, _pack_attend(*filled, ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(dev), flags))
+    ws = Q.new_empty((need + 1) // 2) if need else None   # (elements of 2 bytes at least)
+    _call_on(dev, L.b200attn_cache_attend, _pack_attend(*filled, ws.data_ptr() if need else 0, need, torch._C._cuda_getCurrentRawStream(dev), flags))
     return out, lse
 
 

@@ -122,7 +122,7 @@ int validate(const b200attn_attend_args *a, bool pointers) {
 // Workspace: the slots of cut units, then the entries.
 long long units(const CaParams &p) { return (long long)p.B * p.Hkv * p.nrt; }
 size_t entries_bytes(const CaParams &p) { return (size_t)(p.by_cta ? p.grid : units(p)) * 8 * sizeof(int); }
-size_t attend_bytes(const CaParams &p) { return ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + entries_bytes(p); }
+size_t attend_bytes(const CaParams &p) { return p.uncut ? 0 : ((size_t)p.grid * 2 * ca_slot_floats(p.RT, p.D) + 3) / 4 * 16 + entries_bytes(p); }
 
 void share_out(CaParams &p, int RT, int TK, int OH, int grid) {
     p.RT = RT; p.TK = TK; p.OH = OH; p.grid = grid;
@@ -154,6 +154,10 @@ void fill(CaParams &p, const b200attn_attend_args &a) {
 
 template <typename T>
 int launch_combine(const CaParams &p, cudaStream_t st) {
+    if (p.uncut) {
+        count_launches(1);
+        return B200ATTN_OK;
+    }
     const dim3 grid((unsigned)(p.by_cta ? p.grid : units(p)), (unsigned)(((p.RT < p.R ? p.RT : p.R) + p.join_rows - 1) / p.join_rows));
     CU_TRY(p.D <= 64 ? launch_dependent(ca_combine_kernel<T, 2>, grid, CB_THREADS, 0, 1, st, p)
                      : p.D <= 128 ? launch_dependent(ca_combine_kernel<T, 4>, grid, CB_THREADS, 0, 1, st, p) : launch_dependent(ca_combine_kernel<T, 8>, grid, CB_THREADS, 0, 1, st, p));
@@ -214,6 +218,8 @@ bool narrow_shape(const b200attn_attend_args *a, const HostCall &c, CaParams p, 
     cn.nst = (int)((room - front) / ((size_t)cn.gp * CN_GROUP));
     if (cn.nst > CT_MAX_STAGES) cn.nst = CT_MAX_STAGES;
     share_out(p, p.R, CN_TK, CN_OH, c.sm_count);
+    // a short cache's units are not cut: nothing is joined then, by a second launch
+    p.uncut = (p.S + CN_TK - 1) / CN_TK + (p.drafts ? (p.T + CN_TK - 1) / CN_TK : 0) <= (units(p) * 4 >= c.sm_count * 3 ? CN_UNCUT_MANY : CN_UNCUT_FEW);
     cn.a = p;
     *out = cn;
     return true;
@@ -269,6 +275,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CnParams cn;
     bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
     share_out(p, CG_ROWS, CG_KEYS, CG_OH, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
+    p.uncut = narrow && cn.a.uncut;
     // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
     size_t bytes = attend_bytes(p);
     const size_t other = narrow ? attend_bytes(cn.a) : tc ? attend_bytes(ct.a) : 0;
@@ -284,17 +291,17 @@ int attend(const b200attn_attend_args *a, size_t *need) {
         narrow = narrow && maps;
         tc = tc && maps;
     }
-    void *ws = a->workspace;
+    void *ws = bytes ? a->workspace : nullptr;
     if (ws) {
         if (a->workspace_bytes < bytes) return fail(B200ATTN_ERR_INVALID_ARG, "workspace_bytes is %zu, this call needs %zu", a->workspace_bytes, bytes);
         if ((uintptr_t)ws & 15) return fail(B200ATTN_ERR_INVALID_ARG, "workspace must be aligned to 16 bytes");
-    } else if ((rc = host_workspace(&c, bytes, st, &ws))) {
+    } else if (bytes && (rc = host_workspace(&c, bytes, st, &ws))) {
         return rc;
     }
     CaParams &q = narrow ? cn.a : tc ? ct.a : p;
     count_drafts(q);
     q.part = (float *)ws;
-    q.entries = (int *)((char *)ws + attend_bytes(q) - entries_bytes(q));
+    if (ws) q.entries = (int *)((char *)ws + attend_bytes(q) - entries_bytes(q));
     if (narrow) rc = a->dtype == B200ATTN_F16 ? launch_attend_narrow<true>(cn, c, m, st) : launch_attend_narrow<false>(cn, c, m, st);
     else if (tc) rc = a->dtype == B200ATTN_F16 ? launch_attend_tc<true>(ct, c, m, st) : launch_attend_tc<false>(ct, c, m, st);
     else if (a->dtype == B200ATTN_F32) rc = p.D % 4 == 0 && tc_aligned(a) ? launch_attend<float, true>(p, c, st) : launch_attend<float, false>(p, c, st);
@@ -539,7 +546,7 @@ extern "C" {
 int b200attn_cache_attend(const b200attn_attend_args *args) { return attend(args, nullptr); }
 size_t b200attn_cache_attend_workspace(const b200attn_attend_args *args) {
     size_t need = 0;
-    return attend(args, &need) == B200ATTN_OK ? need : 0;
+    return attend(args, &need) == B200ATTN_OK ? (fail(B200ATTN_OK, "%s", ""), need) : 0;
 }
 int b200attn_cache_commit(const b200attn_commit_args *args) { return commit(args); }
 int b200attn_cache_weights(const b200attn_weights_args *args) { return weights(args); }

@@ -34,6 +34,7 @@ struct CaParams {
     int R;               // rows of a key head: T * G
     int RT, nrt, TK;     // rows of a unit, units of a key head, keys of a tile
     int OH;              // items in front of a unit's tiles
+    int uncut;           // a unit belongs as a whole to the range that its first item is in: nothing to join
     long long DT;        // tiles of new keys, summed over the units of a key head
     int drafts;          // new keys are given
     int grid;            // CTAs that share the items out
@@ -111,10 +112,10 @@ struct CaWalk {
     int at, ct, nt;       // first item of this CTA in the unit; tiles of cached keys; all tiles
     __device__ __forceinline__ void unit(const CaParams &p) { nt = ct + ca_draft_tiles(p, rt); }
     __device__ __forceinline__ int tile(const CaParams &p) const { return max(at - p.OH, 0); }
-    __device__ __forceinline__ int end(const CaParams &p) const { return (int)min((long long)nt, at + left - p.OH); }
-    __device__ __forceinline__ bool whole(const CaParams &p) const { return at <= p.OH && at + left >= p.OH + nt; }
+    __device__ __forceinline__ int end(const CaParams &p) const { return p.uncut ? nt : (int)min((long long)nt, at + left - p.OH); }
+    __device__ __forceinline__ bool whole(const CaParams &p) const { return p.uncut || (at <= p.OH && at + left >= p.OH + nt); }
     __device__ __forceinline__ void settle(const CaParams &p) {   // a range that ends before a unit's first tile has no part in it
-        if (at + left <= p.OH) left = 0;
+        if (!p.uncut && at + left <= p.OH) left = 0;
     }
     __device__ __forceinline__ void start(const CaParams &p, const CaStart &s, int c) {
         const long long i0 = ca_range(s.total, s.grid, c);
@@ -133,6 +134,7 @@ struct CaWalk {
         }
         at = (int)rem;
         u0 = i0 - rem;
+        if (p.uncut && at > 0) next(p);   // (another range's unit)
         settle(p);
     }
     __device__ __forceinline__ void next(const CaParams &p) {
@@ -157,7 +159,7 @@ struct CaWalk {
 // What ca_combine_kernel goes by, {first CTA of a cut unit or -1, its slot, last CTA, b, h, rt}; every other part is in slot 0 of its CTA.  Kept per unit where
 // there are no more units than CTAs: written by the CTA with the unit's first tile, which calls this for each of its units ...
 __device__ __forceinline__ void ca_entry_of_unit(const CaParams &p, const CaStart &s, const CaWalk &w, int c, bool first_of_range) {
-    if (p.by_cta || w.tile(p) != 0) return;
+    if (p.uncut || p.by_cta || w.tile(p) != 0) return;
     int *e = p.entries + (((size_t)w.b * p.Hkv + w.h) * p.nrt + w.rt) * 8;
     e[1] = first_of_range ? 0 : 1;
     e[2] = ca_cta_of(s.total, s.grid, w.u0 + p.OH + w.nt - 1);
@@ -166,7 +168,7 @@ __device__ __forceinline__ void ca_entry_of_unit(const CaParams &p, const CaStar
 }
 // ... else per CTA: by each CTA for the first unit of its range, which is listed where it was cut by this range's beginning and by none before it.
 __device__ __forceinline__ void ca_entry_of_cta(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
-    if (!p.by_cta) return;
+    if (p.uncut || !p.by_cta) return;
     int *e = p.entries + (size_t)c * 8;
     e[0] = -1;
     if (w.left == 0 || w.at <= p.OH) return;

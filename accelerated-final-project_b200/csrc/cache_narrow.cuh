@@ -25,6 +25,10 @@ struct CnParams {
     int tmem_cols;
 };
 constexpr int CN_THREADS = 256, CN_TK = 128;
+// Tiles that a cache's capacity and the new tokens may have for its units not to be cut, so that nothing is joined by a second launch: more where the units fill the
+// SMs by themselves.  Cut / not, one token, 32 / 8 heads of 128: one sequence of 2, 4, 7 tiles 10.5 / 9.8, 10.6 / 11.8, 10.8 / 14.8 us (and 4 us of the host's time
+// less); 16 sequences of 4, 9, 16 tiles 17 / 13, 22 / 18, 32 / 29; 64 of 4, 7, 9, 12 tiles 45 / 39, 53 / 52, 60 / 61, 72 / 76.
+constexpr int CN_UNCUT_FEW = 4, CN_UNCUT_MANY = 8;
 constexpr int CN_OH = 1;   // a unit's beginning and end, in tiles (0 / 1 / 3: 184.4 / 182.9 / 186.4 us for the call above)
 constexpr uint32_t CN_GROUP = CN_TK * 128u;   // 128 keys x 64 columns
 
@@ -285,16 +289,27 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.s_read[g & 1]);   // these scores may be overwritten
-                if (draft && there) {
-                    // row r = token * G + head of the group
-                    const unsigned char *col = p.mask ? p.mask + w.b * p.mask_b + j : nullptr;
-                    for (int t = 0; t < p.T; ++t) {
-                        if (col ? __ldg(col + (long long)t * p.T) == 0 : j > t) {
+                if (draft) {   // rows t G .. t G + G - 1 are token t's
+                    unsigned long long hidden;
+                    if (p.mask == nullptr) {   // a chain: this key is seen from its own token on
+                        const int first_row = min(j * p.G, 64);
+                        hidden = first_row == 64 ? ~0ull : (1ull << first_row) - 1ull;
+                    } else {
+                        const unsigned long long token = p.G == 64 ? ~0ull : (1ull << p.G) - 1ull;
+                        const unsigned char *col = p.mask + w.b * p.mask_b + min(j, p.T - 1);
+                        hidden = 0;
+                        for (int t0 = 0; t0 < p.T; t0 += 8) {
+                            unsigned char see[8];
 #pragma unroll
-                            for (int r = 0; r < N; ++r)
-                                if (r >= t * p.G && r < (t + 1) * p.G) x[r] = -INFINITY;
+                            for (int k = 0; k < 8; ++k) see[k] = t0 + k < p.T ? __ldg(col + (long long)(t0 + k) * p.T) : 1;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (see[k] == 0) hidden |= token << ((t0 + k) * p.G);
                         }
                     }
+#pragma unroll
+                    for (int r = 0; r < N; ++r)
+                        if (hidden >> r & 1ull) x[r] = -INFINITY;
                 }
                 float top = -INFINITY;   // the largest score over its row's reference
 #pragma unroll
@@ -311,10 +326,14 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (ct_any(failed)) { stop = true; break; }
                     // ---- new references where a row's maximum is beyond its own; what has been added up so far is rescaled ----
 #pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        if (r >= R) break;
-                        const float m = cn_warp_max(x[r]);
-                        if (lane == 0) s_red[q][r] = m;
+                    for (int r0 = 0; r0 < N; r0 += 16) {
+                        if (r0 >= R) break;
+                        float m[16];
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) m[r] = cn_warp_max(x[r0 + r]);
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4)
+                            if (lane == 0) *reinterpret_cast<float4 *>(&s_red[q][r0 + r]) = make_float4(m[r], m[r + 1], m[r + 2], m[r + 3]);
                     }
                     ct_sync();
                     if (tid < R) {
@@ -371,10 +390,15 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (stop || ct_any(failed)) break;
             // ---- the unit's sums, then its outputs ----
 #pragma unroll
-            for (int r = 0; r < N; ++r) {
-                if (r >= R) break;
-                const float x = warp_sum(l[r]);
-                if (lane == 0) s_red[q][r] = x;
+            for (int r0 = 0; r0 < N; r0 += 16) {   // (16 reductions side by side: one after the other they cost 32 rows 2 us)
+                if (r0 >= R) break;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) l[r0 + r] += __shfl_xor_sync(0xffffffffu, l[r0 + r], o);
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    if (lane == 0) *reinterpret_cast<float4 *>(&s_red[q][r0 + r]) = make_float4(l[r0 + r], l[r0 + r + 1], l[r0 + r + 2], l[r0 + r + 3]);
             }
             ct_sync();
             const bool whole = w.whole != 0, bad = s_bad[seg & (CT_SLOTS - 1)] == seg + 1;

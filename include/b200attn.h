@@ -309,7 +309,8 @@ typedef struct b200attn_attend_args {
     unsigned flags;              /* B200ATTN_FLAG_ASYNC, B200ATTN_FLAG_FORCE_GENERIC */
 } b200attn_attend_args;
 int b200attn_cache_attend(const b200attn_attend_args *args);
-/* Bytes of workspace that this call needs; needs no valid pointers.  0 and a message for b200attn_last_error() where the call would be refused. */
+/* Bytes of workspace that this call needs; needs no valid pointers.  0: none (short caches), or the call would be refused: then b200attn_last_error() says why, and is
+ * "" otherwise. */
 size_t b200attn_cache_attend_workspace(const b200attn_attend_args *args);
 
 /* The i-th accepted token of sequence b, the new token t = accepted[b,i], becomes row length[b] + i: K and V of that row are copied from Kd and Vd
