@@ -451,7 +451,7 @@ int weights(const b200attn_weights_args *a) {
         return host_end(&c, st, a->flags & B200ATTN_FLAG_ASYNC);
     }
     if (rc != -1) return rc;
-    if (a->dtype == B200ATTN_F32) rc = p.D % 4 == 0 && strides_fit(a->K, a->dtype, p.B, p.Hkv, p.S) ? launch_weights<float, true>(p, c, st) : launch_weights<float, false>(p, c, st);
+    if (a->dtype == B200ATTN_F32) rc = p.D % 4 == 0 && strides_fit(a->K, a->dtype, p.B, p.Hkv, p.S) && strides_fit(a->Q, a->dtype, p.B, p.Hq, p.T) ? launch_weights<float, true>(p, c, st) : launch_weights<float, false>(p, c, st);
     else rc = a->dtype == B200ATTN_F16 ? launch_weights<__half, false>(p, c, st) : launch_weights<__nv_bfloat16, false>(p, c, st);
     if (rc) return rc;
     set_last_path("cache_generic");

@@ -508,15 +508,16 @@ struct CwParams {
     unsigned spin_limit;
 };
 
-// Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows.
+// Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows; the next 16 rows
+// are on their way under the present ones' products (8 heads, 142 tokens, up to 303 rows, head_d 80, fp32: 44 us with each load waited for).
 template <typename T, bool FAST>
 __global__ void __launch_bounds__(CG_THREADS)
 cw_generic_kernel(const CwParams p) {
     extern __shared__ __align__(16) float cg_smem[];
-    __shared__ float s_lse[CG_ROWS], s_half[CG_KEYS];
-    __shared__ int s_i[CG_ROWS];
+    __shared__ float s_lse[2][CG_ROWS], s_half[CG_KEYS];
+    __shared__ int s_i[2][CG_ROWS];
     const int pitch = cg_pitch(p.D), tid = threadIdx.x;
-    float *qs = cg_smem, *ks = qs + CG_ROWS * pitch;
+    float *ks = cg_smem, *qs = ks + CG_KEYS * pitch;   // qs: two buffers where FAST
     grid_launch_dependents();
     grid_dependency_wait();
     const int b = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * CG_KEYS;
@@ -524,40 +525,62 @@ cw_generic_kernel(const CwParams p) {
     if (j0 >= n) return;
     const int count = ca_count(p.accepted, b, p.A, p.T, n);
     if (count == 0) return;
-    if (FAST)
-        for (int i = tid; i < CG_KEYS * (pitch - p.D); i += CG_THREADS) ks[i / (pitch - p.D) * pitch + p.D + i % (pitch - p.D)] = 0.0f;
+    if (FAST)   // the columns behind head_d, once
+        for (int i = tid; i < (CG_KEYS + 2 * CG_ROWS) * (pitch - p.D); i += CG_THREADS) ks[i / (pitch - p.D) * pitch + p.D + i % (pitch - p.D)] = 0.0f;
     cg_load<T, FAST>(ks, p.K, p.k, b, h, j0, min(CG_KEYS, n - j0), p.D, p.S);
-    const int j = tid & 63, rb = (tid >> 6) * 8;
-    float sum = 0.0f;
-    for (int r0 = 0; r0 < count * p.G; r0 += CG_ROWS) {
-        __syncthreads();
+    const int j = tid & 63, rb = (tid >> 6) * 8, rows = count * p.G;
+    const int *list = p.accepted ? p.accepted + (long long)b * p.A : nullptr;
+    // 16 rows from r0 on into buffer `u`; where FAST they are on their way when this returns
+    auto load = [&](int r0, int u) {
+        float *dst = qs + u * CG_ROWS * pitch;
         if (tid < CG_ROWS) {
             const int r = r0 + tid, i = r / p.G;
             float x = -INFINITY;
-            if (i < count) x = p.lse[((long long)b * p.Hq + h * p.G + r % p.G) * p.T + (p.accepted ? p.accepted[(long long)b * p.A + i] : i)];
-            s_i[tid] = x == -INFINITY ? -1 : i;   // a token that saw nothing gave no weight
-            s_lse[tid] = x;
+            if (r < rows) x = p.lse[((long long)b * p.Hq + h * p.G + r - i * p.G) * p.T + (list ? list[i] : i)];
+            s_i[u][tid] = x == -INFINITY ? -1 : i;   // a token that saw nothing gave no weight
+            s_lse[u][tid] = x;
         }
-        for (int i0 = tid; i0 < CG_ROWS * pitch; i0 += 4 * CG_THREADS) {
-            float x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i0 + k * CG_THREADS, q = i / pitch, d = i - q * pitch, r = r0 + q, a = r / p.G;
-                x[k] = q < CG_ROWS && a < count && d < p.D ? to_f32(ca_row<T>(p.Q, p.q, b, h * p.G + r % p.G, p.accepted ? p.accepted[(long long)b * p.A + a] : a)[d]) : 0.0f;
+        if (FAST) {
+            const int pieces = p.D >> 2;
+            for (int k = tid; k < CG_ROWS * pieces; k += CG_THREADS) {
+                const int q = k / pieces, c = k - q * pieces, r = min(r0 + q, rows - 1), i = r / p.G;
+                cg_copy16(dst + q * pitch + 4 * c, ca_row<T>(p.Q, p.q, b, h * p.G + r - i * p.G, list ? list[i] : i) + 4 * c, r0 + q < rows);
             }
+            cg_commit();
+        } else {
+            for (int i0 = tid; i0 < CG_ROWS * pitch; i0 += 4 * CG_THREADS) {
+                float x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i0 + k * CG_THREADS < CG_ROWS * pitch) qs[i0 + k * CG_THREADS] = x[k];
+                for (int k = 0; k < 4; ++k) {
+                    const int at = i0 + k * CG_THREADS, q = at / pitch, d = at - q * pitch, r = r0 + q, i = r / p.G;
+                    x[k] = q < CG_ROWS && r < rows && d < p.D ? to_f32(ca_row<T>(p.Q, p.q, b, h * p.G + r - i * p.G, list ? list[i] : i)[d]) : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i0 + k * CG_THREADS < CG_ROWS * pitch) dst[i0 + k * CG_THREADS] = x[k];
+            }
+        }
+    };
+    float sum = 0.0f;
+    // rows of tokens in front of the first that sees any of these keys are left out
+    const long long none = (long long)(j0 - (n - count)) * p.G;
+    const int first = none <= 0 ? 0 : (int)(none / CG_ROWS * CG_ROWS);
+    if (FAST) load(first, 0);
+    for (int r0 = first, u = 0; r0 < rows; r0 += CG_ROWS, u ^= FAST ? 1 : 0) {
+        if (!FAST) {
+            __syncthreads();
+            load(r0, 0);
         }
         cg_wait<0>();
-        __syncthreads();
-        if (r0 + rb >= count * p.G) continue;   // (the same for a warp)
+        __syncthreads();   // (and everybody is done with the other buffer)
+        if (FAST && r0 + CG_ROWS < rows) load(r0 + CG_ROWS, u ^ 1);
+        if (r0 + rb >= rows) continue;   // (the same for a warp)
         float s[8];
-        cg_scores(qs + rb * pitch, ks + j * pitch, pitch, s);
+        cg_scores(qs + (u * CG_ROWS + rb) * pitch, ks + j * pitch, pitch, s);
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const int i = s_i[rb + r];
-            if (i >= 0 && j0 + j <= n - count + i) sum += exp2f(fmaf(s[r], p.scale_log2, -1.4426950408889634f * s_lse[rb + r]));
+            const int i = s_i[u][rb + r];
+            if (i >= 0 && j0 + j <= n - count + i) sum += exp2f(fmaf(s[r], p.scale_log2, -1.4426950408889634f * s_lse[u][rb + r]));
         }
     }
     if (tid >= 64) s_half[j] = sum;
