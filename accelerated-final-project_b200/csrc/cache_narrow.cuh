@@ -11,7 +11,8 @@
 // A row's reference only has to be within 2^8 of its maximum (the exponents stay exact in fp32, weights below 2^8 in fp16): per tile the threads
 // only vote whether some score is beyond that - one barrier - and reduce maxima, set new references and rescale where it is, which is at a
 // unit's first tile and hardly ever again.  Roundings as in cache_tc.cuh.
-//   64 sequences, one token, 32 / 8 heads of 128, 0 to 8192 rows cached, bf16 (1.07 GB): rows as lanes 250 us (1.63 GHz under the power cap)
+//   64 sequences, one token, 32 / 8 heads of 128, 0 to 8192 rows cached, bf16 (1.07 GB): 180 us, 6.0 TB/s, 0.91 of the copy rate; rows as lanes 250 us (1.63 GHz
+//   under the power cap).  SMs get rates that differ by 12 % either way, and shares are equal.
 #pragma once
 
 #include "cache_tc.cuh"

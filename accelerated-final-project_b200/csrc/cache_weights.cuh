@@ -6,6 +6,8 @@
 // tile needs no joining).  Per pair the accepted rows of Q are brought into shared memory once: by TMA where all new tokens are accepted, else gathered
 // (the list names tokens anywhere).  More rows than fit are taken in chunks, each over the CTA's tiles of the pair again.  Blocks of rows that see nothing
 // of a tile are left out.
+//   32 sequences, up to 6 tokens, 32 / 8 heads of 128, 100 to 8000 rows, bf16 (244 MB read): 47 us, 5.2 TB/s; 700 tokens, 16 heads of 64, up to 2501 rows: 28 us,
+//   bound by the exponentials of 11 blocks a tile.
 //   warp 0       the walk over the tiles; one thread requests K tiles (and Q) by TMA
 //   warp 1       one thread issues the MMAs, 64 rows at a time, into two buffers per summing warpgroup
 //   warps 2, 3   gather the next rows of Q beside the present ones (61 us a call of 32 sequences, up to 6 tokens, 100 to 8000 rows, where the
