@@ -232,7 +232,8 @@ static int set_smem_attr(DeviceCtx &c, int slot, Kern kern) {
 }
 
 // Test hook (b200attn_debug_lost_arrival): the per-head barrier of the fused kernel expects this many
-// arrivals more than there are slices, i.e. waits for a flag that nothing sets, with this poll limit.
+// arrivals more than there are slices, i.e. waits for a flag that nothing sets, with this poll limit; so do the
+// barriers of the key tiles in the tensor-core kernels of the cache calls.
 static std::atomic<unsigned> g_test_wait_extra{0}, g_test_spin_limit{0};
 
 // b200attn_set_option
@@ -877,6 +878,7 @@ int host_begin(HostCall *h) {
     h->max_smem = c->max_smem_optin;
     h->err_dev = c->err_dev; h->err_sys = c->err_host_dev;
     h->spin_limit = current_spin_limit();
+    h->wait_extra = g_test_wait_extra.load();
     if (*reinterpret_cast<volatile unsigned *>(c->err_host) != 0) {
         std::lock_guard<std::mutex> lk(c->mu);
         cudaDeviceSynchronize();

@@ -270,7 +270,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     cudaStream_t st = (cudaStream_t)a->stream;
     CaParams p{};
     fill(p, *a);
-    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit; p.wait_extra = c.wait_extra;
     CtParams ct;
     CnParams cn;
     bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
@@ -444,7 +444,7 @@ int weights(const b200attn_weights_args *a) {
     p.len = a->length; p.accepted = a->accepted; p.lse = a->lse; p.weights = a->weights;
     p.A = A; p.B = a->batch_sz; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.G = G; p.T = a->len_new; p.S = a->capacity; p.D = a->head_d;
     p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_d) : a->scale) * 1.4426950408889634f;
-    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit;
+    p.err = c.err_dev; p.err_sys = c.err_sys; p.spin_limit = c.spin_limit; p.wait_extra = c.wait_extra;
     rc = weights_tc(a, p, c, st);
     if (rc == B200ATTN_OK) {
         set_last_path("cache_tc");

@@ -46,7 +46,7 @@ struct CaParams {
     int by_cta;          // ... per CTA, else per unit
     int join_rows;       // rows that a block of ca_combine_kernel joins
     unsigned *err, *err_sys;
-    unsigned spin_limit;
+    unsigned spin_limit, wait_extra;   // wait_extra: test hook
 };
 
 __host__ __device__ inline size_t ca_slot_floats(int RT, int D) { return ((size_t)RT * (D + 2) + 3) & ~(size_t)3; }
@@ -167,6 +167,10 @@ __device__ __forceinline__ void ca_entry_of_unit(const CaParams &p, const CaStar
     e[2] = ca_cta_of(s.total, s.grid, w.u0 + p.OH + w.nt - 1);
     e[3] = w.b; e[4] = w.h; e[5] = w.rt;
     e[0] = w.whole(p) ? -1 : c;
+}
+// By a CTA that gives up in the unit `w` is at: the entries that it has not written yet.  The joining launch comes all the same, and takes addresses from them.
+__device__ __forceinline__ void ca_entries_left(const CaParams &p, const CaStart &s, CaWalk &w, int c, int seg) {
+    for (; w.left > 0; ++seg, w.next(p)) ca_entry_of_unit(p, s, w, c, seg == 0);
 }
 // ... else per CTA: by each CTA for the first unit of its range, which is listed where it was cut by this range's beginning and by none before it.
 __device__ __forceinline__ void ca_entry_of_cta(const CaParams &p, const CaStart &s, const CaWalk &w, int c) {
@@ -525,7 +529,7 @@ struct CwParams {
     int B, Hq, Hkv, G, T, S, D;
     float scale_log2;
     unsigned *err, *err_sys;
-    unsigned spin_limit;
+    unsigned spin_limit, wait_extra;
 };
 
 // Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows; the next 16 rows

@@ -83,7 +83,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lim = p.spin_limit;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.kv_full[i], 1); mbar_init(&bars.kv_empty[i], 2); mbar_init(&bars.ready[i], 1); }
+        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.kv_full[i], 1 + p.wait_extra); mbar_init(&bars.kv_empty[i], 2); mbar_init(&bars.ready[i], 1); }
         for (int i = 0; i < CT_SLOTS; ++i) { mbar_init(&bars.seg[i], 1); s_bad[i] = 0; }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.q_full[i], 1); mbar_init(&bars.q_empty[i], 1);
@@ -147,7 +147,10 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (ok) {
                 s_seg[seg & (CT_SLOTS - 1)].whole = -1;
                 mbar_arrive(&bars.seg[seg & (CT_SLOTS - 1)]);
-            } else CN_FAIL_AT(0, true)
+            } else {
+                CN_FAIL_AT(0, true)
+                ca_entries_left(p, s_start, w, blockIdx.x, seg);
+            }
         }
     } else if (warp == 3) {
         int s = 0;

@@ -224,7 +224,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     const uint32_t lim = p.spin_limit;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.kv_full[i], 1); mbar_init(&bars.kv_empty[i], NT + 1); mbar_init(&bars.ready[i], 1); }
+        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.kv_full[i], 1 + p.wait_extra); mbar_init(&bars.kv_empty[i], NT + 1); mbar_init(&bars.ready[i], 1); }
         for (int i = 0; i < CT_SLOTS; ++i) { mbar_init(&bars.seg[i], 1); s_bad[i] = 0; }
         for (int i = 0; i < 2; ++i) { mbar_init(&bars.q_full[i], 1); mbar_init(&bars.q_empty[i], NT); }
         for (int t = 0; t < 2; ++t) {
@@ -298,6 +298,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 } else {
                     report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << 16));
                     failed = true;
+                    ca_entries_left(p, s_start, w, blockIdx.x, seg);
                 }
             }
         } else if (warp == 3) {

@@ -76,7 +76,7 @@ cw_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     const uint32_t lim = p.spin_limit;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.k_full[i], 1); mbar_init(&bars.k_empty[i], 1); }
+        for (int i = 0; i < CT_MAX_STAGES; ++i) { mbar_init(&bars.k_full[i], 1 + p.wait_extra); mbar_init(&bars.k_empty[i], 1); }
         for (int i = 0; i < CX_SLOTS; ++i) mbar_init(&bars.seg[i], 1);
         for (int i = 0; i < 2; ++i) { mbar_init(&bars.q_full[i], cx.box_t ? 3 : 2); mbar_init(&bars.q_empty[i], 8); s_skip[i] = 0; }
         for (int i = 0; i < CX_BUFS; ++i) { mbar_init(&bars.s_full[i], 1); mbar_init(&bars.s_read[i], 4); }

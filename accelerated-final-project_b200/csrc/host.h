@@ -19,7 +19,7 @@ struct HostCall {
     int dev = 0, sm_count = 0;
     size_t max_smem = 0;             // opt-in shared memory of a CTA, static part included
     unsigned *err_dev = nullptr, *err_sys = nullptr;
-    unsigned spin_limit = 0;
+    unsigned spin_limit = 0, wait_extra = 0;   // wait_extra: arrivals that a kernel waits for and nobody makes (b200attn_debug_lost_arrival)
     std::unique_lock<std::mutex> lock;   // held by a call that uses the library's workspace, until it has enqueued its work
 };
 // Looks the current device up; reports what an earlier asynchronous call left behind.

@@ -229,7 +229,8 @@ int b200attn_set_option(int option, long long value);
  *   launches, P V launches] in out[0..2] and the launch counts in out[3..5], clearing the record.
  * b200attn_debug_lost_arrival: failure detection without a fault.  With extra > 0 the per-head barrier
  *   of the fp32 split-head_d kernels waits (at most spin_limit polls) for arrivals that never come, gives
- *   up, and the call reports B200ATTN_ERR_KERNEL; (0, 0) restores normal operation.
+ *   up, and the call reports B200ATTN_ERR_KERNEL; (0, 0) restores normal operation.  The tensor-core kernels of
+ *   the cache calls wait for their first key tile in the same way.
  * b200attn_debug_tile_of: host copy of the tile enumeration of the bf16 two-kernel path (big = 0: tile j
  *   of a head in launch `mode` -> query tile, key tile; big = 1: the 256-row variant); returns the number
  *   of tiles per head of that launch or -1 when the launch does not exist for the shape.  Needs no GPU. */
