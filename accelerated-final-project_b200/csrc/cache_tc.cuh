@@ -186,11 +186,12 @@ __device__ __forceinline__ void ct_store_rows(unsigned char *at, uint32_t (&w)[3
     }
 }
 
-#define CT_FAIL_AT(site, cond)                                                                          \
-    if (cond) {                                                                                         \
+// A lane whose wait has run out stays with its warp, which has barriers and collective instructions in front of it: it waits no more, computes on what there
+// is, in bounds as ever, and the warp leaves together at the unit's end.  (It costs the waits nothing; a vote at each would.)
+#define CT_WAIT_AT(site, wait)                                                                          \
+    if (!failed && !(wait)) {                                                                           \
         report_kernel_error(p.err, p.err_sys, (unsigned)KERR_MBAR_TIMEOUT | (1u << (16 + (site))));     \
         failed = true;                                                                                  \
-        break;                                                                                          \
     }
 
 constexpr int ct_threads(int NT) { return 128 + NT * 128; }
@@ -431,19 +432,20 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         uint32_t g = 0;   // key tiles so far
         uint32_t r[TK / 32][32];
         auto pv_done = [&](uint32_t x) { return mbar_wait(&bars.o_done[t][x & 1], (x >> 1) & 1u, lim); };
-        for (int seg = 0; !failed; ++seg) {
-            CT_FAIL_AT(7, !mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim));
+        for (int seg = 0;; ++seg) {
+            CT_WAIT_AT(7, mbar_wait(&bars.seg[seg & (CT_SLOTS - 1)], (uint32_t)(seg / CT_SLOTS) & 1u, lim));
+            if (__any_sync(0xffffffffu, failed)) { failed = true; break; }
             const CtSeg &w = s_seg[seg & (CT_SLOTS - 1)];
             if (w.whole < 0) break;
             const int tok0 = (w.rt * NT + t) * ct.tpt, rows = min(ct.tpt, p.T - tok0) * p.G;
             if (NT == 2 && rows <= 0) {   // a tile's hand-offs (above)
-                CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                CT_WAIT_AT(3, mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&bars.s_read[t][g & 1]);
                     for (int h = 0; h < NH; ++h) mbar_arrive(&bars.p_full[t][g & 1][h]);
                 }
-                CT_FAIL_AT(6, !pv_done(g));
+                CT_WAIT_AT(6, pv_done(g));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.o_empty[t]);
                 ++g;
@@ -459,10 +461,10 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 const int j0 = (draft ? i - nct : i) * TK;
                 const bool part = draft || i + 1 == nct;   // (the same for every thread) keys that may not be there, or not be seen
                 if (!act) {   // a warp without rows keeps the hand-offs in step
-                    CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                    CT_WAIT_AT(3, mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.s_read[t][g & 1]);
-                    if (g >= (uint32_t)ct.np) CT_FAIL_AT(5, !pv_done(g - ct.np));
+                    if (g >= (uint32_t)ct.np) CT_WAIT_AT(5, pv_done(g - ct.np));
                     __syncwarp();
                     if (lane == 0)
                         for (int h = 0; h < NH; ++h) mbar_arrive(&bars.p_full[t][g & 1][h]);
@@ -486,7 +488,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                         }
                     }
                 }
-                CT_FAIL_AT(3, !mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
+                CT_WAIT_AT(3, mbar_wait(&bars.s_full[t][g & 1], (g >> 1) & 1u, lim));
                 tc_fence_after();
                 const uint32_t ts = tl + (NT == 1 ? (g & 1) : t) * 128u;
 #pragma unroll
@@ -517,7 +519,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 } else {
                     const bool need = mine && top > m_ref + CT_RESCALE_LOG2;
                     if (__any_sync(0xffffffffu, need)) {
-                        CT_FAIL_AT(4, !pv_done(g - 1));
+                        CT_WAIT_AT(4, pv_done(g - 1));
                         tc_fence_after();
                         const float m_new = need ? top : m_ref;
                         const float f = need ? fast_exp2(m_ref - m_new) : 1.0f;   // (0 where the row had seen nothing)
@@ -535,7 +537,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     }
                 }
                 const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;   // a row that has seen nothing: every score is -inf
-                if (g >= (uint32_t)ct.np) CT_FAIL_AT(5, !pv_done(g - ct.np));   // the MMAs have read what was in this P buffer
+                if (g >= (uint32_t)ct.np) CT_WAIT_AT(5, pv_done(g - ct.np));   // the MMAs have read what was in this P buffer
                 const uint32_t pw = prow + (ct.np == 2 ? (g & 1) * NH * slab : 0u);
                 const uint64_t sl2_2 = ct_pair(sl2, sl2), neg_2 = ct_pair(neg, neg);
                 uint64_t sum = 0;   // a pair of sums
@@ -564,9 +566,8 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 ct_unpair(sum, sum0, sum1);
                 l += sum0 + sum1;
             }
-            if (failed) break;
             // ---- epilogue of the unit ----
-            CT_FAIL_AT(6, !pv_done(g - 1));
+            CT_WAIT_AT(6, pv_done(g - 1));
             tc_fence_after();
             if (act) {
                 const bool whole = w.whole != 0, bad = s_bad[seg & (CT_SLOTS - 1)] == seg + 1;
@@ -631,7 +632,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
-#undef CT_FAIL_AT
+#undef CT_WAIT_AT
 
 // ---- host: tensor maps ----------------------------------------------------------------------------------------------------
 // [B, heads, rows, D] as {D, rows, heads, B}, boxes of 64 columns x `box_rows`; what lies outside reads as 0.  A dimension of size 1 has no stride to speak of.

@@ -40,6 +40,10 @@ ATTEND = [
     ("cache_narrow", (1, 8, 2, 3, 5000, (5000,), 128, "tree")),              # few units, each cut over many CTAs: an entry per unit
     ("cache_narrow", (90, 4, 2, 2, 1500, (1500, 3, 0, 900), 64, "chain")),   # more units than CTAs: several a CTA, an entry per CTA
     ("cache_narrow", (70, 8, 2, 1, 1500, (1500, 1400), 128, "chain")),       # one unit a CTA or two: an entry per unit
+    ("cache_tc", (1, 16, 2, 64, 3000, (3000,), 128, "tree")),                # two row tiles a unit
+    ("cache_tc", (2, 4, 4, 200, 700, (700, 90), 64, "none")),                # ... the last one without a second tile
+    ("cache_tc", (70, 16, 2, 16, 900, (900, 0, 5), 64, "tree")),             # one row tile a unit
+    ("cache_tc", (3, 16, 2, 30, 500, (500, 31), 256, "chain")),              # tiles of 64 keys
 ]
 
 
