@@ -30,6 +30,12 @@ int check_capacity(int capacity) {
     return B200ATTN_OK;
 }
 
+int check_scale(float scale) {   // (the kernels take it times log2 e)
+    if (!(scale >= 0.0f) || std::isinf(scale * 1.4426950408889634f))
+        return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, also times log2 e, or 0 for 1/sqrt(head_d)");
+    return B200ATTN_OK;
+}
+
 int check_view(const char *name, const b200attn_view &v, int dtype) {
     if (v.ptr == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be non-NULL", name);
     if ((uintptr_t)v.ptr & (esize(dtype) - 1)) return fail(B200ATTN_ERR_INVALID_ARG, "%s must be aligned to the element size", name);
@@ -98,7 +104,7 @@ int validate(const b200attn_attend_args *a, bool pointers) {
     if ((rc = check_capacity(a->capacity))) return rc;
     if ((long long)a->len_new * (a->num_heads / a->num_kv_heads) > (1ll << 30))
         return fail(B200ATTN_ERR_TOO_LARGE, "len_new times the query heads of a key head is %lld, at most 2^30 are taken", (long long)a->len_new * (a->num_heads / a->num_kv_heads));
-    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");
+    if ((rc = check_scale(a->scale))) return rc;
     if ((a->Kd.ptr == nullptr) != (a->Vd.ptr == nullptr)) return fail(B200ATTN_ERR_INVALID_ARG, "Kd and Vd must be given together");
     if (a->mask && a->Kd.ptr == nullptr) return fail(B200ATTN_ERR_INVALID_ARG, "a mask needs Kd and Vd");
     if (a->mask && a->mask_stride_b != 0 && a->mask_stride_b != (long long)a->len_new * a->len_new)
@@ -432,7 +438,7 @@ int weights(const b200attn_weights_args *a) {
     if ((rc = check_capacity(a->capacity))) return rc;
     const int A = a->accepted ? a->max_accepted : a->len_new, G = a->num_heads / a->num_kv_heads;
     if ((long long)A * G > (1ll << 30)) return fail(B200ATTN_ERR_TOO_LARGE, "accepted tokens times the query heads of a key head are %lld, at most 2^30 are taken", (long long)A * G);
-    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(B200ATTN_ERR_INVALID_ARG, "scale must be positive and finite, or 0 for 1/sqrt(head_d)");
+    if ((rc = check_scale(a->scale))) return rc;
     if ((rc = check_view("Q", a->Q, a->dtype)) || (rc = check_view("K", a->K, a->dtype)) || (rc = check_accepted(a->accepted, a->max_accepted))) return rc;
     if (!a->length || !a->lse || !a->weights) return fail(B200ATTN_ERR_INVALID_ARG, "length, lse and weights must be non-NULL");
     if (((uintptr_t)a->length | (uintptr_t)a->lse | (uintptr_t)a->weights) & 3) return fail(B200ATTN_ERR_INVALID_ARG, "length, lse and weights must be aligned to 4 bytes");

@@ -4,7 +4,8 @@
 // Attention, for the rows r = t G + g of a key head (G query heads share it), visible keys j:
 //     s_rj = scale q_r . k_j,   lse_r = log sum_j exp(s_rj),   out_r = sum_j exp(s_rj - lse_r) v_j.
 // One pass over the keys with a running maximum m and sum l: when m grows to m', l and the accumulator are multiplied by exp(m - m').
-// Parts over different keys join by the same rule.
+// Parts over different keys join by the same rule.  Exponents are differences of scores, times scale log2 e; where one is taken as s c - m with m = s' c rounded
+// (one multiply-add), m has to be below CA_EXACT: from there on its rounding alone is more than an exponential takes.
 //
 // Sharing out: a unit is (sequence, key head, tile of RT rows); its items are the tiles of TK cached keys, then those of the new tokens' keys.  In front of
 // them stand OH items without work: what a unit's beginning and end cost a CTA, in tiles (short sequences would be taken for cheap otherwise).
@@ -21,6 +22,10 @@
 namespace b200attn {
 
 constexpr int CA_MAX_D = 256;
+constexpr float CA_EXACT = 16777216.0f;   // 2^24: rounded by half at the most
+
+// the reference m (log2 units) of a row is one that the differences of scores have to be taken from first; not that of a row that has seen nothing (-inf)
+__device__ __forceinline__ bool ca_large(float m) { return fabsf(m) >= CA_EXACT && fabsf(m) < INFINITY; }
 
 struct CaView { long long b, h, l; };   // strides in elements
 
@@ -426,14 +431,14 @@ ca_generic_kernel(const CaParams p) {
             if (tile + 1 < end) load(ks, false, tile + 1);
             else if (FAST) cg_commit();   // (an empty group: the counts below stay the same)
             for (int r = warp; r < rows; r += CG_THREADS / 32) {
-                const float a = ps[lane * PP + r], b = ps[(lane + 32) * PP + r], mo = s_m[r];
-                const float mn = fmaxf(mo, warp_max(fmaxf(a, b)) * p.scale_log2);
-                const float ea = a == -INFINITY ? 0.0f : exp2f(fmaf(a, p.scale_log2, -mn)), eb = b == -INFINITY ? 0.0f : exp2f(fmaf(b, p.scale_log2, -mn));
+                const float a = ps[lane * PP + r], b = ps[(lane + 32) * PP + r], mo = s_m[r];   // (maxima of q . k, not yet scaled)
+                const float mn = fmaxf(mo, warp_max(fmaxf(a, b)));
+                const float ea = a == -INFINITY ? 0.0f : exp2f((a - mn) * p.scale_log2), eb = b == -INFINITY ? 0.0f : exp2f((b - mn) * p.scale_log2);
                 const float sum = warp_sum(ea + eb);
                 ps[lane * PP + r] = ea;
                 ps[(lane + 32) * PP + r] = eb;
                 if (lane == 0) {
-                    const float f = mn == -INFINITY ? 0.0f : exp2f(mo - mn);
+                    const float f = mn == -INFINITY ? 0.0f : exp2f((mo - mn) * p.scale_log2);
                     s_f[r] = f;
                     s_l[r] = s_l[r] * f + sum;
                     s_m[r] = mn;
@@ -491,7 +496,7 @@ ca_generic_kernel(const CaParams p) {
             }
         }
         if (tid < rows) {
-            const float m = s_m[tid], l = s_l[tid];
+            const float m = s_m[tid] * p.scale_log2, l = s_l[tid];
             if (!whole) {
                 part[(size_t)p.RT * p.D + 2 * tid] = m;
                 part[(size_t)p.RT * p.D + 2 * tid + 1] = l;

@@ -50,7 +50,7 @@ __device__ __forceinline__ float cn_warp_max(float x) {
 }
 __device__ __forceinline__ void ct_st_shared_u16(uint32_t addr, uint16_t x) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(x) : "memory"); }
 
-constexpr float CN_UNSET = 1.7e38f;   // minus the reference of a row that has seen nothing: any score is far beyond it
+constexpr float CN_UNSET = 3.402823466e38f;   // minus the reference of a row that has seen nothing: any finite score is beyond it
 
 #define CN_FAIL_AT(site, cond)                                                                          \
     if (cond) {                                                                                         \
@@ -70,6 +70,8 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __shared__ uint32_t tmem_slot;
     __shared__ int s_bad[CT_SLOTS];
     __shared__ __align__(16) float s_neg[N], s_f[N], s_inv[N], s_red[4][N];   // minus the reference (log2 units), factor of a change, 1 / l, per-warp values
+    __shared__ __align__(16) float s_x[N], s_zero[N];   // the reference before its scaling, 0 where there is none; zeros
+    __shared__ int s_large;                             // some reference is large (ca_large)
     const CaParams &p = cn.a;
     const uint32_t raw_addr = smem_u32(ct_smem_raw);
     unsigned char *smem = ct_smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
@@ -93,7 +95,8 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
         if (p.drafts) { tma_prefetch_desc(&tmKd); tma_prefetch_desc(&tmVd); }
     }
-    if (threadIdx.x < N) s_neg[threadIdx.x] = CN_UNSET;
+    if (threadIdx.x < N) { s_neg[threadIdx.x] = CN_UNSET; s_x[threadIdx.x] = s_zero[threadIdx.x] = 0.0f; }
+    if (threadIdx.x == 0) s_large = 0;
     if (warp == 1) tmem_alloc(&tmem_slot, (uint32_t)cn.tmem_cols);
     grid_dependency_wait();
     if (warp == 2) {
@@ -341,11 +344,13 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     ct_sync();
                     if (tid < R) {
-                        const float m = fmaxf(fmaxf(s_red[0][tid], s_red[1][tid]), fmaxf(s_red[2][tid], s_red[3][tid])) * sl2, old = s_neg[tid];
+                        const float mx = fmaxf(fmaxf(s_red[0][tid], s_red[1][tid]), fmaxf(s_red[2][tid], s_red[3][tid])), m = mx * sl2, old = s_neg[tid];
                         float f = 1.0f;
                         if (m + old > CT_RESCALE_LOG2) {
                             f = old == CN_UNSET ? 0.0f : fast_exp2(-old - m);
                             s_neg[tid] = -m;
+                            s_x[tid] = mx;
+                            if (ca_large(m)) s_large = 1;
                         }
                         s_f[tid] = f;
                     }
@@ -372,10 +377,17 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 if (g >= 2) CN_FAIL_AT(5, !pv_done(g - 2));   // the MMAs have read what was in this P buffer
                 const uint32_t pb = pw + (g & 1) * 2 * slab;
+                const float *refs = s_neg;
+                if (s_large) {   // (the same for all four warps)
+                    refs = s_zero;
+#pragma unroll
+                    for (int r = 0; r < N; ++r)
+                        if (r < R) x[r] -= s_x[r];
+                }
 #pragma unroll
                 for (int r0 = 0; r0 < N; r0 += 8) {   // (8 rows without a branch)
                     if (r0 >= R) break;
-                    const float4 na = *reinterpret_cast<const float4 *>(s_neg + r0), nb = *reinterpret_cast<const float4 *>(s_neg + r0 + 4);
+                    const float4 na = *reinterpret_cast<const float4 *>(refs + r0), nb = *reinterpret_cast<const float4 *>(refs + r0 + 4);
                     const float nn[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
                     float e[8];
 #pragma unroll
@@ -418,6 +430,8 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 s_inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
                 s_neg[tid] = CN_UNSET;
+                s_x[tid] = 0.0f;
+                if (tid == 0) s_large = 0;
             }
             CN_FAIL_AT(6, !pv_done(g - 1));
             tc_fence_after();

@@ -454,7 +454,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
             const bool act = 32 * q < rows;       // the same for a warp
             const bool mine = row < rows;
             const int tok = min(tok0 + row / p.G, p.T - 1);
-            float m_ref = -INFINITY, l = 0.0f;
+            float x_ref = -INFINITY, l = 0.0f;   // the reference is x_ref sl2
             const int first = w.tile, end = w.end, nct = w.ct;
             for (int i = first; i < end; ++i, ++g) {
                 const bool draft = i >= nct;
@@ -513,16 +513,15 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                         a = ct_max3(a, __uint_as_float(r[x][k]), __uint_as_float(r[x][k + 1]));
                         b = ct_max3(b, __uint_as_float(r[x][k + 2]), __uint_as_float(r[x][k + 3]));
                     }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                if (i == first) {
-                    m_ref = top;
-                } else {
-                    const bool need = mine && top > m_ref + CT_RESCALE_LOG2;
+                const float topx = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                bool taken = false;   // the scores are differences from x_ref already
+                const bool need = i > first && mine && topx * sl2 > x_ref * sl2 + CT_RESCALE_LOG2;
+                if (i == first) x_ref = topx;
+                if (__any_sync(0xffffffffu, need || (mine && ca_large(x_ref * sl2)))) {
                     if (__any_sync(0xffffffffu, need)) {
                         CT_WAIT_AT(4, pv_done(g - 1));
                         tc_fence_after();
-                        const float m_new = need ? top : m_ref;
-                        const float f = need ? fast_exp2(m_ref - m_new) : 1.0f;   // (0 where the row had seen nothing)
+                        const float f = need ? fast_exp2(x_ref * sl2 - topx * sl2) : 1.0f;   // (0 where the row had seen nothing)
                         uint32_t o[16];
                         for (int c = 0; c < p.D; c += 16) {
                             tmem_ld16(to + c, o);
@@ -533,10 +532,18 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                         }
                         tmem_st_wait();
                         l *= f;
-                        m_ref = m_new;
+                        if (need) x_ref = topx;
+                    }
+                    if (__any_sync(0xffffffffu, mine && ca_large(x_ref * sl2))) {   // differences first, then the scale
+                        const float x0 = x_ref == -INFINITY ? 0.0f : x_ref;
+#pragma unroll
+                        for (int x = 0; x < TK / 32; ++x)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) r[x][k] = __float_as_uint(__uint_as_float(r[x][k]) - x0);
+                        taken = true;
                     }
                 }
-                const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;   // a row that has seen nothing: every score is -inf
+                const float neg = taken || x_ref == -INFINITY ? 0.0f : -x_ref * sl2;   // a row that has seen nothing: every score is -inf
                 if (g >= (uint32_t)ct.np) CT_WAIT_AT(5, pv_done(g - ct.np));   // the MMAs have read what was in this P buffer
                 const uint32_t pw = prow + (ct.np == 2 ? (g & 1) * NH * slab : 0u);
                 const uint64_t sl2_2 = ct_pair(sl2, sl2), neg_2 = ct_pair(neg, neg);
@@ -612,6 +619,7 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     }
                 }
                 if (mine) {
+                    const float m_ref = x_ref * sl2;
                     if (!whole) {
                         prt[(size_t)p.RT * p.D + 2 * urow] = m_ref;
                         prt[(size_t)p.RT * p.D + 2 * urow + 1] = l;

@@ -288,7 +288,8 @@ typedef struct b200attn_view {   /* a tensor [B, heads, rows, D] */
 /* out[b,h,t] = sum_j w_j V_j, w = softmax over the keys that token t sees of scale * Q[b,h,t] . K_j: the rows j < length[b] of the cache
  * and, where Kd and Vd [B,Hkv,T,D] are given, the new tokens u with mask[b,t,u] != 0, or, without a mask, u <= t (a chain: the next token, or
  * a prompt's next piece).  Without Kd and Vd the queries see the cache alone (cross attention to an encoder's states).
- * lse[b,h,t] = log of the sum of exp(scale * Q . K_j), fp32.  A token that sees no key has out 0 and lse -inf.  Scores, softmax and
+ * lse[b,h,t] = log of the sum of exp(scale * Q . K_j), fp32.  A token that sees no key has out 0 and lse -inf; so does one whose every score is -inf.  Q . K_j, and its product
+ * with scale log2 e, count as infinite beyond fp32's range.  Scores, softmax and
  * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V.  A masked key and its value
  * have no effect on a row, whatever they hold. */
 typedef struct b200attn_attend_args {
@@ -302,7 +303,7 @@ typedef struct b200attn_attend_args {
     long long mask_stride_b;     /* T*T, or 0 where all sequences share one mask */
     int batch_sz, num_heads, num_kv_heads, len_new, capacity, head_d;   /* B, Hq, Hkv, T, S, D; D <= 256 */
     int dtype;                   /* enum b200attn_dtype */
-    float scale;                 /* 0 means 1/sqrt(head_d) */
+    float scale;                 /* 0 means 1/sqrt(head_d); up to 2.3e38 */
     void *workspace;             /* device memory of b200attn_cache_attend_workspace bytes, 16-byte aligned; NULL: the library's own, with
                                     the rules of b200attn_forward_ex for streams, threads and captures */
     size_t workspace_bytes;

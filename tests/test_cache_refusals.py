@@ -1,0 +1,10 @@
+"""CPU tests of what the cache entry points refuse, beside test_cache.py."""
+import pytest
+
+from test_cache import attend_args, status, weights_args
+
+
+@pytest.mark.parametrize("name,args", [("attend", attend_args), ("weights", weights_args)])
+def test_a_scale_that_overflows_in_units_of_log2_e_is_refused(pkg, name, args):
+    rc, msg = status(pkg, name, args(pkg, scale=2.4e38))   # times log2 e: beyond fp32
+    assert rc == 1 and b"scale" in msg, msg
