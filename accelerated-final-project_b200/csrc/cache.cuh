@@ -200,6 +200,26 @@ __device__ __forceinline__ const T *ca_row(const void *base, const CaView &v, in
     return reinterpret_cast<const T *>(base) + b * v.b + h * v.h + l * v.l;
 }
 
+// ---- values that are not finite -----------------------------------------------------------------------------------------
+// A weight is above 0, but may be rounded to 0, and 0 times an infinite value is NaN.  So a result that is NaN, though no score of its row was, is looked at
+// again where it was written: the values that the row sees in that column decide, whatever they weigh.
+constexpr unsigned CA_POS = 1, CA_NEG = 2, CA_NAN = 4;
+__device__ __forceinline__ unsigned ca_kind(float v) { return fabsf(v) < INFINITY ? 0u : v != v ? CA_NAN : v > 0.0f ? CA_POS : CA_NEG; }
+// a sum of values of these kinds: an infinity where all that are not finite have one sign
+template <typename T>
+__device__ __forceinline__ void ca_settle(T *sum, unsigned kinds) {
+    const float x = to_f32(*sum);
+    if (x != x && (kinds == CA_POS || kinds == CA_NEG)) *sum = OutCvt<T>::one(kinds == CA_POS ? INFINITY : -INFINITY);
+}
+// By one thread: the kinds of column d of the new tokens [j0, j1) that token t sees.
+template <typename T>
+__device__ unsigned ca_new_kinds(const CaParams &p, int b, int h, int j0, int j1, int t, int d) {
+    unsigned kinds = 0;
+    for (int j = j0; j < j1; ++j)
+        if (p.mask ? p.mask[b * p.mask_b + (long long)t * p.T + j] != 0 : j <= t) kinds |= ca_kind(to_f32(ca_row<T>(p.Vd, p.vd, b, h, j)[d]));
+    return kinds;
+}
+
 // ---- joining the parts of cut units ---------------------------------------------------------------------------------
 // Block (c, y): rows join_rows y .. of the unit that entry c lists.  A row is taken by `per` warps that share its parts out, so that a row cut over the whole
 // chip (one sequence, one key head) does not wait for one part after the other; a warp asks for its first four parts' accumulators before it knows their
@@ -275,6 +295,17 @@ ca_combine_kernel(const CaParams p) {
                 for (int i = 0; i < NI; ++i) acc[i] += s_acc[w][lane + 32 * i];
         }
         if (!mine) continue;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) odd |= acc[i] != acc[i];
+        if (odd && l == l) {   // (a part's weight may be rounded to 0, too)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                unsigned kinds = 0;
+                for (int k = 0; k < parts && acc[i] != acc[i]; ++k) kinds |= ca_kind(part(k)[(size_t)row * p.D + lane + 32 * i]);
+                ca_settle(&acc[i], kinds);
+            }
+        }
         const int r = rt * p.RT + row, t = r / p.G, hq = h * p.G + r % p.G;
         T *out = ca_row<T>(p.O, p.o, b, hq, t);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -354,9 +385,26 @@ __device__ __forceinline__ void cg_scores(const float *q, const float *k, int pi
     else cg_scores<8>(q, k, pitch, s);
 }
 
+// By one thread: column d of `n` rows, the first of them row r0 of the key head, whose sums over cached rows [j0, j1) and new tokens [u0, u1) were written to the
+// output or, as parts, from `part` on.  `l`: the rows' sums of weights (NaN: a score was NaN).
+template <typename T>
+__device__ __noinline__ void cg_settle(const CaParams &p, int b, int h, int r0, int n, int j0, int j1, int u0, int u1, int d, const float *l, float *part) {
+    const T *v = ca_row<T>(p.V, p.v, b, h, 0) + d;
+    unsigned cached = 0;
+#pragma unroll 8
+    for (int j = j0; j < j1; ++j) cached |= ca_kind(to_f32(v[j * p.v.l]));
+    for (int r = 0; r < n; ++r) {
+        if (l[r] != l[r]) continue;
+        const int t = (r0 + r) / p.G;
+        const unsigned kinds = cached | ca_new_kinds<T>(p, b, h, u0, u1, t, d);
+        if (part) ca_settle(part + (size_t)r * p.D + d, kinds);
+        else ca_settle(ca_row<T>(p.O, p.o, b, h * p.G + (r0 + r) % p.G, t) + d, kinds);
+    }
+}
+
 template <typename T, int DB, bool FAST>   // DB: columns rounded up to 64, 128 or 256
 __global__ void __launch_bounds__(CG_THREADS)
-ca_generic_kernel(const CaParams p) {
+ca_generic_kernel(const __grid_constant__ CaParams p) {
     extern __shared__ __align__(16) float cg_smem[];
     __shared__ CaStart s_start;
     __shared__ float s_m[CG_ROWS], s_l[CG_ROWS], s_f[CG_ROWS];
@@ -433,7 +481,7 @@ ca_generic_kernel(const CaParams p) {
             for (int r = warp; r < rows; r += CG_THREADS / 32) {
                 const float a = ps[lane * PP + r], b = ps[(lane + 32) * PP + r], mo = s_m[r];   // (maxima of q . k, not yet scaled)
                 const float mn = fmaxf(mo, warp_max(fmaxf(a, b)));
-                const float ea = a == -INFINITY ? 0.0f : exp2f((a - mn) * p.scale_log2), eb = b == -INFINITY ? 0.0f : exp2f((b - mn) * p.scale_log2);
+                const float ea = a == -INFINITY ? -0.0f : exp2f((a - mn) * p.scale_log2), eb = b == -INFINITY ? -0.0f : exp2f((b - mn) * p.scale_log2);
                 const float sum = warp_sum(ea + eb);
                 ps[lane * PP + r] = ea;
                 ps[(lane + 32) * PP + r] = eb;
@@ -466,8 +514,8 @@ ca_generic_kernel(const CaParams p) {
                                 const float v = col + 128 * c < pitch ? vs[j * pitch + col + 128 * c] : 0.0f;
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
-                                    // a key that the row does not see weighs exactly 0; its value may be NaN
-                                    acc[c][r + k] = decltype(masked)::value && e[k] == 0.0f ? acc[c][r + k] : fmaf(e[k], v, acc[c][r + k]);
+                                    // a key that the row does not see weighs -0; its value may be NaN
+                                    acc[c][r + k] = decltype(masked)::value && __float_as_uint(e[k]) == 0x80000000u ? acc[c][r + k] : fmaf(e[k], v, acc[c][r + k]);
                             }
                         }
                     };
@@ -481,6 +529,7 @@ ca_generic_kernel(const CaParams p) {
         }
         const bool whole = w.whole(p);
         float *part = p.part + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * ca_slot_floats(p.RT, p.D);
+        bool odd[NC] = {};
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const int rr = rbase + r;
@@ -491,10 +540,16 @@ ca_generic_kernel(const CaParams p) {
             for (int c = 0; c < NC; ++c) {
                 const int d = col + 128 * c;
                 if (d >= p.D) continue;
+                odd[c] |= acc[c][r] != acc[c][r];
                 if (whole) o[d] = OutCvt<T>::one(acc[c][r] * inv);
                 else part[(size_t)rr * p.D + d] = acc[c][r];
             }
         }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (odd[c])
+                cg_settle<T>(p, w.b, w.h, row0 + rbase, min(NR, rows - rbase), w.tile(p) * CG_KEYS, min(w.n, min(end, w.ct) * CG_KEYS), max(w.tile(p) - w.ct, 0) * CG_KEYS,
+                             min(p.T, (end - w.ct) * CG_KEYS), col + 128 * c, s_l + rbase, whole ? nullptr : part + (size_t)rbase * p.D);
         if (tid < rows) {
             const float m = s_m[tid] * p.scale_log2, l = s_l[tid];
             if (!whole) {

@@ -436,6 +436,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             CN_FAIL_AT(6, !pv_done(g - 1));
             tc_fence_after();
             ct_sync();
+            bool odd = false;   // a sum is NaN
             for (int c = 0; c < nh; ++c) {
                 // lane -> column: with 64 rows in the MMA, row d of the accumulator is in lane 32 (d / 16) + d % 16
                 const int d = p.D <= 64 ? (lane < 16 ? 16 * q + lane : p.D) : 128 * c + tid;
@@ -445,7 +446,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     uint32_t o[16];
                     tmem_ld16(tl + t_o + c * N + r0, o);
                     tmem_ld_wait();
-                    if (bad && d < p.D) {   // values that are not finite, for the rows that see them
+                    if (bad && d < p.D) {   // values of new tokens that are not finite, for the rows that see them
                         for (int j = max(first - nct, 0) * CN_TK; j < min(p.T, (end - nct) * CN_TK); ++j) {
                             const float v = to_f32(ca_row<T>(p.Vd, p.vd, b, h, j)[d]);
                             if (fabsf(v) < INFINITY) continue;
@@ -461,6 +462,7 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     for (int r = 0; r < 16; ++r) {
                         if (r0 + r < R && d < p.D) {
                             const float v = __uint_as_float(o[r]);
+                            odd |= v != v;
                             if (whole) {
                                 const uint16_t y = pack_16(v * s_inv[r0 + r], F16);
                                 *reinterpret_cast<uint16_t *>(ca_row<T>(p.O, p.o, b, h * p.G + hg, t) + d) = y;
@@ -469,6 +471,20 @@ ca_narrow_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             }
                         }
                         if (++hg == p.G) { hg = 0; ++t; }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (__any_sync(0xffffffffu, odd)) {
+                for (int c = 0; c < nh; ++c) {
+                    const int d = p.D <= 64 ? (lane < 16 ? 16 * q + lane : p.D) : 128 * c + tid;
+                    const unsigned cached = ct_cached_kinds<F16>(p, b, h, first * CN_TK, min(w.n, min(end, nct) * CN_TK), d);
+                    for (int r = 0; d < p.D && r < R; ++r) {
+                        if (s_inv[r] != s_inv[r]) continue;   // (a score was NaN)
+                        const int t = r / p.G;
+                        const unsigned kinds = cached | ca_new_kinds<T>(p, b, h, max(first - nct, 0) * CN_TK, min(p.T, (end - nct) * CN_TK), t, d);
+                        if (whole) ca_settle(ca_row<T>(p.O, p.o, b, h * p.G + r % p.G, t) + d, kinds);
+                        else ca_settle(prt + (size_t)r * p.D + d, kinds);
                     }
                     __syncwarp();
                 }

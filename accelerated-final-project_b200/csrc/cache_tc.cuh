@@ -10,7 +10,8 @@
 //   warp 3        sees every V tile before the MMAs do: rows behind the cache's last are set to 0 (0 weight times NaN would be NaN); in a tile of
 //                 new tokens, which some rows see and others do not, values that are not finite are set to 0 and remembered
 //   warpgroups    a thread per row: scores into registers, the row's mask, running maximum and sum, P as 16-bit values to shared memory; at the end of a
-//                 unit O / l to the output or (O, m, l) to the workspace.  Values that warp 3 took out are added for the rows that see them.
+//                 unit O / l to the output or (O, m, l) to the workspace.  Values that warp 3 took out are added for the rows that see them, and sums that an
+//                 infinite cached value times a weight rounded to 0 made NaN are settled (the look for them costs the last call below 1.8 us).
 // The accumulator O stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 over the reference that its exponents are
 // taken against (m is that reference, so the result is exact; weights up to 2^8 stay inside fp16).  Rounding: P to the tensors' type; all else is fp32.
 // Warps of rows that do not exist only keep the hand-offs in step.  Every wait is bounded; one that expires sets the error word.
@@ -99,6 +100,12 @@ __device__ __forceinline__ float ct_max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// NaN where one of the three is NaN, else the largest of them.
+__device__ __forceinline__ float ct_max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // A pair of 16-bit values with those that are not finite set to 0.
 template <bool F16>
@@ -183,6 +190,70 @@ __device__ __forceinline__ void ct_store_rows(unsigned char *at, uint32_t (&w)[3
         unsigned char *row = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), (lane & ~3) + m));
         if (m < rows && j * 32 < bytes) *reinterpret_cast<uint4 *>(row + j * 32) = make_uint4(w[8 * m], w[8 * m + 1], w[8 * m + 2], w[8 * m + 3]);
         if (m < rows && j * 32 + 16 < bytes) *reinterpret_cast<uint4 *>(row + j * 32 + 16) = make_uint4(w[8 * m + 4], w[8 * m + 5], w[8 * m + 6], w[8 * m + 7]);
+    }
+}
+
+// By one whole warp: which of up to 32 rows, `row` those of the lanes, hold a value that is not finite.
+template <bool F16>
+__device__ __forceinline__ unsigned ct_odd_rows(const void *row, bool there, int D) {
+    bool odd = false;
+    if (there)
+        for (int d = 0; d < D; d += 8) {   // (rows are on 16 bytes, head_d is a multiple of 8)
+            const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(row) + d);
+            odd |= ct_finite<F16>(a.x) != a.x || ct_finite<F16>(a.y) != a.y || ct_finite<F16>(a.z) != a.z || ct_finite<F16>(a.w) != a.w;
+        }
+    return __ballot_sync(0xffffffffu, odd);
+}
+// By one whole warp: the kinds of the cached values of rows [j0, j1) in the lane's column d.
+template <bool F16>
+__device__ unsigned ct_cached_kinds(const CaParams &p, int b, int h, int j0, int j1, int d) {
+    using T = typename CtType<F16>::T;
+    const int lane = threadIdx.x & 31;
+    const T *v = ca_row<T>(p.V, p.v, b, h, 0);
+    unsigned kinds = 0;
+    for (int j = j0; j < j1; j += 32) {
+        if (ct_odd_rows<F16>(v + min(j + lane, j1 - 1) * p.v.l, j + lane < j1, p.D) == 0) continue;
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k)
+            if (j + k < j1 && d < p.D) kinds |= ca_kind(to_f32(v[(j + k) * p.v.l + d]));
+        if (__all_sync(0xffffffffu, d >= p.D || kinds > CA_NEG)) break;   // (NaN in every column: more rows change nothing)
+    }
+    return kinds;
+}
+
+// By one whole warp, behind the stores of a unit, or of this CTA's part of it: what values that are not finite leave in the lane's row, token `tok` (-1: no row), which
+// is at `o` of the output or `part` of a part.  `settle`: a sum of the row is NaN, and no score was; `fresh`: some of the new tokens' values, taken out of
+// the products, are not finite - they are added for the rows that see them.
+template <bool F16>
+__device__ __noinline__ void ct_odd_values(const CaParams &p, const CtSeg &w, int TK, int tok, bool settle, bool fresh, typename CtType<F16>::T *o, float *part) {
+    using T = typename CtType<F16>::T;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();   // (the warp's lanes have written each other's rows)
+    if (__any_sync(0xffffffffu, settle)) {
+        for (int c = 0; c < p.D; c += 32) {
+            const unsigned kinds = ct_cached_kinds<F16>(p, w.b, w.h, w.tile * TK, min(w.n, min(w.end, w.ct) * TK), c + lane);
+            for (int k = 0; k < min(32, p.D - c); ++k) {
+                const unsigned of = __shfl_sync(0xffffffffu, kinds, k);
+                if (settle && o) ca_settle(o + c + k, of);
+                else if (settle) ca_settle(part + c + k, of);
+            }
+        }
+    }
+    if (!fresh) return;
+    const T *vd = ca_row<T>(p.Vd, p.vd, w.b, w.h, 0);
+    const int j1 = min(p.T, (w.end - w.ct) * TK);
+    for (int j0 = max(w.tile - w.ct, 0) * TK; j0 < j1; j0 += 32) {
+        unsigned odd = ct_odd_rows<F16>(vd + min(j0 + lane, j1 - 1) * p.vd.l, j0 + lane < j1, p.D);
+        for (; odd; odd &= odd - 1) {
+            const int j = j0 + __ffs(odd) - 1;
+            if (tok < 0 || (p.mask ? p.mask[w.b * p.mask_b + (long long)tok * p.T + j] == 0 : j > tok)) continue;
+            for (int d = 0; d < p.D; ++d) {
+                const float x = to_f32(vd[j * p.vd.l + d]);
+                if (fabsf(x) < INFINITY) continue;
+                if (o) o[d] = OutCvt<T>::one(to_f32(o[d]) + x);
+                else part[d] += x;
+            }
+        }
     }
 }
 
@@ -586,13 +657,21 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                 // 32 columns of a row: as fp32, 128 bytes of a part; two of them, as 16-bit values, 128 bytes of the output.  Lanes trade pieces so that a
                 // store covers whole lines of eight rows, not 16 bytes of 32 (7 us a unit of 128 columns).
                 uint32_t v[32];
+                float nan[2] = {0.0f, 0.0f};   // NaN where a sum is (what lies behind head_d may be anything)
+                auto columns = [&](int c) {   // c to c + 31 of the accumulator
+                    tmem_ld32(to + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) nan[x] = ct_max3_nan(nan[x], __uint_as_float(v[k + 2 * x]), __uint_as_float(v[k + 2 * x + 1]));
+                };
                 if (whole) {
                     uint32_t out[32];
                     for (int c = 0; c < p.D; c += 64) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            tmem_ld32(to + c + 32 * x, v);
-                            tmem_ld_wait();
+                            columns(c + 32 * x);
 #pragma unroll
                             for (int k = 0; k < 16; ++k) out[16 * x + k] = pack_16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv, F16);
                         }
@@ -600,24 +679,13 @@ ca_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
                     }
                 } else {
                     for (int c = 0; c < p.D; c += 32) {
-                        tmem_ld32(to + c, v);
-                        tmem_ld_wait();
+                        columns(c);
                         ct_store_rows(reinterpret_cast<unsigned char *>(prt + (size_t)urow * p.D + c), v, lane, rows - (row & ~3), (p.D - c) * 4);
                     }
                 }
-                if (bad) {   // values that are not finite, for the rows that see them (the warp's lanes have written each other's rows)
-                    __syncwarp();
-                    for (int j = max(first - nct, 0) * TK; mine && j < min(p.T, (end - nct) * TK); ++j) {
-                        if (p.mask ? p.mask[w.b * p.mask_b + (long long)tok * p.T + j] == 0 : j > tok) continue;
-                        const T *vd = ca_row<T>(p.Vd, p.vd, w.b, w.h, j);
-                        for (int d = 0; d < p.D; ++d) {
-                            const float x = to_f32(vd[d]);
-                            if (fabsf(x) < INFINITY) continue;
-                            if (whole) o[d] = OutCvt<T>::one(to_f32(o[d]) + x);
-                            else prt[(size_t)urow * p.D + d] += x;
-                        }
-                    }
-                }
+                const bool settle = mine && l == l && (nan[0] != nan[0] || nan[1] != nan[1]);
+                if (bad || __any_sync(0xffffffffu, settle))
+                    ct_odd_values<F16>(p, w, TK, mine ? tok : -1, settle, bad, whole ? o : nullptr, whole ? nullptr : prt + (size_t)urow * p.D);
                 if (mine) {
                     const float m_ref = x_ref * sl2;
                     if (!whole) {

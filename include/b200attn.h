@@ -290,8 +290,8 @@ typedef struct b200attn_view {   /* a tensor [B, heads, rows, D] */
  * a prompt's next piece).  Without Kd and Vd the queries see the cache alone (cross attention to an encoder's states).
  * lse[b,h,t] = log of the sum of exp(scale * Q . K_j), fp32.  A token that sees no key has out 0 and lse -inf; so does one whose every score is -inf.  Q . K_j, and its product
  * with scale log2 e, count as infinite beyond fp32's range.  Scores, softmax and
- * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V.  A masked key and its value
- * have no effect on a row, whatever they hold. */
+ * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V.  A value that is not
+ * finite reaches every row that sees it, however small its weight; a masked key and its value have no effect on a row, whatever they hold. */
 typedef struct b200attn_attend_args {
     size_t struct_size;          /* sizeof(b200attn_attend_args) */
     b200attn_view Q, K, V;       /* [B,Hq,T,D], [B,Hkv,S,D] */

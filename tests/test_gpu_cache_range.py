@@ -65,3 +65,64 @@ def test_attend_with_large_products(pkg, cuda, path, dtype):
     """The same from large products of the tensors' own values."""
     for a in (2.0 ** 126, -2.0 ** 126):
         one_score(pkg, path, dtype, a, 1.0, 700, (700, 300))
+
+
+def with_low_keys(dtype, shape, drafts, low, seed):
+    """A problem whose queries share a direction, and cached and new keys far down it (by e^-40: nothing in fp16; by e^-300: nothing in fp32), whose values are not finite."""
+    import torch
+    from test_gpu_cache import Problem
+    _, B, Hq, Hkv, T, D = shape
+    S, lengths = (300, (300, 129)) if seed % 2 else (5000, (5000, 2))
+    p = Problem(dtype, B, Hq, Hkv, T, S, lengths, D, drafts, seed=seed)
+    p.Q[..., 0], p.K[..., 0] = 8.0, 0.0
+    if drafts != "none":
+        p.Kd[..., 0] = 0.0
+        p.Kd[:, :, T // 2] = math.nan
+    down = -low * math.sqrt(D) / 8.0
+    g = torch.Generator().manual_seed(seed)
+    for b, n in enumerate(p.length.tolist()):
+        for at, value, column, h in ((0, math.inf, 0, 0), (n // 3, -math.inf, 1, 0), (n // 2, math.nan, 2, Hkv - 1), (n - 1, math.inf, D - 1, Hkv - 1), (n // 4, math.inf, 1, 0),
+                                     (n // 5, math.inf, D // 2, 0), (n // 6, math.inf, D // 2, 0)):
+            p.V[b, h, at, column] = value
+            p.K[b, h, at, 0] = down
+    # every value of a column, and one that weighs what others do
+    p.V[0, 0, : int(p.length[0]), 5], p.V[B - 1, 0, 1, 6] = math.inf, -math.inf
+    if drafts != "none" and T > 2:
+        p.Vd[0, 0, 0, 3], p.Vd[0, 0, 1, 4], p.Vd[0, Hkv - 1, 0, 0] = math.inf, -math.inf, -math.inf
+        p.Kd[0, :, :2, 0] = down
+    return p
+
+
+@pytest.mark.parametrize("drafts", ["none", "tree"])
+@pytest.mark.parametrize("low", [0.0, 40.0, 300.0])
+@pytest.mark.parametrize("path,dtype", CASES, ids=IDS)
+def test_attend_with_cached_values_that_are_not_finite(pkg, cuda, path, dtype, low, drafts):
+    """A cached value that is infinite is so in the result, NaN where another of the other sign is seen, whatever it weighs."""
+    import cache_ref as ref
+    for seed in (60, 61):
+        p = with_low_keys(dtype, path, drafts, low, seed)
+        out, lse = pkg.cache_attend(*p.args(), flags=pkg.FLAG_FORCE_GENERIC if path[0] == "cache_generic" else 0)
+        assert pkg.last_path() == path[0]
+        want, want_lse, b_out, b_lse = ref.attend(*p.args())
+        ok, worst = ref.close(lse, want_lse, b_lse)
+        assert ok, ("lse", worst)
+        ok, worst = ref.close(out, want, b_out)
+        assert ok, ("out", worst)
+
+
+@pytest.mark.parametrize("dtype,path,T,G", [("bf16", "cache_narrow", 1, 4), ("f16", "cache_tc", 40, 2), ("f32", "cache_generic", 1, 1)])
+def test_a_cache_of_nothing_finite(pkg, cuda, dtype, path, T, G):
+    """Long caches that are NaN throughout, or infinite throughout a column: an answer, in time."""
+    import torch
+    td = getattr(torch, DT[dtype])
+    B, Hkv, S, D = 74, 2, 60000, 128
+    Q, K = torch.randn(B, Hkv * G, T, D, device="cuda").to(td), torch.zeros(B, Hkv, S, D, dtype=td, device="cuda")
+    K[:, :, : S // 2] = -1000.0
+    V = torch.zeros(B, Hkv, S, D, dtype=td, device="cuda")
+    V[0], V[1:, :, :, 7] = math.nan, -math.inf
+    n = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    out, _ = pkg.cache_attend(Q, K, V, n)
+    assert pkg.last_path() == path
+    want = torch.zeros(B, Hkv * G, T, D, device="cuda")
+    want[0], want[1:, :, :, 7] = math.nan, -math.inf
+    assert torch.equal(out.float().nan_to_num(1.0, 2.0, 3.0), want.nan_to_num(1.0, 2.0, 3.0))
