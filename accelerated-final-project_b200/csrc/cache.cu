@@ -170,6 +170,15 @@ int launch_combine(const CaParams &p, cudaStream_t st) {
     count_launches(2);   // with the kernel whose parts these are
     return B200ATTN_OK;
 }
+// CTAs of ca_generic_kernel that share the work out: as many as run at once, so that equal shares end together.  Four, three or one an SM by the registers that its
+// three widths take, and no more than fit its shared memory (two at head_d 117 to 128; three of 117 to 124 would fill it to the byte, and do not run at once).
+//   fp32, 8 x 8 heads, 4 tokens, 4096 rows, head_d 128 / 124: 97 / 115 us with two an SM, 128 / 131 with three; 2 x 16 heads of 333 tokens over 1500 rows, 128: 690, 908
+int generic_grid(const CaParams &p, const HostCall &c) {
+    const int most = p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1;
+    const size_t cta = (cg_smem_bytes(p.D) + CG_STATIC_SMEM + 127) / 128 * 128 + 1024;   // (the system keeps 1 KB per CTA)
+    const int fit = (int)(c.max_smem / cta);
+    return c.sm_count * (fit < most ? fit : most);
+}
 template <typename T, int DB, bool FAST>
 int launch_generic(const CaParams &p, const HostCall &c, cudaStream_t st) {
     const size_t smem = cg_smem_bytes(p.D);
@@ -280,7 +289,7 @@ int attend(const b200attn_attend_args *a, size_t *need) {
     CtParams ct;
     CnParams cn;
     bool narrow = narrow_shape(a, c, p, &cn), tc = !narrow && tc_shape(a, c, p, &ct);
-    share_out(p, CG_ROWS, CG_KEYS, CG_OH, c.sm_count * (p.D <= 64 ? 4 : p.D <= 128 ? 3 : 1));
+    share_out(p, CG_ROWS, CG_KEYS, CG_OH, generic_grid(p, c));
     p.uncut = narrow && cn.a.uncut;
     // the larger of the two kernels' needs: which one runs goes by the tensors' alignment, too
     size_t bytes = attend_bytes(p);

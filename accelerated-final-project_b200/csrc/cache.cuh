@@ -325,6 +325,7 @@ ca_combine_kernel(const CaParams p) {
 constexpr int CG_ROWS = 16, CG_KEYS = 64, CG_THREADS = 128;
 constexpr int CG_OH = 0;   // items in front of a unit's tiles (1: 72 us instead of 58, before the copies were asynchronous)
 __host__ __device__ inline int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
+constexpr size_t CG_STATIC_SMEM = 256;   // of a kernel below, at the most
 inline size_t cg_smem_bytes(int D) { return ((size_t)(CG_ROWS + 2 * CG_KEYS) * cg_pitch(D) + CG_KEYS * (CG_ROWS + 4)) * sizeof(float); }
 
 __device__ __forceinline__ void cg_copy16(float *dst, const void *src, bool there) {   // zeros where there is nothing to copy
