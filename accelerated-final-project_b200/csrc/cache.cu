@@ -382,7 +382,7 @@ int commit(const b200attn_commit_args *a) {
 
 template <typename T, bool FAST>
 int launch_weights(const CwParams &p, const HostCall &c, cudaStream_t st) {
-    const size_t smem = cg_smem_bytes(p.D);
+    const size_t smem = cw_smem_bytes(p.D, FAST);
     int rc = raise_smem<cw_generic_kernel<T, FAST>>(c);
     if (rc) return rc;
     CU_TRY(launch_dependent(cw_generic_kernel<T, FAST>, dim3((unsigned)((p.S + CG_KEYS - 1) / CG_KEYS), (unsigned)p.Hkv, (unsigned)p.B), CG_THREADS, smem, 1, st, p));

@@ -324,7 +324,7 @@ ca_combine_kernel(const CaParams p) {
 //   2 x 8 heads, 7 tokens, 1501 and 2999 rows cached, head_d 64, fp32 (18.5 MB): 40 us with element-wise loads, one after the other
 constexpr int CG_ROWS = 16, CG_KEYS = 64, CG_THREADS = 128;
 constexpr int CG_OH = 0;   // items in front of a unit's tiles (1: 72 us instead of 58, before the copies were asynchronous)
-__host__ __device__ inline int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
+__host__ __device__ constexpr int cg_pitch(int D) { return (((D + 3) >> 2) | 1) << 2; }   // floats: whole 16 bytes, an odd number of them
 constexpr size_t CG_STATIC_SMEM = 256;   // of a kernel below, at the most
 inline size_t cg_smem_bytes(int D) { return ((size_t)(CG_ROWS + 2 * CG_KEYS) * cg_pitch(D) + CG_KEYS * (CG_ROWS + 4)) * sizeof(float); }
 
@@ -592,6 +592,8 @@ struct CwParams {
     unsigned *err, *err_sys;
     unsigned spin_limit, wait_extra;
 };
+
+constexpr size_t cw_smem_bytes(int D, bool fast) { return (size_t)(CG_KEYS + (fast ? 2 : 1) * CG_ROWS) * cg_pitch(D) * sizeof(float); }
 
 // Block: 64 keys of a head; thread = key (two threads share a key's rows).  A key's sum is taken by its threads in the order of the rows; the next 16 rows
 // are on their way under the present ones' products (8 heads, 142 tokens, up to 303 rows, head_d 80, fp32: 44 us with each load waited for).
