@@ -1043,19 +1043,14 @@ ce_select_kernel(const CeParams p) {
     int all;
     int mine = ce_scan<CE_THREADS>(equals, s_warp, &all);
     // numbers over the CTAs in front of this one: `slot` of s_count in each, which the caller's total goes into
-    auto in_front = [&](int total, int slot, int *sum) {
+    auto in_front = [&](int total, int slot) {
         if (tid == 0) s_count[slot] = total;
         ce_cluster_sync(cl);
-        int before = 0, every = 0;
-        for (uint32_t o = 0; o < cl; ++o) {
-            const int v = cl > 1 ? ce_remote(&s_count[slot], o) : s_count[slot];
-            if (o < rank) before += v;
-            every += v;
-        }
-        if (sum) *sum = every;
+        int before = 0;
+        for (uint32_t o = 0; o < rank; ++o) before += ce_remote(&s_count[slot], o);
         return before;
     };
-    int room = need - in_front(all, 0, nullptr) - mine;
+    int room = need - in_front(all, 0) - mine;
     for (int i = w0; i < w1; ++i) {
         unsigned eq = equal[i];
         if (__popc(eq) <= room) {
@@ -1083,7 +1078,7 @@ ce_select_kernel(const CeParams p) {
         number[i] = mine;
         mine += __popc(into ? stays[i] : stays[i] & ~front(i));
     }
-    const int base = in_front(all, 1, nullptr);   // (a barrier: the numbers are there)
+    const int base = in_front(all, 1);   // (a barrier: the numbers are there)
     __syncthreads();
 #pragma unroll 4
     for (int i = warp; i < words; i += CE_THREADS / 32) {
@@ -1107,7 +1102,7 @@ ce_select_kernel(const CeParams p) {
         number[i] = mine;
         mine += __popc(~stays[i] & front(i));
     }
-    const int holes = in_front(all, 2, nullptr);   // (a barrier: all lists are there)
+    const int holes = in_front(all, 2);   // (a barrier: all lists are there)
     __syncthreads();
     for (int i = warp; i < words; i += CE_THREADS / 32) {
         const unsigned f = front(i), free = ~stays[i] & f;
