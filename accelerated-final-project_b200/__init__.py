@@ -184,6 +184,13 @@ def check(status):
         raise B200AttnError(status, lib().b200attn_last_error().decode())
 
 
+_INVALID_ARG = 1
+
+
+def _refuse(message):
+    raise B200AttnError(_INVALID_ARG, message)
+
+
 def forward(Q, K, V, out=None, pe=PE_NONE, rotary_dim=0, rope_base=0.0, cos_cache=None, sin_cache=None,
             stream=None, flags=0):
     """Attention forward on torch CUDA tensors Q [B,H,Lq,D], K/V [B,H,Lk,D] (float32 or bfloat16,
@@ -253,28 +260,28 @@ def forward_host(Q, K, V, out, pe=PE_NONE, rotary_dim=0, rope_base=0.0, flags=0)
 
 
 def rope_k(X, out=None, pairing=PE_ROPE_INTERLEAVED, rotary_dim=0, rope_base=0.0, pos0=0, cos_cache=None, sin_cache=None, stream=None):
-    """RoPE(X) for a torch CUDA tensor [B,H,L,D] through b200attn_rope_k.  Returns `out`."""
-    import torch
+    """RoPE(X) for a torch CUDA tensor [B,H,L,D] (float32, bfloat16 or float16, contiguous) through b200attn_rope_k.  Returns `out`."""
+    torch = _torch or _with_torch()
+    if X.dim() != 4 or X.dtype not in _DTYPES or not X.is_cuda or not X.is_contiguous():
+        _refuse("X must be a contiguous 4-dimensional float32, bfloat16 or float16 CUDA tensor [B, heads, rows, D]")
     B, H, L, D = X.shape
     if out is None:
         out = torch.empty_like(X)
+    elif out.shape != X.shape or out.dtype is not X.dtype or out.device != X.device or not out.is_contiguous():
+        _refuse(f"out must be a contiguous {X.dtype} tensor of shape {tuple(X.shape)} on {X.device}")
+    for c in (cos_cache, sin_cache):
+        if c is not None and (c.dtype is not torch.float32 or c.device != X.device or not c.is_contiguous() or c.numel() < (pos0 + L) * (rotary_dim or D)):
+            _refuse(f"cos_cache and sin_cache must be contiguous float32 tensors [{pos0 + L}, {rotary_dim or D}] on {X.device}")
     if stream is None:
         stream = torch.cuda.current_stream(X.device).cuda_stream
     with torch.cuda.device(X.device):
-        check(lib().b200attn_rope_k(X.data_ptr(), out.data_ptr(), B, H, L, D, F32 if X.dtype == torch.float32 else BF16, pairing, rotary_dim,
+        check(lib().b200attn_rope_k(X.data_ptr(), out.data_ptr(), B, H, L, D, _DTYPES[X.dtype], pairing, rotary_dim,
                                     rope_base, pos0, cos_cache.data_ptr() if cos_cache is not None else None,
                                     sin_cache.data_ptr() if sin_cache is not None else None, stream))
     return out
 
 
 # ---- a key/value cache ----------------------------------------------------------------------------------------------
-
-_INVALID_ARG = 1
-
-
-def _refuse(message):
-    raise B200AttnError(_INVALID_ARG, message)
-
 
 # (a short call is bound by these functions, as above: 22 us of which the two launches take 5, one token over 777 cached rows, with the checks
 # spread over more attribute look-ups; shapes are compared as tuples, and what a function has allocated itself is not checked)

@@ -8,3 +8,10 @@ from test_cache import attend_args, status, weights_args
 def test_a_scale_that_overflows_in_units_of_log2_e_is_refused(pkg, name, args):
     rc, msg = status(pkg, name, args(pkg, scale=2.4e38))   # times log2 e: beyond fp32
     assert rc == 1 and b"scale" in msg, msg
+
+
+def test_rope_k_refuses_what_it_would_misread(pkg):
+    import torch
+    for X in (torch.zeros(1, 2, 3, 8), torch.zeros(2, 3, 8), torch.zeros(1, 2, 3, 8, dtype=torch.float64), torch.zeros(1, 3, 2, 8).transpose(1, 2)):
+        with pytest.raises(pkg.B200AttnError):
+            pkg.rope_k(X)
