@@ -20,7 +20,7 @@ def sources():
 
 
 def deps():
-    return sources() + sorted(glob.glob(os.path.join(HERE, "csrc", "*.cuh"))) + \
+    return sources() + sorted(glob.glob(os.path.join(HERE, "csrc", "*.cuh"))) + sorted(glob.glob(os.path.join(HERE, "csrc", "*.h"))) + \
         sorted(glob.glob(os.path.join(HERE, "..", "include", "*.h")))
 
 
