@@ -407,6 +407,8 @@ def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, ne
         _refuse("Kd must be [B, heads, new tokens, D] and accepted [B, most accepted tokens]")
     T, dtype, i32 = Kd.shape[2], K.dtype, torch.int32
     A = 0 if accepted is None else accepted.shape[1]
+    if accepted is not None and A == 0:   # (its address would be that of no list)
+        _refuse("accepted must have room for one token of a sequence at least; -1 names none")
     n = _dense(length, "length", (B,), i32, dev)
     if n == 0:
         _refuse("length must be given")
@@ -435,6 +437,8 @@ def cache_weights(Q, K, length, lse, weights, accepted=None, scale=0.0, stream=N
         _refuse("Q must be [B, heads, new tokens, D] and accepted [B, most accepted tokens]")
     Hq, T, dtype = Q.shape[1], Q.shape[2], K.dtype
     A = 0 if accepted is None else accepted.shape[1]
+    if accepted is not None and A == 0:   # (its address would be that of no list)
+        _refuse("accepted must have room for one token of a sequence at least; -1 names none")
     stream = torch._C._cuda_getCurrentRawStream(dev)
     if length is None or lse is None or weights is None:
         _refuse("length, lse and weights must be given")

@@ -110,3 +110,16 @@ def test_unaligned_views_go_to_the_cuda_cores(pkg, cuda):
     p.V = flat[1:].view(p.V.shape)
     check_attend(pkg, p)
     assert pkg.last_path() == "cache_generic"
+
+
+def test_a_list_without_entries_is_refused(pkg, cuda):
+    """Not taken for no list, which accepts every token."""
+    import torch
+    p = Problem("bf16", 2, 8, 2, 5, 300, (100, 41), 128, "chain", seed=74)
+    w, lse = torch.zeros(2, 2, 300, device="cuda"), torch.zeros(2, 8, 5, device="cuda")
+    none = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    K = p.K.clone()
+    for call in (lambda: pkg.cache_commit(p.K, p.V, p.length, p.Kd, p.Vd, accepted=none, weights=w), lambda: pkg.cache_weights(p.Q, p.K, p.length, lse, w, accepted=none)):
+        with pytest.raises(pkg.B200AttnError):
+            call()
+    assert ref.same(p.K, K) and float(w.abs().sum()) == 0
