@@ -475,6 +475,8 @@ def cache_evict(K, V, length, weights, keep, sink=0, recent=0, pos=None, next_po
         if Ko.dim() != 4 or Wo is None or (Po is None) != (pos is None):
             _refuse("`into` must be (K, V, weights, pos), with pos where this cache has one")
         So = Ko.shape[2]
+        if So == 0:   # (its addresses would be those of no other cache)
+            _refuse("`into` must have rows")
         o_shape = (B, Hkv, So, D)
         target = _view(Ko, "K of `into`", o_shape, dtype, dev) + _view(Vo, "V of `into`", o_shape, dtype, dev) + (
             _dense(Wo, "weights of `into`", (B, Hkv, So), f32, dev), _dense(Po, "pos of `into`", (B, Hkv, So), i32, dev))

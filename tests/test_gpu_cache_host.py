@@ -123,3 +123,16 @@ def test_a_list_without_entries_is_refused(pkg, cuda):
         with pytest.raises(pkg.B200AttnError):
             call()
     assert ref.same(p.K, K) and float(w.abs().sum()) == 0
+
+
+def test_a_cache_without_rows_to_evict_into_is_refused(pkg, cuda):
+    """Not taken for no other cache, which evicts in place."""
+    import torch
+    K, V, w, pos = eviction(2, 2, 300, 64, "bf16", 75, "plain")
+    before = [t.clone() for t in (K, V, w, pos)]
+    n = torch.tensor([300, 120], dtype=torch.int32, device="cuda")
+    for at, nxt in ((pos, n), (None, None)):
+        into = (K[:, :, :0], V[:, :, :0], w[:, :, :0].contiguous(), pos[:, :, :0].contiguous() if at is not None else None)
+        with pytest.raises(pkg.B200AttnError):
+            pkg.cache_evict(K, V, n, w, 100, pos=at, next_pos=nxt, into=into)
+    assert all(ref.same(x, y) for x, y in zip((K, V, w, pos), before))
