@@ -83,7 +83,13 @@ def _packer(cls):
     packed = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
     size = C.sizeof(cls)
     tail = bytes(size - packed.size)   # the structure's own alignment
-    return lambda *values: packed.pack(size, *values) + tail
+
+    def pack(*values):
+        try:
+            return packed.pack(size, *values) + tail
+        except (struct.error, OverflowError) as e:   # a number that its field does not hold
+            _refuse(f"{cls.__name__}: {e}")
+    return pack
 
 
 _pack_attend, _pack_commit, _pack_weights, _pack_evict = (_packer(c) for c in (AttendArgs, CommitArgs, WeightsArgs, EvictArgs))

@@ -15,3 +15,11 @@ def test_rope_k_refuses_what_it_would_misread(pkg):
     for X in (torch.zeros(1, 2, 3, 8), torch.zeros(2, 3, 8), torch.zeros(1, 2, 3, 8, dtype=torch.float64), torch.zeros(1, 3, 2, 8).transpose(1, 2)):
         with pytest.raises(pkg.B200AttnError):
             pkg.rope_k(X)
+
+
+@pytest.mark.parametrize("cls,pack,field,value", [("AttendArgs", "_pack_attend", "scale", 1e39), ("EvictArgs", "_pack_evict", "keep", 1 << 31), ("WeightsArgs", "_pack_weights", "flags", -1),
+                                                  ("CommitArgs", "_pack_commit", "max_accepted", 0.5)])
+def test_numbers_that_a_field_does_not_hold_are_refused(pkg, cls, pack, field, value):
+    names = [n for n, _ in getattr(pkg, cls)._fields_][1:]
+    with pytest.raises(pkg.B200AttnError):
+        getattr(pkg, pack)(*(value if n == field else 0 for n in names))
