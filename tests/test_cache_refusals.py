@@ -17,9 +17,16 @@ def test_rope_k_refuses_what_it_would_misread(pkg):
             pkg.rope_k(X)
 
 
-@pytest.mark.parametrize("cls,pack,field,value", [("AttendArgs", "_pack_attend", "scale", 1e39), ("EvictArgs", "_pack_evict", "keep", 1 << 31), ("WeightsArgs", "_pack_weights", "flags", -1),
+@pytest.mark.parametrize("cls,pack,field,value", [("AttendArgs", "_pack_attend", "capacity", 1 << 31), ("EvictArgs", "_pack_evict", "keep", 1 << 31), ("WeightsArgs", "_pack_weights", "flags", -1),
                                                   ("CommitArgs", "_pack_commit", "max_accepted", 0.5)])
 def test_numbers_that_a_field_does_not_hold_are_refused(pkg, cls, pack, field, value):
     names = [n for n, _ in getattr(pkg, cls)._fields_][1:]
     with pytest.raises(pkg.B200AttnError):
         getattr(pkg, pack)(*(value if n == field else 0 for n in names))
+
+
+def test_a_scale_beyond_fp32_arrives_as_infinity_and_is_refused(pkg):
+    names = [n for n, _ in pkg.AttendArgs._fields_][1:]
+    a = attend_args(pkg)
+    packed = pkg._pack_attend(*((1e39 if n == "scale" else getattr(a, n) or 0) for n in names))
+    assert pkg.lib().b200attn_cache_attend(packed) == 1 and b"scale" in pkg.lib().b200attn_last_error()
