@@ -403,7 +403,7 @@ def cache_attend(Q, K, V, length, Kd=None, Vd=None, mask=None, scale=0.0, out=No
 def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, next_pos=None, stream=None, flags=0):
     """The accepted ones of T new tokens (accepted [B, A] int32, padded with -1; None: all) become rows of the cache from row length[b] on:
     K, V [B, Hkv, S, D] are written from Kd, Vd [B, Hkv, T, D], weights [B, Hkv, S] with 0, pos [B, Hkv, S] with next_pos[b] + i.  Returns the new
-    lengths [B] (int32); `length` stays (b200attn_cache_commit)."""
+    lengths [B] (int32); `length` stays (b200attn_cache_commit).  Tokens that the cache has no room for are dropped: see the new lengths."""
     torch, dev, k_shape = _cache_shape(K)
     B, Hkv, S, D = k_shape
     if stream is not None and (at := _elsewhere(stream, dev)) is not None:
@@ -432,8 +432,8 @@ def cache_commit(K, V, length, Kd, Vd, accepted=None, weights=None, pos=None, ne
 
 def cache_weights(Q, K, length, lse, weights, accepted=None, scale=0.0, stream=None, flags=0):
     """Adds to weights [B, Hkv, S] the attention weight that each cached row had from the accepted tokens, which are the cache's last rows by now:
-    Q [B, Hq, T, D] and lse [B, Hq, T] are those of the cache_attend call, `length` and `accepted` those after and of cache_commit.  Returns
-    `weights` (b200attn_cache_weights)."""
+    Q [B, Hq, T, D] and lse [B, Hq, T] are those of the cache_attend call, `length` and `accepted` those after and of cache_commit (where that had no
+    room for all, a list that ends in front of those it dropped).  Returns `weights` (b200attn_cache_weights)."""
     torch, dev, k_shape = _cache_shape(K)
     B, Hkv, S, D = k_shape
     if stream is not None and (at := _elsewhere(stream, dev)) is not None:

@@ -849,8 +849,8 @@ __device__ __forceinline__ void ce_move_rows(const CeParams &p, int b, int h, in
 //   into another cache: the numbers of the rows that stay are their new places.  In place: the kept rows from m on are listed by their number, and the i-th
 //   freed row below m takes the i-th of them, from the list of the CTA that has it.
 // Where few rows leave, in place, they are picked one after the other instead: a reduction over the block each.
-// Bound by latency: three passes over shared memory and some ten barriers; so a cluster's CTAs have 1024 threads (512: 48 us instead of 37 for 4 x 8 heads, up to 32768 rows), one that
-// shares its SM 512.
+// Bound by latency: three passes over shared memory and some ten barriers; so a cluster's CTAs have 1024 threads (512: 48 us instead of 37 for 4 x 8 heads, up to 32768 rows), one on its
+// own 512, of which two share an SM up to some 10000 rows.  Beyond 24896 rows a CTA's ranks are not kept but read anew in each pass.
 //   32 sequences x 8 heads, up to 4102 rows: 22 us with 1024 threads that read weights and positions anew in each pass, 19 with the ranks in shared memory, 23
 //   with two bits a round by counting; 4 x 8 heads, up to 32768 rows: 91, 33
 template <typename P, int CE_THREADS>

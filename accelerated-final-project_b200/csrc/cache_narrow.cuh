@@ -28,7 +28,8 @@ struct CnParams {
 constexpr int CN_THREADS = 256, CN_TK = 128;
 // Tiles that a cache's capacity and the new tokens may have for its units not to be cut, so that nothing is joined by a second launch: more where the units fill the
 // SMs by themselves.  Cut / not, one token, 32 / 8 heads of 128: one sequence of 2, 4, 7 tiles 10.5 / 9.8, 10.6 / 11.8, 10.8 / 14.8 us (and 4 us of the host's time
-// less); 16 sequences of 4, 9, 16 tiles 17 / 13, 22 / 18, 32 / 29; 64 of 4, 7, 9, 12 tiles 45 / 39, 53 / 52, 60 / 61, 72 / 76.
+// less); 16 sequences of 4, 9, 16 tiles 17 / 13, 22 / 18, 32 / 29; 64 of 4, 7, 9, 12 tiles 45 / 39, 53 / 52, 60 / 61, 72 / 76.  The second line is where many units
+// an SM break even; 16 sequences, a unit an SM, would gain beyond it.  It goes by the capacity, as the lengths are not known on the host.
 constexpr int CN_UNCUT_FEW = 4, CN_UNCUT_MANY = 8;
 constexpr int CN_OH = 1;   // a unit's beginning and end, in tiles (0 / 1 / 3: 184.4 / 182.9 / 186.4 us for the call above)
 constexpr uint32_t CN_GROUP = CN_TK * 128u;   // 128 keys x 64 columns

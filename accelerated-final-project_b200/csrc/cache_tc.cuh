@@ -2,9 +2,8 @@
 // heads a key head, 16-byte aligned rows.  The formulas and the sharing-out are those of cache.cuh.
 //
 // Rows (token t, query head g of the group: row t G + g) are the lanes of tensor memory, so the query heads that share a key head and the tokens of a
-// tree share every key tile: a tile of K and V is read once for up to 128 rows (ca_tc_kernel<1, ..>) or 256 (<2, ..>), and with one token and
-// four heads the MMAs compute 124 rows that nobody looks at - they are free: a tile of 128 keys (64 KB) takes 1.5 us from HBM at a 148th of its rate and
-// 0.55 us on the tensor cores.
+// tree share every key tile: a tile of K and V is read once for up to 128 rows (ca_tc_kernel<1, ..>) or 256 (<2, ..>).  The MMAs compute 128 rows whether
+// they exist or not, which takes time and power where few do: up to 64 rows a key head go to cache_narrow.cuh, with keys as the lanes.
 //   warp 0        one thread requests Q, K and V tiles by TMA through a ring of stages, in the order K_0 | K_1 V_0 | K_2 V_1 | ...
 //   warps 1, 2    one thread per row tile issues the MMAs: S = Q K^T, then O += P V once P is there
 //   warp 3        sees every V tile before the MMAs do: rows behind the cache's last are set to 0 (0 weight times NaN would be NaN); in a tile of
@@ -13,7 +12,8 @@
 //                 unit O / l to the output or (O, m, l) to the workspace.  Values that warp 3 took out are added for the rows that see them, and sums that an
 //                 infinite cached value times a weight rounded to 0 made NaN are settled (the look for them costs the last call below 1.8 us).
 // The accumulator O stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 over the reference that its exponents are
-// taken against (m is that reference, so the result is exact; weights up to 2^8 stay inside fp16).  Rounding: P to the tensors' type; all else is fp32.
+// taken against (m is that reference, so the result is exact; weights up to 2^8 stay inside fp16).  Rounding: P to the tensors' type, since the MMA takes both
+// operands in one 16-bit type and two products of P's halves would double its time; its error is of the size of the result's own rounding.  All else is fp32.
 // Warps of rows that do not exist only keep the hand-offs in step.  Every wait is bounded; one that expires sets the error word.
 // Bound by the row threads' chain per tile - scores from tensor memory, maximum, 128 exponentials, weights to shared memory: 4.0 thousand clocks where the MMAs of two
 // row tiles take 2.0:  8 sequences of 48 drafts, 32 / 8 heads of 128, 1000 to 32768 rows, bf16 157 us (185 back to back, power cap); 1000 tokens behind 2000
@@ -28,7 +28,9 @@ namespace b200attn {
 
 constexpr int CT_MAX_STAGES = 8;
 // A unit's beginning and end (Q, the first tile without another under it, the epilogue), in tiles.  0 / 4 / 6: 8 sequences of 48 drafts, 1000 to 32768 rows,
-// 218 / 168 / 167 us; cross attention of 333 tokens to 100 to 1500 rows 87 / 60 / 63; 1000 tokens behind 2000 and 7001 rows 235 / 224 / 227.
+// 218 / 168 / 167 us; cross attention of 333 tokens to 100 to 1500 rows 87 / 60 / 63; 1000 tokens behind 2000 and 7001 rows 235 / 224 / 227.  With tiles of 64 keys, 2 /
+// 4 / 8, head_d 256, 16 / 4 heads: 8 x 48 drafts, 1000 to 16384 rows 102 / 101 / 100 us; 1000 tokens behind 2000 and 7001 rows 205 / 203 / 199; 8 x 333 tokens, 16
+// heads, to 100 to 1500 rows 78 / 78 / 79; the drafts at head_d 192 86 / 83 / 83.
 constexpr int CT_OH = 4;
 constexpr float CT_RESCALE_LOG2 = 8.0f;
 

@@ -191,7 +191,7 @@ const char *b200attn_last_error(void);
  * cluster pipeline) or "tc_decode" (bf16, up to 64 queries against a long K/V: key splits on the tensor cores
  * plus a combine kernel).  b200attn_cache_attend and b200attn_cache_weights name theirs, too: "cache_narrow" (16 bit, up to 64 rows a
  * key head: keys as the lanes of tensor memory), "cache_tc" (16 bit, tensor cores) and "cache_generic" (CUDA cores: fp32, head_d that is not a multiple of
- * 8, rows that do not begin on 16 bytes). */
+ * 8, rows that do not begin on 16 bytes, a stride of 0 over more than one sequence, head or row, more than 128 query heads a key head). */
 const char *b200attn_last_path(void);
 
 /* Number of kernel launches issued by this library in this process so far. */
@@ -276,7 +276,7 @@ const char *b200attn_static_last_error(void);
  *
  * Common to all four.  They have no counterpart in the reference.  Tensors are views: the last dimension (D) is contiguous, the others have
  * strides in elements, so a projection's output [B,T,heads,D] is passed as it is; pointers are aligned to the element size.  The
- * other arrays are dense.  The work is enqueued on `stream` and waited for unless B200ATTN_FLAG_ASYNC is set.  Values that only the device
+ * other arrays are dense.  What a call writes overlaps none of its other arguments.  The work is enqueued on `stream` and waited for unless B200ATTN_FLAG_ASYNC is set.  Values that only the device
  * knows cannot be refused by the host: a length outside [0, capacity] counts as the nearer of the two; rows behind the last valid one are
  * neither read to any effect (whatever they hold, NaN included) nor written.  A capacity is at most 2^30 rows.  Calls that share no tensors may be made at the same time from several threads and streams when each
  * has a workspace of its own. */
@@ -290,7 +290,8 @@ typedef struct b200attn_view {   /* a tensor [B, heads, rows, D] */
  * a prompt's next piece).  Without Kd and Vd the queries see the cache alone (cross attention to an encoder's states).
  * lse[b,h,t] = log of the sum of exp(scale * Q . K_j), fp32.  A token that sees no key has out 0 and lse -inf; so does one whose every score is -inf.  Q . K_j, and its product
  * with scale log2 e, count as infinite beyond fp32's range.  Scores, softmax and
- * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V.  A value that is not
+ * accumulators are fp32; on the tensor cores (16-bit types) the weights are rounded to the tensors' type for the product with V, at every
+ * head_d (b200attn_forward_ex keeps them in fp32 where head_d is a multiple of 8 but none of 64).  A value that is not
  * finite reaches every row that sees it, however small its weight; a masked key and its value have no effect on a row, whatever they hold. */
 typedef struct b200attn_attend_args {
     size_t struct_size;          /* sizeof(b200attn_attend_args) */
@@ -317,7 +318,8 @@ size_t b200attn_cache_attend_workspace(const b200attn_attend_args *args);
 
 /* The i-th accepted token of sequence b, the new token t = accepted[b,i], becomes row length[b] + i: K and V of that row are copied from Kd and Vd
  * [B,Hkv,T,D], weights[b,h,row] = 0, pos[b,h,row] = next_pos[b] + i.  The list ends at the first index outside [0, T) (pad it with -1) or after
- * `max_accepted` entries; accepted NULL takes all T tokens in order.  Tokens that the cache has no room for are dropped.
+ * `max_accepted` entries; accepted NULL takes all T tokens in order.  Tokens that the cache has no room for are dropped;
+ * length_out tells it, and a list that is used again (b200attn_cache_weights) has to end in front of them.
  * length_out[b] = length[b] + the number of rows written; the caches of all layers can be given the same `length`. */
 typedef struct b200attn_commit_args {
     size_t struct_size;
@@ -338,7 +340,8 @@ int b200attn_cache_commit(const b200attn_commit_args *args);
 
 /* weights[b,g,j] += sum over the accepted tokens and the query heads h of key head g of exp(scale * Q[b,h,t] . K[b,g,j] - lse[b,h,t]), where the i-th of
  * the n accepted tokens of a sequence sees the rows j <= length[b] - n + i: the accepted tokens are the cache's last n rows (this call comes
- * after the commit, `length` is the length after it), and Q and lse are those of the b200attn_cache_attend call before.  Sums in fp32, in an order that
+ * after the commit, `length` is the length after it), and Q and lse are those of the b200attn_cache_attend call before; a weight is as exact as its lse, an
+ * fp32 number.  Sums in fp32, in an order that
  * does not change from call to call.  `accepted` as above; a list longer than length[b] counts for its first length[b] entries; a token whose
  * lse is -inf (it saw nothing) gave no weight. */
 typedef struct b200attn_weights_args {
@@ -358,7 +361,8 @@ int b200attn_cache_weights(const b200attn_weights_args *args);
 
 /* Leaves m = min(length[b], keep) rows in each head of the cache: first the protected ones, then those of largest weight, among equals the
  * lowest row (NaN is the least weight of all).  Protected are the tokens of the first `sink` positions and of the last `recent` ones: pos < sink or
- * pos >= next_pos[b] - recent, with the row's index for pos and length[b] for next_pos where those are NULL.
+ * pos >= next_pos[b] - recent, with the row's index for pos and length[b] for next_pos where those are NULL (right while
+ * nothing has been evicted).
  * In place (K_out.ptr NULL) a row that stays does not move if its index is below m; the other kept rows fill the freed rows, both taken in
  * order, so that a step's eviction moves few rows: rows do not stay in the order of their tokens, `pos` tells it.  Into another cache (K_out,
  * V_out, weights_out and, with pos, pos_out given, capacity_out >= min(keep, capacity), no overlap) the kept rows are copied in order and this cache stays as it is.
